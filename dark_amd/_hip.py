@@ -20,7 +20,7 @@ LIB_PATH = os.environ.get("DARK_HIP_LIB") or os.path.join(_HERE, "libdark_hip.so
 DARK_OK, DARK_ERR_ARG, DARK_ERR_HIP, DARK_ERR_UNSUPPORTED = 0, 1, 2, 3
 DARK_F32, DARK_BF16 = 0, 1
 CONF_PROB, CONF_MARGIN, CONF_NEG_ENTROPY = 0, 1, 2
-ABI_VERSION = 7
+ABI_VERSION = 8
 SHARD_PART_BYTES = 280
 SAMPLE_LDS_MAX_V = 32768   # DARK_SAMPLE_LDS_MAX_V: larger vocabularies sample from a registered row workspace
 
@@ -50,6 +50,36 @@ class Gpt2Desc(C.Structure):
                 ("wpe", C.c_void_p),
                 ("lnf_w", C.c_void_p), ("lnf_b", C.c_void_p), ("ident_cos", C.c_void_p), ("ident_sin", C.c_void_p),
                 ("layers", C.POINTER(Gpt2LayerWeights))]
+
+
+class PagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("slot_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("dtype", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("reserved", C.c_int32)]
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_w", "k_w", "rope_cos", "rope_sin", "pos")] +
+                [(n, C.c_int64) for n in ("q_ts", "q_hs", "k_ts", "k_hs", "qo_ts", "qo_hs", "ko_ts", "ko_hs")] +
+                [(n, C.c_int32) for n in ("dtype", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "max_pos")] +
+                [("eps", C.c_float), ("reserved", C.c_int32)])
+
+
+class KVAppendArgs(C.Structure):
+    _fields_ = ([("kv", PagedKV)] +
+                [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "q_w", "k_w", "rope_cos", "rope_sin", "pos", "slots")] +
+                [(n, C.c_int64) for n in ("q_ts", "q_hs", "k_ts", "k_hs", "v_ts", "v_hs", "qo_ts", "qo_hs")] +
+                [(n, C.c_int32) for n in ("n_tokens", "n_heads", "max_pos")] + [("eps", C.c_float)])
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = ([("kv", PagedKV)] +
+                [(n, C.c_void_p) for n in ("q", "out", "lse", "block_table", "cu_q", "kv_len", "q_index", "key_mask",
+                                           "workspace")] +
+                [(n, C.c_int64) for n in ("workspace_bytes", "q_ts", "q_hs", "o_ts", "o_hs", "table_stride",
+                                          "mask_stride")] +
+                [(n, C.c_int32) for n in ("n_tokens", "n_heads", "n_seqs", "table_width", "max_q", "max_kv", "causal")] +
+                [("scale", C.c_float)])
 
 
 # name -> (restype, argtypes); every symbol include/dark_hip.h declares
@@ -158,6 +188,11 @@ SIGNATURES = {
                                          C.c_void_p, C.c_int64, C.c_void_p]),
     "dark_dbg_layernorm": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                      C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p]),
+    # (the argument structs go as the bytes of their fields: kv_cache.py packs them, one call converts one pointer)
+    "dark_qk_norm_rope": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "dark_kv_append": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "dark_paged_attention_workspace_bytes": (C.c_size_t, [C.c_void_p]),
+    "dark_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
     "dark_dbg_embed": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                  C.c_void_p]),
 }

@@ -1,0 +1,245 @@
+// Per-head RMS norm + position rotation of queries and keys, and the placement of new tokens in the pages of a
+// key / value cache.  The three jobs are one kernel: a token's rows (heads of q, k and v) are read once, normed and
+// rotated in fp32 registers and stored once, wherever they belong.
+//
+// Bound by HBM: 2 * (heads read) * head_dim elements a token against ~8 flops an element.  One wave per token: a row is
+// held by LPR lanes, lane c of them with the 16 bytes at chunk c of the row's first half and of its second half -- the
+// two elements of every rotated pair in one lane -- so the 64 / LPR rows of one pass need no exchange but the norm's sum
+// (log2(LPR) xor-shuffles), and the token's cos / sin, read once, serve all its heads.
+#include "common.h"
+
+namespace dark {
+
+struct RowsArgs {
+  // role 0 = q -> q_out, 1 = k -> k_out / pages, 2 = v -> pages
+  const void* src[3];
+  void* dst[3];
+  const float* w[2];
+  const float *cosT, *sinT;
+  const int32_t* pos;
+  const int64_t* slots;       // null: dst[1] is a plain [T, heads, HD] output
+  int64_t src_ts[3], src_hs[3], dst_ts[3], dst_hs[3];
+  int64_t page_stride, n_slots;
+  int32_t T, h_end[3];        // rows [0, h_end[0]) are q heads, then k heads, then v heads
+  int32_t max_pos, page_log2;
+  float eps;
+};
+
+template <typename T> struct RowVec;
+template <> struct RowVec<bf16_t> {
+  static constexpr int N = 8;
+  typedef bf16x8 raw;
+  __device__ static __forceinline__ void up(const raw& r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)r[i];
+  }
+  __device__ static __forceinline__ raw down(const float (&f)[8]) {
+    raw r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (bf16_t)f[i];
+    return r;
+  }
+};
+template <> struct RowVec<float> {
+  static constexpr int N = 4;
+  typedef f32x4 raw;
+  __device__ static __forceinline__ void up(const raw& r, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = r[i];
+  }
+  __device__ static __forceinline__ raw down(const float (&f)[4]) { return (raw){f[0], f[1], f[2], f[3]}; }
+};
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
+  constexpr int N = RowVec<T>::N, HALF = HD / 2, CH = HALF / N;         // CH lanes hold a row
+  constexpr int LPR = CH <= 4 ? 4 : CH <= 8 ? 8 : 16, RPP = 64 / LPR;   // lanes a row is given, rows of one pass
+  typedef typename RowVec<T>::raw raw;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= a.T) return;
+  const int c = lane & (LPR - 1), r0 = lane / LPR;
+  const bool on = c < CH;
+  const int cc = on ? c : 0;
+  float cs[N], sn[N], wq[2 * N], wk[2 * N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
+  if (a.cosT) {
+    int p = a.pos[t];
+    p = p < 0 ? 0 : (p >= a.max_pos ? a.max_pos - 1 : p);
+    const float* cp = a.cosT + (int64_t)p * HALF + cc * N;
+    const float* sp = a.sinT + (int64_t)p * HALF + cc * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { cs[i] = cp[i]; sn[i] = sp[i]; }
+  }
+  int64_t slot = -1;
+  if (a.slots) {
+    slot = a.slots[t];
+    if (slot >= a.n_slots) slot = -1;
+  }
+  const int64_t in_cache = slot < 0 ? 0 : (slot >> a.page_log2) * a.page_stride;
+  const int64_t in_page = slot < 0 ? 0 : slot & (((int64_t)1 << a.page_log2) - 1);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    wq[i] = a.w[0] ? a.w[0][cc * N + i] : 1.f;
+    wq[N + i] = a.w[0] ? a.w[0][HALF + cc * N + i] : 1.f;
+    wk[i] = a.w[1] ? a.w[1][cc * N + i] : 1.f;
+    wk[N + i] = a.w[1] ? a.w[1][HALF + cc * N + i] : 1.f;
+  }
+  const int rows = a.h_end[2];
+  for (int r = r0; r < rows + r0; r += RPP) {   // (the same trip count for every lane: the shuffles need whole groups)
+    const bool live = r < rows;
+    const int role = !live ? 0 : (r < a.h_end[0] ? 0 : r < a.h_end[1] ? 1 : 2);
+    const int h = r - (role == 0 ? 0 : a.h_end[role - 1]);
+    raw x1 = {}, x2 = {};
+    if (live && on) {
+      const T* s = (const T*)a.src[role] + t * a.src_ts[role] + h * a.src_hs[role] + c * N;
+      x1 = *(const raw*)s;
+      x2 = *(const raw*)(s + HALF);
+    }
+    raw y1 = x1, y2 = x2;
+    if (role < 2) {
+      float f1[N], f2[N], o1[N], o2[N];
+      RowVec<T>::up(x1, f1);
+      RowVec<T>::up(x2, f2);
+      if (a.w[role]) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss += f1[i] * f1[i] + f2[i] * f2[i];
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          f1[i] *= inv * (role ? wk[i] : wq[i]);
+          f2[i] *= inv * (role ? wk[N + i] : wq[N + i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        o1[i] = f1[i] * cs[i] - f2[i] * sn[i];
+        o2[i] = f2[i] * cs[i] + f1[i] * sn[i];
+      }
+      y1 = RowVec<T>::down(o1);
+      y2 = RowVec<T>::down(o2);
+    }
+    const bool paged = role > 0 && a.slots;
+    if (live && on && (!paged || slot >= 0)) {
+      T* d = (T*)a.dst[role] + (paged ? in_cache + in_page * a.dst_ts[role] : t * a.dst_ts[role]) + h * a.dst_hs[role] + c * N;
+      *(raw*)d = y1;
+      *(raw*)(d + HALF) = y2;
+    }
+  }
+}
+
+static bool aligned16(const void* p, int64_t s0, int64_t s1, int es) {
+  return ((uintptr_t)p & 15) == 0 && (s0 * es) % 16 == 0 && (s1 * es) % 16 == 0;
+}
+
+// a stream of another device than the current one would run there on this device's pointers
+int check_stream_device(hipStream_t st) {
+  if (st == nullptr) return DARK_OK;
+  int cur = 0;
+  hipDevice_t sdev = 0;
+  DARK_CHECK_HIP(hipGetDevice(&cur));
+  DARK_CHECK_HIP(hipStreamGetDevice(st, &sdev));
+  DARK_CHECK_ARG((int)sdev == cur, "stream belongs to device %d but device %d is current (make the tensors' device current "
+                 "before calling)", (int)sdev, cur);
+  return DARK_OK;
+}
+
+int check_paged_kv(const dark_paged_kv* kv, const char* who) {
+  DARK_CHECK_ARG(kv->dtype == DARK_F32 || kv->dtype == DARK_BF16, "%s: bad dtype %d", who, kv->dtype);
+  const int es = kv->dtype == DARK_BF16 ? 2 : 4;
+  DARK_CHECK_ARG(kv->head_dim == 64 || kv->head_dim == 96 || kv->head_dim == 128, "%s: head_dim=%d must be 64, 96 or 128", who, kv->head_dim);
+  DARK_CHECK_ARG(kv->n_kv_heads >= 1 && kv->n_kv_heads <= 4096, "%s: n_kv_heads=%d", who, kv->n_kv_heads);
+  DARK_CHECK_ARG(kv->page_size >= 1 && kv->page_size <= 4096 && (kv->page_size & (kv->page_size - 1)) == 0,
+                 "%s: page_size=%d must be a power of two up to 4096", who, kv->page_size);
+  DARK_CHECK_ARG(kv->n_pages >= 0, "%s: n_pages=%d", who, kv->n_pages);
+  DARK_CHECK_ARG(kv->n_pages == 0 || (kv->k && kv->v), "%s: null cache pointer", who);
+  DARK_CHECK_ARG(kv->page_stride >= 0 && kv->slot_stride >= 0 && kv->head_stride >= 0, "%s: negative cache stride", who);
+  DARK_CHECK_ARG(aligned16(kv->k, kv->page_stride, kv->slot_stride, es) && aligned16(kv->v, kv->head_stride, 0, es),
+                 "%s: the cache's pointers and strides must be multiples of 16 bytes", who);
+  return DARK_OK;
+}
+
+static int launch_head_rows(const RowsArgs& a, int dtype, int HD, hipStream_t st) {
+  DARK_TRY(check_stream_device(st));
+  const dim3 grid((unsigned)cdiv(a.T, 4)), block(256);
+#define DARK_ROWS(T, HDv) hipLaunchKernelGGL((head_rows_kernel<T, HDv>), grid, block, 0, st, a)
+  if (dtype == DARK_BF16) {
+    if (HD == 64) DARK_ROWS(bf16_t, 64); else if (HD == 96) DARK_ROWS(bf16_t, 96); else DARK_ROWS(bf16_t, 128);
+  } else {
+    if (HD == 64) DARK_ROWS(float, 64); else if (HD == 96) DARK_ROWS(float, 96); else DARK_ROWS(float, 128);
+  }
+#undef DARK_ROWS
+  DARK_CHECK_LAUNCH();
+  return DARK_OK;
+}
+
+static int check_rows(const char* who, int dtype, int T, int Hq, int Hk, int HD, float eps) {
+  DARK_CHECK_ARG(dtype == DARK_F32 || dtype == DARK_BF16, "%s: bad dtype %d", who, dtype);
+  DARK_CHECK_ARG(HD == 64 || HD == 96 || HD == 128, "%s: head_dim=%d must be 64, 96 or 128", who, HD);
+  DARK_CHECK_ARG(T >= 0 && T < (1 << 30), "%s: n_tokens=%d", who, T);
+  DARK_CHECK_ARG(Hq >= 0 && Hq <= 4096 && Hk >= 0 && Hk <= 4096, "%s: heads %d / %d", who, Hq, Hk);
+  DARK_CHECK_ARG(eps >= 0.f, "%s: eps=%g", who, (double)eps);
+  return DARK_OK;
+}
+
+}  // namespace dark
+
+using namespace dark;
+
+extern "C" {
+
+int dark_qk_norm_rope(const dark_qk_norm_rope_args* p, void* stream) {
+  const char* who = "qk_norm_rope";
+  DARK_CHECK_ARG(p != nullptr, "%s: null arguments", who);
+  DARK_TRY(check_rows(who, p->dtype, p->n_tokens, p->n_heads, p->n_kv_heads, p->head_dim, p->eps));
+  if (p->n_tokens == 0 || p->n_heads + p->n_kv_heads == 0) return DARK_OK;
+  const int es = p->dtype == DARK_BF16 ? 2 : 4;
+  DARK_CHECK_ARG((p->n_heads == 0 || (p->q && p->q_out)) && (p->n_kv_heads == 0 || (p->k && p->k_out)), "%s: null pointer", who);
+  DARK_CHECK_ARG((p->rope_cos == nullptr) == (p->rope_sin == nullptr), "%s: rope_cos and rope_sin go together", who);
+  DARK_CHECK_ARG(!p->rope_cos || (p->pos && p->max_pos >= 1), "%s: a rotation needs positions and a table", who);
+  DARK_CHECK_ARG(aligned16(p->q, p->q_ts, p->q_hs, es) && aligned16(p->k, p->k_ts, p->k_hs, es) &&
+                     aligned16(p->q_out, p->qo_ts, p->qo_hs, es) && aligned16(p->k_out, p->ko_ts, p->ko_hs, es),
+                 "%s: pointers and strides must be multiples of 16 bytes", who);
+  RowsArgs a = {};
+  a.src[0] = p->q; a.src[1] = p->k; a.dst[0] = p->q_out; a.dst[1] = p->k_out;
+  a.w[0] = p->q_w; a.w[1] = p->k_w; a.cosT = p->rope_cos; a.sinT = p->rope_sin; a.pos = p->pos;
+  a.src_ts[0] = p->q_ts; a.src_hs[0] = p->q_hs; a.src_ts[1] = p->k_ts; a.src_hs[1] = p->k_hs;
+  a.dst_ts[0] = p->qo_ts; a.dst_hs[0] = p->qo_hs; a.dst_ts[1] = p->ko_ts; a.dst_hs[1] = p->ko_hs;
+  a.T = p->n_tokens; a.max_pos = p->max_pos; a.eps = p->eps;
+  a.h_end[0] = p->n_heads; a.h_end[1] = a.h_end[2] = p->n_heads + p->n_kv_heads;
+  return launch_head_rows(a, p->dtype, p->head_dim, (hipStream_t)stream);
+}
+
+int dark_kv_append(const dark_kv_append_args* p, void* stream) {
+  const char* who = "kv_append";
+  DARK_CHECK_ARG(p != nullptr, "%s: null arguments", who);
+  DARK_TRY(check_paged_kv(&p->kv, who));
+  DARK_TRY(check_rows(who, p->kv.dtype, p->n_tokens, p->n_heads, p->kv.n_kv_heads, p->kv.head_dim, p->eps));
+  if (p->n_tokens == 0) return DARK_OK;
+  const int es = p->kv.dtype == DARK_BF16 ? 2 : 4;
+  DARK_CHECK_ARG(p->k && p->v && p->slots, "%s: null pointer", who);
+  DARK_CHECK_ARG((p->q == nullptr) == (p->q_out == nullptr) && (p->n_heads == 0 || p->q), "%s: q and q_out go together", who);
+  DARK_CHECK_ARG((p->rope_cos == nullptr) == (p->rope_sin == nullptr), "%s: rope_cos and rope_sin go together", who);
+  DARK_CHECK_ARG(!p->rope_cos || (p->pos && p->max_pos >= 1), "%s: a rotation needs positions and a table", who);
+  DARK_CHECK_ARG(aligned16(p->q, p->q_ts, p->q_hs, es) && aligned16(p->k, p->k_ts, p->k_hs, es) &&
+                     aligned16(p->v, p->v_ts, p->v_hs, es) && aligned16(p->q_out, p->qo_ts, p->qo_hs, es),
+                 "%s: pointers and strides must be multiples of 16 bytes", who);
+  RowsArgs a = {};
+  const int Hq = p->q ? p->n_heads : 0, Hk = p->kv.n_kv_heads;
+  a.src[0] = p->q; a.src[1] = p->k; a.src[2] = p->v;
+  a.dst[0] = p->q_out; a.dst[1] = p->kv.k; a.dst[2] = p->kv.v;
+  a.w[0] = p->q_w; a.w[1] = p->k_w; a.cosT = p->rope_cos; a.sinT = p->rope_sin; a.pos = p->pos; a.slots = p->slots;
+  a.src_ts[0] = p->q_ts; a.src_hs[0] = p->q_hs; a.src_ts[1] = p->k_ts; a.src_hs[1] = p->k_hs; a.src_ts[2] = p->v_ts; a.src_hs[2] = p->v_hs;
+  a.dst_ts[0] = p->qo_ts; a.dst_hs[0] = p->qo_hs;
+  a.dst_ts[1] = a.dst_ts[2] = p->kv.slot_stride; a.dst_hs[1] = a.dst_hs[2] = p->kv.head_stride;
+  a.page_stride = p->kv.page_stride; a.n_slots = (int64_t)p->kv.n_pages * p->kv.page_size;
+  a.T = p->n_tokens; a.max_pos = p->max_pos; a.eps = p->eps; a.page_log2 = __builtin_ctz((unsigned)p->kv.page_size);
+  a.h_end[0] = Hq; a.h_end[1] = Hq + Hk; a.h_end[2] = Hq + 2 * Hk;
+  return launch_head_rows(a, p->kv.dtype, p->kv.head_dim, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define DARK_HIP_ABI_VERSION 7
+#define DARK_HIP_ABI_VERSION 8
 
 #define DARK_OK 0
 #define DARK_ERR_ARG 1         /* bad shape / pointer / unsupported size */
@@ -358,6 +358,94 @@ int dark_prof_select_gemm(int epi);
  * flavour on fewer rows (dark_forward_hidden_rows), the roofline figure is quoted on the full-size launches */
 int dark_prof_select_gemm_rows(int epi, int rows);
 int dark_prof_read(double* total_ms, double* total_flops, int* launches);
+
+/* ---- paged key / value cache.  Serves denoise steps that recompute only the positions that can still change against
+ * the cached keys and values of the others, and windows of any length.  NO COUNTERPART IN THE REFERENCE: its callers run
+ * with use_cache=False (configuration_dream.py:29-50, trainer.py:152-157) and recompute the whole window in every step.
+ *
+ * One layer's cache: `n_pages` pages of `page_size` slots (a power of two); element (page, slot, head, i) of k and of v
+ * lies at page * page_stride + slot * slot_stride + head * head_stride + i (strides in elements, the same for k and v; all
+ * strides multiples of 16 bytes, k and v 16-byte aligned).  Token j of a sequence lies in slot j % page_size of the page
+ * that entry j / page_size of the sequence's block table names.  Types: DARK_F32, DARK_BF16; head_dim 64, 96 or 128. */
+typedef struct dark_paged_kv {
+  void* k;
+  void* v;
+  int64_t page_stride, slot_stride, head_stride;
+  int32_t dtype, n_pages, page_size, n_kv_heads, head_dim, reserved;
+} dark_paged_kv;
+
+/* RMS norm of every query and key head with its position rotation in one pass (q_norm / k_norm of a model with
+ * DreamConfig(qk_norm=True); rotation as apply_rotary_pos_emb, modeling_dream_length.py:183-207):
+ *   n = w * x / sqrt(mean(x^2) + eps) over the head_dim elements of a head;  out = n * cos + rotate_half(n) * sin
+ * in fp32, rounded once.  q [n_tokens, n_heads, head_dim], k [n_tokens, n_kv_heads, head_dim]: element strides *_ts between
+ * tokens and *_hs between heads, last dimension contiguous (so views of a fused q/k/v projection are taken as they are);
+ * pointers and strides multiples of 16 bytes.  q_out = q (same strides) runs in place, k_out = k likewise; any other
+ * overlap of an output with an input is not allowed.
+ *   q_w, k_w [head_dim] fp32, NULL = no norm for that operand
+ *   rope_cos, rope_sin [max_pos, head_dim/2] fp32, both NULL = no rotation; pos [n_tokens] int32, clamped to the table */
+typedef struct dark_qk_norm_rope_args {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const float *q_w, *k_w, *rope_cos, *rope_sin;
+  const int32_t* pos;
+  int64_t q_ts, q_hs, k_ts, k_hs, qo_ts, qo_hs, ko_ts, ko_hs;
+  int32_t dtype, n_tokens, n_heads, n_kv_heads, head_dim, max_pos;
+  float eps;
+  int32_t reserved;
+} dark_qk_norm_rope_args;
+int dark_qk_norm_rope(const dark_qk_norm_rope_args* a, void* stream);
+
+/* New tokens into the pages: k rotated (and normed, where k_w is given) -> its slot, v -> its slot, q (nullable) rotated
+ * (and normed) -> q_out, one launch.  slots [n_tokens] int64: page * page_size + slot in the page; a token whose slot is
+ * negative or beyond the cache is not stored (its q_out is written all the same).  The slots of one call must differ:
+ * where two are equal the slot holds, for each 16 bytes, one of the tokens' values.  q, k, v, q_out: strides, alignment
+ * and in-place rule as above; q_out = NULL needs q = NULL. */
+typedef struct dark_kv_append_args {
+  dark_paged_kv kv;
+  const void *q, *k, *v;
+  void* q_out;
+  const float *q_w, *k_w, *rope_cos, *rope_sin;
+  const int32_t* pos;
+  const int64_t* slots;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, qo_ts, qo_hs;
+  int32_t n_tokens, n_heads, max_pos;
+  float eps;
+} dark_kv_append_args;
+int dark_kv_append(const dark_kv_append_args* a, void* stream);
+
+/* Attention of a chunk of new tokens over the pages; keys of a token and of its head's group (n_heads a multiple of
+ * n_kv_heads; query head h reads key head h / (n_heads / n_kv_heads)):
+ *   out[t] = sum_j softmax_j(scale * q[t] . k[j]) v[j] over the keys j < kv_len of t's sequence that its mask, its block
+ *   table and (causal) its own index leave; a token for which none is left gets zeros and lse = -inf.
+ * Tokens cu_q[b] .. cu_q[b+1]-1 belong to sequence b (cu_q non-decreasing; tokens before cu_q[0] and behind
+ * cu_q[n_seqs] are left as they were).  Whatever lies in slots that no key of a token uses -- NaN, infinities -- does not
+ * reach its output; scores, softmax statistics and sums are fp32.
+ *   q, out [n_tokens, n_heads, head_dim]: strides and alignment as above; out must not overlap q
+ *   block_table [n_seqs, table_width] int32, row stride table_stride; an entry outside [0, n_pages) leaves its keys out
+ *   kv_len [n_seqs] int32: keys of the sequence, the chunk's own included; clamped to [0, min(max_kv, table_width *
+ *     page_size)]
+ *   q_index [n_tokens] int32 or NULL = the last tokens of the sequence: kv_len - (new tokens) + i (read if causal only)
+ *   key_mask [n_seqs, >= max_kv] uint8 (0 = left out), row stride mask_stride, or NULL
+ *   max_q, max_kv: no sequence has more new tokens / more keys (tokens of a sequence beyond max_q may be left as they
+ *     were, keys beyond max_kv are left out)
+ *   lse [n_tokens, n_heads] fp32 or NULL: log(sum_j exp(score))
+ * workspace: dark_paged_attention_workspace_bytes(a) bytes, 16-byte aligned (0: none needed); calls that overlap must not
+ * share it. */
+typedef struct dark_paged_attention_args {
+  dark_paged_kv kv;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t *block_table, *cu_q, *kv_len, *q_index;
+  const uint8_t* key_mask;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride;
+  int32_t n_tokens, n_heads, n_seqs, table_width, max_q, max_kv, causal;
+  float scale;
+} dark_paged_attention_args;
+size_t dark_paged_attention_workspace_bytes(const dark_paged_attention_args* a);
+int dark_paged_attention(const dark_paged_attention_args* a, void* stream);
 
 /* ---- GPT-2 backbone of the legacy denoiser: akgr/abduction_model/model/custom_gpt.py:25-114,
  * `DiffusionModel(GPT2LMHeadModel)` built by create_gpt2_transformer (:446-472).  Weights are packed by

@@ -1,0 +1,408 @@
+"""The paged key / value cache's operators (dark_amd/kv_cache.py) on the GPU against float64 (oracle/kv_cache_oracle.py).
+
+Tolerances are bounds by arithmetic, with u = 2^-24 and, for bf16, h = 2^-8 (half a step, relative):
+  norm + rotation: a lane adds 16 squares and 4 partial sums (20 u, halved by the root), mean, eps, root, division, weight,
+    product and the rotation's sum: below 24 u of |first term| + |second term|; bf16 adds its one rounding, h |y|.
+  attention: a score is a sum of D products, off by at most (D + 3) u z (z = scale * sum |q_i k_i|), the exponent and the
+    hardware's exp2 by a few u (1 + |s|): a weight is off by a relative d = (D + 8) u (z + 1), a normalised one by 2 d;
+    n keys added up in any order, and rescaled once a tile, add (2 n + 64) u: together (2 d + (2 n + 64) u) a with
+    a = sum_j p_j |v_j|.  bf16 rounds every weight once (h a) and the output once (h |out|).
+  lse: d + (2 n + 64) u + 4 u |lse|.
+"""
+import math
+
+import pytest
+import torch
+
+from dark_amd import _hip, kv_cache
+from oracle import kv_cache_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U, HALF = 2.0 ** -24, 2.0 ** -8
+
+
+def tables(n, D, theta=1000.0):
+    f = theta ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+    ang = torch.arange(n, dtype=torch.float64)[:, None] * f
+    return ang.cos().float().contiguous(), ang.sin().float().contiguous()
+
+
+def check_rows(got, y, a, dtype):
+    tol = 24 * U * a + (HALF * y.abs() if dtype == torch.bfloat16 else 0) + 1e-37
+    err = (got.cpu().double() - y).abs()
+    assert bool((err <= tol).all()), (err / tol).max()
+
+
+def check_attention(got, ref, n, D, dtype, lse=None):
+    out, l, a, z = ref
+    own = ~out.isnan().any(-1).any(-1) | False
+    d = (D + 8) * U * (z + 1)
+    tol = (2 * d[..., None] + (2 * n + 64) * U) * a + 1e-30
+    if dtype == torch.bfloat16:
+        tol = tol + HALF * a + HALF * out.abs()
+    err = (got.cpu().double() - out).abs()
+    assert bool((err <= tol)[own].all()), (err / tol)[own].max()
+    if lse is not None:
+        fin = own[:, None] & (l > -math.inf)
+        e = (lse.cpu().double() - l).abs()
+        assert bool((e <= d + (2 * n + 64) * U + 4 * U * l.abs())[fin].all())
+        assert bool((lse.cpu()[own[:, None] & (l == -math.inf)] == -math.inf).all())
+
+
+# --------------------------------------------------------------------------- norm + rotation
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,H,Hk,D", [(1, 8, 8, 96), (5, 12, 12, 64), (77, 32, 8, 128), (3, 7, 1, 96), (130, 1, 1, 128),
+                                      (9, 40, 10, 64)])
+@pytest.mark.parametrize("norm,rope", [(True, True), (False, True), (True, False), (False, False)])
+def test_qk_norm_rope(dtype, T, H, Hk, D, norm, rope):
+    g = torch.Generator().manual_seed(T * 31 + H + D)
+    qkv = (torch.randn(T, H + 2 * Hk, D, generator=g) * 2).to(dtype)
+    qkv[0, 0] = 0                                             # a row of zeros: eps alone under the root
+    qw, kw = ((1 + 0.2 * torch.randn(D, generator=g)) if norm else None for _ in range(2))
+    cos, sin = tables(300, D) if rope else (None, None)
+    pos = torch.randint(-3, 310, (T,), generator=g, dtype=torch.int32) if rope else None   # clamped to the table
+    d = lambda t: None if t is None else t.to(DEV)
+    x = qkv.to(DEV)
+    q, k = kv_cache.qk_norm_rope(x[:, :H], x[:, H:H + Hk], d(qw), d(kw), d(cos), d(sin), d(pos), eps=1e-6)
+    for got, src, w in ((q, qkv[:, :H], qw), (k, qkv[:, H:H + Hk], kw)):
+        check_rows(got, *O.norm_rope(src, w, cos, sin, pos, 1e-6), dtype)
+    assert torch.equal(x.cpu(), qkv)
+    # in place on the fused projection's output: the same bits, v untouched
+    kv_cache.qk_norm_rope(x[:, :H], x[:, H:H + Hk], d(qw), d(kw), d(cos), d(sin), d(pos), eps=1e-6, q_out=x[:, :H],
+                          k_out=x[:, H:H + Hk])
+    assert torch.equal(x[:, :H], q) and torch.equal(x[:, H:H + Hk], k) and torch.equal(x[:, H + Hk:].cpu(), qkv[:, H + Hk:])
+
+
+def test_qk_norm_rope_strides():
+    """[H, T, D] memory order, one norm only, far positions, huge and tiny rows, and inputs the kernel cannot take as
+    they are (a misaligned view, a last dimension with a stride)."""
+    g = torch.Generator().manual_seed(3)
+    T, H, D = 33, 4, 128
+    cos, sin = tables(70000, D)
+    pos = torch.randint(60000, 70000, (T,), generator=g, dtype=torch.int32)
+    q = torch.randn(H, T, D, generator=g) * torch.logspace(-15, 15, T)[None, :, None]
+    w = torch.randn(D, generator=g)
+    ref = O.norm_rope(q.transpose(0, 1), w, cos, sin, pos, 1e-6)
+    args = [t.to(DEV) for t in (cos, sin, pos)]
+    qd = q.to(DEV).transpose(0, 1)
+    a, b = kv_cache.qk_norm_rope(qd, qd, w.to(DEV), None, *args, eps=1e-6)
+    check_rows(a, *ref, torch.float32)
+    check_rows(b, *O.norm_rope(q.transpose(0, 1), None, cos, sin, pos, 1e-6), torch.float32)
+    buf = torch.zeros(H * T * D + 1, device=DEV)
+    off = buf[1:].view(T, H, D)
+    off.copy_(qd)
+    odd = torch.empty(T, H, 2 * D, device=DEV)[..., ::2]
+    odd.copy_(qd)
+    for x in (off, odd):
+        y, _ = kv_cache.qk_norm_rope(x, x, w.to(DEV), None, *args, eps=1e-6)
+        assert torch.equal(y, a)
+
+
+# --------------------------------------------------------------------------- append
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,H,Hk,D,page", [(1, 8, 8, 96, 16), (53, 12, 12, 64, 1), (200, 32, 8, 128, 64), (7, 3, 1, 96, 4096)])
+@pytest.mark.parametrize("norm,heads_first", [(False, False), (True, True)])
+def test_append_kv(dtype, T, H, Hk, D, page, norm, heads_first):
+    g = torch.Generator().manual_seed(T + D + page)
+    n_pages = T // page + 2
+    shape = (n_pages, Hk, page, D) if heads_first else (n_pages, page, Hk, D)
+    view = (lambda t: t.transpose(1, 2)) if heads_first else (lambda t: t)
+    kc, vc = (torch.randn(shape, generator=g).to(dtype) for _ in range(2))
+    qkv = torch.randn(T, H + 2 * Hk, D, generator=g).to(dtype)
+    qkv[0, H + Hk, 0] = math.nan                              # values are carried, not computed
+    qw, kw = ((1 + 0.2 * torch.randn(D, generator=g)) if norm else None for _ in range(2))
+    cos, sin = tables(500, D)
+    pos = torch.randint(0, 500, (T,), generator=g, dtype=torch.int32)
+    slots = torch.randperm(n_pages * page, generator=g)[:T]
+    slots[T // 2] = -1                                        # not stored
+    if T > 9:
+        slots[3], slots[9] = n_pages * page, 1 << 40
+    d = lambda t: None if t is None else t.to(DEV)
+    kd, vd, x = kc.to(DEV), vc.to(DEV), qkv.to(DEV)
+    q = kv_cache.append_kv(x[:, H:H + Hk], x[:, H + Hk:], view(kd), view(vd), d(slots), d(cos), d(sin), d(pos), q=x[:, :H],
+                           q_weight=d(qw), k_weight=d(kw))
+    check_rows(q, *O.norm_rope(qkv[:, :H], qw, cos, sin, pos, 1e-6), dtype)
+    y, a = O.norm_rope(qkv[:, H:H + Hk], kw, cos, sin, pos, 1e-6)
+    check_rows(view(kd), O.append(view(kc).double(), y, slots), O.append(torch.zeros_like(view(kc)).double(), a, slots), dtype)
+    want = O.append(view(vc), qkv[:, H + Hk:], slots)
+    assert torch.equal(view(vd).cpu().nan_to_num(7.0), want.nan_to_num(7.0)) and int(view(vd).isnan().sum()) == int(want.isnan().sum())
+    # what is not stored stays bit for bit
+    rest = torch.ones(n_pages * page, dtype=torch.bool)
+    rest[slots[(slots >= 0) & (slots < n_pages * page)]] = False
+    assert torch.equal(view(kd).cpu().reshape(-1, Hk, D)[rest], view(kc).reshape(-1, Hk, D)[rest])
+    # without q: the same cache; without a rotation: the keys as they are
+    k2, v2 = kc.to(DEV), vc.to(DEV)
+    assert kv_cache.append_kv(x[:, H:H + Hk], x[:, H + Hk:], view(k2), view(v2), d(slots), d(cos), d(sin), d(pos), k_weight=d(kw)) is None
+    assert torch.equal(k2, kd)
+    kv_cache.append_kv(x[:, H:H + Hk], x[:, H + Hk:], view(k2), view(v2), d(slots))
+    assert torch.equal(view(k2).cpu(), O.append(view(kc), qkv[:, H:H + Hk], slots))
+
+
+# --------------------------------------------------------------------------- attention
+def paged(q_lens, kv_lens, H, Hk, D, page, dtype, seed=0, spare=3, lead=0, tail=0, heads_first=False, fill=math.nan):
+    """A batch over shuffled pages; every slot no sequence uses holds `fill`."""
+    g = torch.Generator().manual_seed(seed + sum(kv_lens) + D)
+    B, per = len(q_lens), [-(-n // page) for n in kv_lens]
+    n_pages = sum(per) + spare
+    ids = torch.randperm(n_pages, generator=g).int()
+    table = torch.full((B, max(per + [1])), -7, dtype=torch.int32)
+    kc = torch.full((n_pages, page, Hk, D), fill).to(dtype)
+    vc = kc.clone()
+    at = 0
+    for b in range(B):
+        table[b, :per[b]] = ids[at:at + per[b]]
+        at += per[b]
+        for j in range(kv_lens[b]):
+            kc[table[b, j // page], j % page] = torch.randn(Hk, D, generator=g).to(dtype)
+            vc[table[b, j // page], j % page] = torch.randn(Hk, D, generator=g).to(dtype)
+    T = lead + sum(q_lens) + tail
+    cu = torch.tensor([lead + sum(q_lens[:b]) for b in range(B + 1)], dtype=torch.int32)
+    q = (torch.randn(T, H, D, generator=g) * 1.5).to(dtype)
+    return dict(q=q, k=kc, v=vc, table=table, cu=cu, kv=torch.tensor(kv_lens, dtype=torch.int32), max_q=max(q_lens + [0]),
+                max_kv=max(kv_lens + [0]), heads_first=heads_first)
+
+
+def run_paged(p, **kw):
+    if p["heads_first"]:
+        k, v = (t.transpose(1, 2).contiguous().to(DEV).transpose(1, 2) for t in (p["k"], p["v"]))
+    else:
+        k, v = p["k"].to(DEV), p["v"].to(DEV)
+    kw = {n: (t.to(DEV) if isinstance(t, torch.Tensor) else t) for n, t in kw.items()}
+    return kv_cache.paged_attention(kw.pop("q", p["q"].to(DEV)), k, v, p["table"].to(DEV), p["cu"].to(DEV), p["kv"].to(DEV),
+                                    p["max_q"], p["max_kv"], **kw)
+
+
+SHAPES = [  # q_lens, kv_lens, H, Hk, D, page
+    ([1], [1], 8, 8, 96, 16),
+    ([1, 1, 1], [0, 33, 64], 8, 8, 96, 16),                       # nothing cached, one key past a tile, whole tiles
+    ([11, 0, 11, 3], [46, 46, 11, 3], 8, 8, 96, 16),              # a denoise step; a sequence without new tokens
+    ([1, 5, 2], [130, 257, 5], 32, 8, 128, 64),
+    ([17, 64, 1], [17, 200, 95], 12, 12, 64, 32),
+    ([70, 33], [333, 33], 4, 1, 128, 128),                        # one key head; pages longer than a tile
+    ([150], [400], 6, 3, 64, 1),                                  # pages of one slot
+    ([3, 2], [40, 9], 28, 4, 128, 8),
+    ([129, 257], [129, 700], 2, 2, 96, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_paged_attention(dtype, causal, shape):
+    q_lens, kv_lens, H, Hk, D, page = SHAPES[shape]
+    p = paged(q_lens, kv_lens, H, Hk, D, page, dtype, seed=shape, heads_first=shape % 2 == 1)
+    out, lse = run_paged(p, causal=causal, return_lse=True)
+    check_attention(out, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=causal), max(kv_lens), D, dtype, lse)
+    again, _ = run_paged(p, causal=causal, return_lse=True)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_lens,H,Hk,D", [([11, 40, 1, 2], 4, 2, 96), ([1, 1, 1, 2], 8, 8, 64), ([200, 130, 7, 2], 2, 1, 128)])
+def test_masks_and_what_lies_in_masked_places(dtype, causal, q_lens, H, Hk, D):
+    """Key masks with NaN and infinities in what they hide, a sequence masked whole, block-table entries that name no
+    page, given places, a scale of its own, tokens before and behind the batch left as they were."""
+    kv_lens = [200, 77, 33, 2]
+    p = paged(q_lens, kv_lens, H, Hk, D, 16, dtype, seed=5, lead=2, tail=3)
+    g = torch.Generator().manual_seed(9)
+    mask = torch.rand(4, 210, generator=g) > 0.4
+    mask[2] = False                                               # nothing left for this sequence
+    mask[0, 64:96] = False                                        # a whole tile
+    for b in range(4):
+        for j in range(kv_lens[b]):
+            if not mask[b, j]:
+                pg, s = p["table"][b, j // 16], j % 16
+                p["k"][pg, s], p["v"][pg, s] = math.nan, math.inf
+    p["table"][0, 1], p["table"][1, 2] = -1, p["k"].shape[0]      # no such pages: their keys are out
+    index = torch.cat([torch.randint(-2, n + 3, (m,), generator=g) for n, m in zip([0] + kv_lens + [0], [2] + q_lens + [3])]).int()
+    kw = dict(causal=causal, q_index=index, key_mask=mask, scale=0.3)
+    out = torch.full(p["q"].shape, 5.0, dtype=dtype, device=DEV)
+    got, lse = run_paged(p, out=out, return_lse=True, **kw)
+    ref = O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], **kw)
+    check_attention(got, ref, 200, D, dtype, lse)
+    assert bool((got[:2] == 5).all()) and bool((got[-3:] == 5).all())
+    at = int(p["cu"][2])
+    assert bool((got[at:at + q_lens[2]] == 0).all())
+    assert torch.equal(run_paged(p, **{**kw, "key_mask": mask.to(torch.uint8)})[2:-3], got[2:-3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("n,q_len,H,Hk", [(150, 150, 2, 2), (45, 6, 8, 2), (300, 300, 4, 1)])
+def test_infinities_and_nan_behind_a_causal_token(dtype, D, n, q_len, H, Hk):
+    """Infinities and NaN in a later token's keys and values reach only the tokens that see it, element by element."""
+    p = paged([q_len], [n], H, Hk, D, 16, dtype, seed=2)
+    clean = O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=True)
+    put = lambda j, h, i, x, t="v": p[t].__setitem__((int(p["table"][0, j // 16]), j % 16, h, i), x)
+    j0 = n - q_len + q_len // 2
+    put(j0, 0, 3, math.nan)
+    put(j0 + 1, 0, 5, math.inf)
+    put(j0 + 1, 0, 7, -math.inf)
+    put(j0 + 2, 0, 5, -math.inf)                                  # +inf and -inf together: NaN
+    put(n - 1, 0, 9, math.nan, "k")                               # the last key: only the last token sees it
+    got = run_paged(p, causal=True).cpu()
+    G, i0 = H // Hk, q_len // 2
+    last = q_len - 1
+    check_attention(got[:i0], tuple(x[:i0] for x in clean), n, D, dtype)
+    assert bool(got[last, :G].isnan().all()), "the last token of the head group that holds the NaN key"
+    check_attention(got[:last, G:], tuple(x[:last, G:] for x in clean), n, D, dtype)    # the other key heads
+    sel = [i for i in range(D) if i not in (3, 5, 7)]
+    mid = slice(i0, last)
+    check_attention(got[mid][:, :G, sel], (clean[0][mid][:, :G, sel], clean[1][mid][:, :G], clean[2][mid][:, :G, sel], clean[3][mid][:, :G]), n, D, dtype)
+    if last > i0:
+        assert bool(got[mid][:, :G, 3].isnan().all())
+    if last > i0 + 1:
+        assert bool((got[i0 + 1:last][:, :G, 7] == -math.inf).all()) and bool((got[i0 + 1, :G, 5] == math.inf).all())
+    if last > i0 + 2:
+        assert bool(got[i0 + 2:last][:, :G, 5].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_lens,kv_lens,H,Hk,D,page", [([1], [5000], 8, 8, 96, 16), ([1, 1, 4], [3001, 1, 700], 8, 2, 128, 64),
+                                                       ([4], [2500], 32, 8, 128, 32), ([40], [2111], 4, 4, 64, 16)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_long_key_axis(dtype, q_lens, kv_lens, H, Hk, D, page, causal):
+    """Few rows over many keys: the axis is split over workgroups and joined; the same bits every time."""
+    p = paged(q_lens, kv_lens, H, Hk, D, page, dtype, seed=1)
+    out, lse = run_paged(p, causal=causal, return_lse=True)
+    check_attention(out, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=causal), max(kv_lens), D, dtype, lse)
+    for _ in range(3):
+        assert torch.equal(run_paged(p, causal=causal), out)
+
+
+def test_views_strides_and_scores_far_apart():
+    """q and out as views of larger tensors; scores so far apart that one key takes the whole row."""
+    p = paged([9, 2], [100, 50], 8, 8, 96, 16, torch.float32, seed=8)
+    p["q"] *= 40
+    wide = torch.zeros(11, 24, 96, device=DEV)
+    wide[:, 8:16] = p["q"].to(DEV)
+    o = torch.full((8, 11, 96), 3.0, device=DEV).transpose(0, 1)
+    got = run_paged(p, q=wide[:, 8:16], out=o)
+    assert got is o
+    check_attention(got, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"]), 100, 96, torch.float32)
+    buf = torch.zeros(p["q"].numel() + 1, device=DEV)
+    odd = buf[1:].view(11, 8, 96)
+    odd.copy_(p["q"])
+    assert torch.equal(run_paged(p, q=odd), got)
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^31 elements, the sequence in its last pages."""
+    page, Hk, D = 64, 8, 128
+    n_pages = (1 << 31) // (page * Hk * D) + 40
+    kc = torch.zeros(n_pages, page, Hk, D, dtype=torch.bfloat16, device=DEV)
+    vc = torch.zeros_like(kc)
+    assert kc.numel() > 1 << 31
+    T = 100
+    g = torch.Generator().manual_seed(0)
+    qkv = torch.randn(T, 3 * Hk, D, generator=g).bfloat16()
+    pages = torch.tensor([[n_pages - 1, n_pages - 7]], dtype=torch.int32)
+    idx = torch.arange(T)
+    slots = (pages[0, idx // page].long() * page + idx % page).to(DEV)
+    x = qkv.to(DEV)
+    kv_cache.append_kv(x[:, Hk:2 * Hk], x[:, 2 * Hk:], kc, vc, slots)
+    out = kv_cache.paged_attention(x[:, :Hk], kc, vc, pages.to(DEV), torch.tensor([0, T], dtype=torch.int32, device=DEV),
+                                   torch.tensor([T], dtype=torch.int32, device=DEV), T, T, causal=True)
+    small = torch.stack([qkv[:64, Hk:2 * Hk], torch.cat([qkv[64:, Hk:2 * Hk], torch.zeros(28, Hk, D).bfloat16()])])
+    smallv = torch.stack([qkv[:64, 2 * Hk:], torch.cat([qkv[64:, 2 * Hk:], torch.zeros(28, Hk, D).bfloat16()])])
+    ref = O.attention(qkv[:, :Hk], small, smallv, torch.tensor([[0, 1]]), [0, T], [T], causal=True)
+    check_attention(out, ref, T, D, torch.bfloat16)
+
+
+# --------------------------------------------------------------------------- together
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prefill_then_tokens(dtype):
+    """A prompt in two chunks, then single tokens, all with norms and rotation, against the whole computed at once."""
+    g = torch.Generator().manual_seed(4)
+    B, H, Hk, D, page, n = 3, 8, 2, 96, 16, 61
+    x = torch.randn(B, n, H + 2 * Hk, D, generator=g).to(dtype)
+    qw, kw = 1 + 0.1 * torch.randn(D, generator=g), 1 + 0.1 * torch.randn(D, generator=g)
+    cos, sin = tables(64, D)
+    per = -(-n // page)
+    table = torch.randperm(B * per, generator=g).view(B, per).int()
+    kc = torch.full((B * per, page, Hk, D), math.nan, dtype=dtype, device=DEV)
+    vc = kc.clone()
+    td, cd, sd, qd, kd = (t.to(DEV) for t in (table, cos, sin, qw, kw))
+    got = torch.empty(B, n, H, D, dtype=dtype)
+    at = 0
+    for step in (40, 17, 1, 1, 2):
+        idx = torch.arange(at, at + step).repeat(B)
+        seq = torch.arange(B).repeat_interleave(step)
+        slots = table[seq, idx // page].long() * page + idx % page
+        c = x[:, at:at + step].reshape(B * step, H + 2 * Hk, D).to(DEV)
+        q = kv_cache.append_kv(c[:, H:H + Hk], c[:, H + Hk:], kc, vc, slots.to(DEV), cd, sd, idx.int().to(DEV), q=c[:, :H],
+                               q_weight=qd, k_weight=kd)
+        o = kv_cache.paged_attention(q, kc, vc, td, torch.arange(0, B * step + 1, step, dtype=torch.int32, device=DEV),
+                                     torch.full((B,), at + step, dtype=torch.int32, device=DEV), step, at + step, causal=True)
+        got[:, at:at + step] = o.cpu().view(B, step, H, D)
+        at += step
+    # the oracle takes the operands as they were stored: rounded to the cache's type
+    pos = torch.arange(n).repeat(B)
+    rows = x.view(B * n, H + 2 * Hk, D)
+    q = O.norm_rope(rows[:, :H], qw, cos, sin, pos, 1e-6)[0].to(dtype)
+    k = kc[table.view(-1).long().to(DEV)].cpu().view(B, per * page, Hk, D)[:, :n].reshape(B * n, Hk, D)
+    check_rows(k, *O.norm_rope(rows[:, H:H + Hk], kw, cos, sin, pos, 1e-6), dtype)
+    pad = lambda t: torch.cat([t.view(B, n, Hk, D), torch.zeros(B, per * page - n, Hk, D, dtype=dtype)], 1).view(B * per, page, Hk, D)
+    ref = O.attention(q, pad(k), pad(rows[:, H + Hk:].contiguous()), torch.arange(B * per).view(B, per), [0, n, 2 * n, 3 * n], [n] * 3, causal=True)
+    out, _, a, z = ref
+    # q's own rounding (its float64 value may sit next to a border): half a step of z in the score
+    step = (HALF if dtype == torch.bfloat16 else 24 * U)
+    tol = (2 * ((D + 8) * U * (z + 1) + 2 * step * z)[..., None] + (2 * n + 64) * U) * a
+    if dtype == torch.bfloat16:
+        tol = tol + HALF * a + HALF * out.abs()
+    assert bool(((got.view(B * n, H, D).double() - out).abs() <= tol).all())
+
+
+def test_other_stream_and_graph():
+    """The calls on a side stream, and captured: every replay on new inputs equals the eager result, with eager calls and
+    two graphs in between (each capture holds its own workspace)."""
+    ps = [paged([1, 4], [3000, 900], 8, 2, 128, 16, torch.bfloat16, seed=s) for s in (1, 2)]
+    dev = [{n: t.to(DEV) for n, t in p.items() if isinstance(t, torch.Tensor)} for p in ps]
+    cos, sin = (t.to(DEV) for t in tables(4096, 128))
+    pos = torch.tensor([2999, 896, 897, 898, 899], dtype=torch.int32, device=DEV)
+    seq = torch.tensor([0, 1, 1, 1, 1], device=DEV)
+
+    def call(d):
+        slots = d["table"][seq, (pos // 16).long()].long() * 16 + pos % 16
+        new = d["q"][:, :4]
+        q = kv_cache.append_kv(new[:, :2], new[:, 2:], d["k"], d["v"], slots, cos, sin, pos, q=d["q"])
+        return kv_cache.paged_attention(q, d["k"], d["v"], d["table"], d["cu"], d["kv"], 4, 3000, causal=True)
+
+    want = [call(d).clone() for d in dev]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [call(d) for d in dev]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    graphs = []
+    for d in dev:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            o = call(d)
+        graphs.append((gr, o))
+    for rep in range(4):
+        for d in dev:
+            d["q"].copy_(torch.randn(d["q"].shape, device=DEV))
+        for gr, _ in graphs:
+            gr.replay()
+        got = [o.clone() for _, o in graphs]
+        want = [call(d) for d in dev]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), rep
+
+
+def test_nothing_to_do():
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device=DEV)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    q, k = kv_cache.qk_norm_rope(z(0, 8, 96), z(0, 8, 96), None, None, None, None, None)
+    assert q.shape == (0, 8, 96)
+    cache = z(2, 16, 8, 96)
+    assert kv_cache.append_kv(z(0, 8, 96), z(0, 8, 96), cache, cache.clone(), z(0, dtype=torch.int64)) is None
+    assert kv_cache.paged_attention(z(0, 8, 96), cache, cache, z(1, 2, dtype=torch.int32), i32(0, 0), i32(5), 0, 5).shape == (0, 8, 96)
+    # an empty cache, no table, nothing cached: zeros
+    none = z(0, 16, 8, 96)
+    out, lse = kv_cache.paged_attention(z(2, 8, 96) + 1, none, none, z(1, 0, dtype=torch.int32), i32(0, 2), i32(7), 2, 7, return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())

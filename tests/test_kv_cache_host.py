@@ -1,0 +1,119 @@
+"""The paged cache's operators without a GPU: what their entry points refuse (C and Python), the packed argument
+structs, and the float64 checker of the GPU tests against a dense attention."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from dark_amd import _hip, kv_cache
+from oracle import kv_cache_oracle as O
+
+
+def test_packed_structs_match_the_header():
+    assert kv_cache._NORM_ROPE.size == C.sizeof(_hip.QkNormRopeArgs)
+    assert kv_cache._APPEND.size == C.sizeof(_hip.KVAppendArgs)
+    assert kv_cache._ATTEND.size == C.sizeof(_hip.PagedAttentionArgs)
+    names = [n for n, _ in _hip.PagedKV._fields_] + [n for n, _ in _hip.PagedAttentionArgs._fields_[1:]]
+    vals = list(range(1, len(names) + 1))
+    a = _hip.PagedAttentionArgs.from_buffer_copy(kv_cache._ATTEND.pack(*vals))
+    got = [getattr(a.kv, n) for n, _ in _hip.PagedKV._fields_] + [getattr(a, n) for n, _ in _hip.PagedAttentionArgs._fields_[1:]]
+    assert got == vals
+
+
+def _kv(**kw):
+    f = dict(k=4096, v=8192, page_stride=16 * 8 * 96, slot_stride=8 * 96, head_stride=96, dtype=1, n_pages=4, page_size=16,
+             n_kv_heads=8, head_dim=96)
+    f.update(kw)
+    return _hip.PagedKV(**f)
+
+
+def _refused(fn, args, msg):
+    lib = _hip.load()
+    assert getattr(lib, fn)(C.byref(args) if args is not None else None, None) == _hip.DARK_ERR_ARG
+    text = lib.dark_hip_last_error().decode()
+    assert msg in text, text
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(dtype=2), "dtype"), (dict(head_dim=80), "head_dim"), (dict(n_tokens=-1), "n_tokens"),
+                                    (dict(q=None), "null pointer"), (dict(q=4104), "16 bytes"), (dict(k_ts=100), "16 bytes"),
+                                    (dict(rope_cos=None), "go together"), (dict(pos=None), "positions"), (dict(eps=-1.0), "eps"),
+                                    (dict(eps=math.nan), "eps")])
+def test_qk_norm_rope_refuses(kw, msg):
+    f = dict(q=4096, k=4096, q_out=8192, k_out=8192, rope_cos=4096, rope_sin=4096, pos=4096, q_ts=768, q_hs=96, k_ts=768, k_hs=96,
+             qo_ts=768, qo_hs=96, ko_ts=768, ko_hs=96, dtype=1, n_tokens=3, n_heads=8, n_kv_heads=8, head_dim=96, max_pos=64, eps=1e-6)
+    f.update(kw)
+    _refused("dark_qk_norm_rope", _hip.QkNormRopeArgs(**f), msg)
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(kv=_kv(page_size=24)), "power of two"), (dict(kv=_kv(k=None)), "null cache"),
+                                    (dict(kv=_kv(slot_stride=100)), "16 bytes"), (dict(kv=_kv(n_kv_heads=0)), "n_kv_heads"),
+                                    (dict(kv=_kv(page_stride=-768)), "negative"), (dict(slots=None), "null pointer"),
+                                    (dict(q=None), "go together"), (dict(rope_sin=None), "go together"), (dict(max_pos=0), "positions"),
+                                    (dict(v_hs=4), "16 bytes"), (dict(n_heads=5000), "heads")])
+def test_kv_append_refuses(kw, msg):
+    f = dict(kv=_kv(), q=4096, k=4096, v=4096, q_out=8192, rope_cos=4096, rope_sin=4096, pos=4096, slots=4096, q_ts=768, q_hs=96,
+             k_ts=768, k_hs=96, v_ts=768, v_hs=96, qo_ts=768, qo_hs=96, n_tokens=3, n_heads=8, max_pos=64, eps=1e-6)
+    f.update(kw)
+    _refused("dark_kv_append", _hip.KVAppendArgs(**f), msg)
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(n_heads=9), "multiple"), (dict(kv=_kv(head_dim=32)), "head_dim"), (dict(q=None), "null pointer"),
+                                    (dict(block_table=None), "null pointer"), (dict(max_kv=-1), "negative"), (dict(scale=math.inf), "scale"),
+                                    (dict(o_ts=4), "16 bytes"), (dict(table_stride=1), "table_stride"), (dict(table_width=1 << 28), "2^31"),
+                                    (dict(max_kv=100000), "workspace")])
+def test_paged_attention_refuses(kw, msg):
+    f = dict(kv=_kv(), q=4096, out=8192, block_table=4096, cu_q=4096, kv_len=4096, q_ts=768, q_hs=96, o_ts=768, o_hs=96,
+             table_stride=4, n_tokens=3, n_heads=8, n_seqs=2, table_width=4, max_q=2, max_kv=64, scale=0.1)
+    f.update(kw)
+    _refused("dark_paged_attention", _hip.PagedAttentionArgs(**f), msg)
+
+
+def test_null_arguments():
+    for fn in ("dark_qk_norm_rope", "dark_kv_append", "dark_paged_attention"):
+        _refused(fn, None, "null arguments")
+    assert _hip.load().dark_paged_attention_workspace_bytes(None) == 0
+
+
+def test_workspace_bytes():
+    """A function of the sizes alone: none for a short axis, parts of (O, m, l) for few rows over a long one."""
+    lib = _hip.load()
+    a = _hip.PagedAttentionArgs(kv=_kv(), n_tokens=3, n_heads=8, n_seqs=2, table_width=1 << 14, max_q=2, max_kv=64, scale=0.1)
+    assert lib.dark_paged_attention_workspace_bytes(C.byref(a)) == 0
+    a.max_kv = 100000
+    n = lib.dark_paged_attention_workspace_bytes(C.byref(a))
+    assert n > 0 and n >= 2 * 3 * 8 * (96 + 2) * 4
+
+
+def test_cpu_tensors_are_refused():
+    q = torch.zeros(1, 8, 96)
+    cache = torch.zeros(2, 16, 8, 96)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        kv_cache.qk_norm_rope(q, q, None, None, None, None, None)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        kv_cache.append_kv(q, q, cache, cache, torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        kv_cache.paged_attention(q, cache, cache, torch.zeros(1, 2, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32),
+                                 torch.tensor([5], dtype=torch.int32), 1, 5)
+
+
+def test_checker_against_dense_attention():
+    g = torch.Generator().manual_seed(1)
+    B, n, H, Hk, D, page = 2, 21, 4, 2, 64, 8
+    q, k, v = (torch.randn(B, n, h, D, generator=g, dtype=torch.float64) for h in (H, Hk, Hk))
+    per = 3
+    table = torch.randperm(B * per, generator=g).view(B, per)
+    kc, vc = (torch.full((B * per, page, Hk, D), math.nan, dtype=torch.float64) for _ in range(2))
+    slots = table[torch.arange(B).repeat_interleave(n), torch.arange(n).repeat(B) // page] * page + torch.arange(n).repeat(B) % page
+    kc, vc = O.append(kc, k.view(B * n, Hk, D), slots), O.append(vc, v.view(B * n, Hk, D), slots)
+    mask = torch.rand(B, n, generator=g) > 0.3
+    mask[:, 0] = True
+    for causal in (False, True):
+        out, lse, _, _ = O.attention(q.view(B * n, H, D), kc, vc, table, [0, n, 2 * n], [n, n], key_mask=mask, causal=causal)
+        s = torch.einsum("bihd,bjhd->bhij", q, k.repeat_interleave(2, 2)) * D ** -0.5
+        s = s.masked_fill(~mask[:, None, None], -math.inf)
+        if causal:
+            s = s.masked_fill(torch.ones(n, n).triu(1).bool(), -math.inf)
+        want = torch.einsum("bhij,bjhd->bihd", s.softmax(-1), v.repeat_interleave(2, 2))
+        torch.testing.assert_close(out.view(B, n, H, D), want, rtol=0, atol=1e-12)
+        torch.testing.assert_close(lse.view(B, n, H), s.logsumexp(-1).transpose(1, 2), rtol=0, atol=1e-12)

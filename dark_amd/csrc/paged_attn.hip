@@ -28,6 +28,7 @@ struct PagedArgs {
   float *part_o, *part_ml;     // [n_split][T][H][HD], [n_split][T][H][2]; null when n_split == 1
   int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride, page_stride, slot_stride, head_stride;
   int32_t T, H, Hk, G, B, width, n_pages, page_log2, causal, n_split, split_keys, n_tiles, cap;
+  int64_t n_units;             // problems of the launch: sequences x key heads x row tiles x parts
   float scale_log2;            // scale * log2(e)
 };
 
@@ -37,31 +38,94 @@ __device__ __forceinline__ int seq_len(const PagedArgs& a, int b) {
   return len < 0 ? 0 : (len > a.cap ? a.cap : len);
 }
 
-template <typename T> struct PVec;
-template <> struct PVec<bf16_t> { static constexpr int N = 8; typedef bf16x8 raw; };
-template <> struct PVec<float> { static constexpr int N = 4; typedef f32x4 raw; };
-
-// infinities and NaN of a V row that some row of the tile must not see (P = 0 there): 0 * inf would be NaN.  They are taken
-// out of the product and counted by a second one over P's indicator: +inf 1, -inf 2^8, NaN 2^16 (at most 32 keys a tile).
-__device__ __forceinline__ float odd_code(float x) {
-  return x != x ? 65536.f : x == INFINITY ? 1.f : x == -INFINITY ? 256.f : 0.f;
-}
+// Infinities and NaN of a V row that some row of the tile must not see (P = 0 there): 0 * inf would be NaN.  They are taken
+// out of the product and counted by a second one over P's indicator, +inf as 1, -inf as 128, NaN as both (at most 64 keys a
+// tile; 129 is a bf16), and added to the rows that do see them.
+__device__ __forceinline__ float odd_code(float x) { return x != x ? 129.f : x == INFINITY ? 1.f : x == -INFINITY ? 128.f : 0.f; }
 __device__ __forceinline__ float odd_apply(float acc, float code) {
-  if (code == 0.f) return acc;
-  const int c = (int)code;
-  const bool nan = c >= 65536, neg = (c & 0xff00) != 0, pos = (c & 0xff) != 0;
-  return (nan || (neg && pos)) ? NAN : acc + (pos ? INFINITY : -INFINITY);
+  const float neg = floorf(code * 0.0078125f), pos = __builtin_fmaf(neg, -128.f, code);
+  acc += pos > 0.f ? INFINITY : 0.f;
+  return acc + (neg > 0.f ? -INFINITY : 0.f);   // (inf - inf: NaN)
+}
+
+// 1 / l; a row without keys has l = 0 and gets zeros, a NaN sum stays one
+__device__ __forceinline__ float norm_of(float l) { return l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l); }
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l > 0.f ? (m + log2f(l)) * 0.69314718055994530942f : (l == 0.f ? -INFINITY : l);
+}
+
+// over the four lanes l, l ^ 16, l ^ 32, l ^ 48 that hold one row (swaps of 16- and 32-lane rows, no LDS)
+__device__ __forceinline__ float quad_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// over the two lanes l, l ^ 32 that hold one row
+__device__ __forceinline__ float pair_max(float x) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The running maximum is a reference, not a result: it is only raised -- and the output rescaled -- once a score exceeds it
+// by this much (log2 units; weights then reach 2^8, which floating types hold as exactly as they hold 1).
+constexpr float kSlack = 8.f;
+
+// 16 dims x 32 keys of V^T as the first operand of the second product: two transposed LDS reads (each 16-lane group fetches
+// a 4-key x 16-dim block row-wise and receives it column-wise), keys in the order P^T has them
+template <int LD>
+__device__ __forceinline__ bf16x8 read_vt(const bf16_t* Vs, int li, int g, int dt) {
+  typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+  const bf16_t* vrow = Vs + (4 * g + (li >> 2)) * LD + dt * 16 + 4 * (li & 3);
+  const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)vrow);
+  const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(vrow + 16 * LD));
+  return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// a finished row (its lanes hold 4 of every 16 columns): the output, or the part of a split axis
+template <typename T, int HD>
+__device__ __forceinline__ void write_row(const PagedArgs& a, bool parts, int64_t at, int tok, int hq, int g,
+                                          const f32x4 (&O)[HD / 16], float m, float l) {
+  if (parts) {
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) *(f32x4*)(a.part_o + at * HD + dt * 16 + 4 * g) = O[dt];
+    if (g == 0) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = l; }
+    return;
+  }
+  const float inv = norm_of(l);
+  T* orow = (T*)a.out + tok * a.o_ts + hq * a.o_hs;
+#pragma unroll
+  for (int dt = 0; dt < HD / 16; ++dt)
+    store4(orow + dt * 16 + 4 * g, make_float4(O[dt][0] * inv, O[dt][1] * inv, O[dt][2] * inv, O[dt][3] * inv));
+  if (a.lse && g == 0) a.lse[(int64_t)tok * a.H + hq] = lse_of(m, l);
+}
+
+// orders a wave's LDS writes before its lanes' reads of each other's (no instruction: LDS serves a wave in order)
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 constexpr int PT_ROWS = 64, PT_KEYS = 32;   // rows of a workgroup (16 a wave), keys of a tile
 
-template <typename T, int HD>
+// ---- fp32: 64 rows of one key head (16 a wave) against tiles of 32 keys in LDS, on 16 x 16 x 4 fp32 matrix instructions.
+template <int HD>
 __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
-  constexpr int VEC = PVec<T>::N, LD = HD + VEC, CH = HD / VEC, NT = PT_KEYS / 16;
-  constexpr bool kF32 = sizeof(T) == 4;
-  typedef typename PVec<T>::raw raw;
-  __shared__ __attribute__((aligned(16))) T Ks[PT_KEYS * LD];
-  __shared__ __attribute__((aligned(16))) T Vs[PT_KEYS * LD];
+  constexpr int VEC = 4, LD = HD + VEC, CH = HD / VEC, NT = PT_KEYS / 16;
+  typedef f32x4 raw;
+  __shared__ __attribute__((aligned(16))) float Ks[PT_KEYS * LD];
+  __shared__ __attribute__((aligned(16))) float Vs[PT_KEYS * LD];
   __shared__ float kbias[PT_KEYS];
   __shared__ int red[8];
 
@@ -101,17 +165,10 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
   const int k_begin = split * a.split_keys;
   const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
 
-  // ---- this lane's share of the queries
-  const T* qrow = (const T*)a.q + tok * a.q_ts + hq * a.q_hs;
-  bf16x8 qb[HD / 32];
+  const float* qrow = (const float*)a.q + tok * a.q_ts + hq * a.q_hs;
   float qf[HD / 4];
-  if constexpr (kF32) {
 #pragma unroll
-    for (int i = 0; i < HD / 4; ++i) qf[i] = qrow[i * 4 + g];
-  } else {
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) qb[i] = *(const bf16x8*)(qrow + i * 32 + g * 8);
-  }
+  for (int i = 0; i < HD / 4; ++i) qf[i] = qrow[i * 4 + g];
 
   f32x4 O[HD / 16];
 #pragma unroll
@@ -133,10 +190,10 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
       if (on) {
         const int64_t off = (int64_t)page * a.page_stride + (int64_t)(key & ((1 << a.page_log2) - 1)) * a.slot_stride +
                             (int64_t)hk * a.head_stride + c * VEC;
-        rk = *(const raw*)((const T*)a.k + off);
-        rv = *(const raw*)((const T*)a.v + off);
+        rk = *(const raw*)((const float*)a.k + off);
+        rv = *(const raw*)((const float*)a.v + off);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) odd |= !(fabsf((float)rv[e]) < INFINITY);
+        for (int e = 0; e < VEC; ++e) odd |= !(fabsf(rv[e]) < INFINITY);
       }
       *(raw*)(Ks + j * LD + c * VEC) = rk;
       *(raw*)(Vs + j * LD + c * VEC) = rv;
@@ -150,15 +207,9 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
 #pragma unroll
     for (int jt = 0; jt < NT; ++jt) {
       S[jt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      const T* kr = Ks + (jt * 16 + li) * LD;
-      if constexpr (kF32) {
+      const float* kr = Ks + (jt * 16 + li) * LD;
 #pragma unroll
-        for (int i = 0; i < HD / 4; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i * 4 + g], qf[i], S[jt], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i)
-          S[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)(kr + i * 32 + g * 8), qb[i], S[jt], 0, 0, 0);
-      }
+      for (int i = 0; i < HD / 4; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i * 4 + g], qf[i], S[jt], 0, 0, 0);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = jt * 16 + 4 * g + r;
@@ -167,8 +218,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
         mx = fmaxf(mx, s);
       }
     }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx = quad_max(mx);
     const float mz = mx == -INFINITY ? 0.f : mx;   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
     const float alpha = __builtin_amdgcn_exp2f(m - mz);
     m = mx;
@@ -185,80 +235,559 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
     for (int i = 0; i < HD / 16; ++i) O[i] *= alpha;
 
     // ---- O^T += V^T P^T
-    if constexpr (kF32) {
 #pragma unroll
-      for (int dt = 0; dt < HD / 16; ++dt) {
-        f32x4 code = {0.f, 0.f, 0.f, 0.f};
+    for (int dt = 0; dt < HD / 16; ++dt) {
+      f32x4 code = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int jt = 0; jt < NT; ++jt)
+      for (int jt = 0; jt < NT; ++jt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = Vs[(jt * 16 + 4 * g + r) * LD + dt * 16 + li];
-            if (odd) {
-              const float c = odd_code(v);
-              code = __builtin_amdgcn_mfma_f32_16x16x4f32(c, S[jt][r] > 0.f ? 1.f : 0.f, code, 0, 0, 0);
-              v = c == 0.f ? v : 0.f;
-            }
-            O[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, S[jt][r], O[dt], 0, 0, 0);
+        for (int r = 0; r < 4; ++r) {
+          float v = Vs[(jt * 16 + 4 * g + r) * LD + dt * 16 + li];
+          if (odd) {
+            const float c = odd_code(v);
+            code = __builtin_amdgcn_mfma_f32_16x16x4f32(c, S[jt][r] > 0.f ? 1.f : 0.f, code, 0, 0, 0);
+            v = c == 0.f ? v : 0.f;
           }
-        if (odd) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) O[dt][r] = odd_apply(O[dt][r], code[r]);
+          O[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, S[jt][r], O[dt], 0, 0, 0);
         }
-      }
-    } else {
-      // P is rounded to bf16 for the matrix instruction (relative 2^-8 a weight, as the operands of every product here)
-      bf16x8 pb, ind;
+      if (odd) {
 #pragma unroll
-      for (int jj = 0; jj < 8; ++jj) {
-        pb[jj] = (bf16_t)S[jj >> 2][jj & 3];
-        ind[jj] = S[jj >> 2][jj & 3] > 0.f ? (bf16_t)1.f : (bf16_t)0.f;
-      }
-#pragma unroll
-      for (int dt = 0; dt < HD / 16; ++dt) {
-        // transposed LDS reads: each 16-lane group fetches a 4-key x 16-dim block row-wise and receives it column-wise
-        typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
-        const T* vrow = Vs + (4 * g + (li >> 2)) * LD + dt * 16 + 4 * (li & 3);
-        const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)vrow);
-        const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(vrow + 16 * LD));
-        bf16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-        f32x4 code = {0.f, 0.f, 0.f, 0.f};
-        if (odd) {
-          bf16x8 vc;
-#pragma unroll
-          for (int jj = 0; jj < 8; ++jj) {
-            const float c = odd_code((float)v[jj]);
-            vc[jj] = (bf16_t)c;
-            v[jj] = c == 0.f ? v[jj] : (bf16_t)0.f;
-          }
-          code = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, ind, code, 0, 0, 0);
-        }
-        O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb, O[dt], 0, 0, 0);
-        if (odd) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) O[dt][r] = odd_apply(O[dt][r], code[r]);
-        }
+        for (int r = 0; r < 4; ++r) O[dt][r] = odd_apply(O[dt][r], code[r]);
       }
     }
     __syncthreads();
   }
 
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  l = quad_sum(l);
   if (!live) return;
-  if (n_parts > 1 && a.n_split > 1) {
-    const int64_t at = ((int64_t)split * a.T + tok) * a.H + hq;
+  write_row<float, HD>(a, n_parts > 1 && a.n_split > 1, ((int64_t)split * a.T + tok) * a.H + hq, tok, hq, g, O, m, l);
+}
+
+// ---- few rows (one token and its head group, a handful of masked positions): 16 rows of one key head against a stream of
+// keys that is read once.  Bound by HBM; what counts is bytes in flight, so every wave streams tiles of its own -- tile t's
+// successor is on its way into the registers t is done with, the pages of the one behind it are looked up -- and waits for
+// nobody: K rows go from
+// memory into the first product's operand as they are, V through LDS of the wave's own for the transposed read.
+// WPP waves share one problem (tiles dealt out in turn, joined in LDS at the end); WPP = 1: four problems a workgroup.
+template <int HD, int WPP>
+__global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const PagedArgs a) {
+  constexpr int LD = HD + 8, NC = HD / 32, NW = WPP == 8 ? 8 : 4;   // NC: 16-byte chunks of a row a lane holds
+  __shared__ __attribute__((aligned(16))) bf16_t Vall[NW][PT_KEYS * LD];
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  bf16_t* Vs = Vall[wave];
+  int64_t id = WPP == 1 ? (int64_t)blockIdx.x * NW + wave : blockIdx.x;
+  if (WPP == 1 && id >= a.n_units) return;
+  const int split = (int)(id % a.n_split); id /= a.n_split;
+  const int tile = (int)(id % a.n_tiles); id /= a.n_tiles;
+  const int hk = (int)(id % a.Hk), b = (int)(id / a.Hk);
+  int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
+  t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
+  t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
+  const int64_t rows = (int64_t)(t1 - t0) * a.G;
+  const int64_t row0 = (int64_t)tile * 16;
+  if (row0 >= rows) return;
+  const int len = seq_len(a, b);
+  const int64_t row = row0 + li;
+  const bool live = row < rows;
+  const int tok = t0 + (int)((live ? row : row0) / a.G), hq = hk * a.G + (int)((live ? row : row0) % a.G);
+  int seen = live ? len : 0;   // keys this lane's row may look at
+  int hi = len, lo = len;
+  if (a.causal) {
+    if (live) {
+      const int64_t last = a.q_index ? (int64_t)a.q_index[tok] : (int64_t)len - (t1 - tok);
+      seen = last + 1 < len ? (last + 1 < 0 ? 0 : (int)(last + 1)) : len;
+    }
+    hi = seen;
+    lo = live ? seen : 0x7fffffff;
 #pragma unroll
-    for (int dt = 0; dt < HD / 16; ++dt) *(f32x4*)(a.part_o + at * HD + dt * 16 + 4 * g) = O[dt];
-    if (g == 0) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = l; }
-    return;
+    for (int o = 1; o < 16; o <<= 1) {
+      hi = max(hi, __shfl_xor(hi, o, 64));
+      lo = min(lo, __shfl_xor(lo, o, 64));
+    }
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    lo = __builtin_amdgcn_readfirstlane(lo);
   }
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);   // (a NaN sum stays one)
-  T* orow = (T*)a.out + tok * a.o_ts + hq * a.o_hs;
+  const int n_parts = len <= 0 ? 1 : (len + a.split_keys - 1) / a.split_keys;
+  if (split >= n_parts) return;
+  const int k_begin = split * a.split_keys;
+  const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
+
+  const bf16_t* qrow = (const bf16_t*)a.q + tok * a.q_ts + hq * a.q_hs;
+  bf16x8 qb[NC];
 #pragma unroll
-  for (int dt = 0; dt < HD / 16; ++dt)
-    store4(orow + dt * 16 + 4 * g, make_float4(O[dt][0] * inv, O[dt][1] * inv, O[dt][2] * inv, O[dt][3] * inv));
-  if (a.lse && g == 0) a.lse[(int64_t)tok * a.H + hq] = l > 0.f ? (m + log2f(l)) * 0.69314718055994530942f : (l == 0.f ? -INFINITY : l);
+  for (int i = 0; i < NC; ++i) qb[i] = *(const bf16x8*)(qrow + i * 32 + g * 8);
+
+  const int32_t* tab = a.table + b * a.table_stride;
+  const uint8_t* km = a.kmask ? a.kmask + b * a.mask_stride : nullptr;
+  const bf16_t* kbase = (const bf16_t*)a.k + (int64_t)hk * a.head_stride + g * 8;
+  const bf16_t* vbase = (const bf16_t*)a.v + (int64_t)hk * a.head_stride + g * 8;
+  const int pmask = (1 << a.page_log2) - 1;
+  // pages of this lane's two keys of a tile, -1 where the key is left out
+  auto lookup = [&](int k0, int (&pg)[2]) {
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      const int key = k0 + jt * 16 + li;
+      int p = -1;
+      if (key < k_end) {
+        p = tab[key >> a.page_log2];
+        if (km && km[key] == 0) p = -1;
+        if (p >= a.n_pages) p = -1;
+      }
+      pg[jt] = p;
+    }
+  };
+  // a lane's share of 32 rows (K or V); a key that is left out is read as zeros
+  auto fetch = [&](const bf16_t* base, int k0, const int (&pg)[2], bf16x8 (&x)[2][NC]) {
+    if (__all(pg[0] >= 0 && pg[1] >= 0)) {
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt) {
+        const bf16_t* p = base + (int64_t)pg[jt] * a.page_stride + (int64_t)((k0 + jt * 16 + li) & pmask) * a.slot_stride;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) x[jt][i] = *(const bf16x8*)(p + i * 32);
+      }
+    } else {
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) x[jt][i] = (bf16x8){};
+        if (pg[jt] >= 0) {
+          const bf16_t* p = base + (int64_t)pg[jt] * a.page_stride + (int64_t)((k0 + jt * 16 + li) & pmask) * a.slot_stride;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) x[jt][i] = *(const bf16x8*)(p + i * 32);
+        }
+      }
+    }
+  };
+
+  f32x4 O[HD / 16];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i) O[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  const int step = WPP * PT_KEYS;
+  int k0 = k_begin + (WPP == 1 ? 0 : wave * PT_KEYS);
+  int pg[2], pn[2], pnn[2];
+  bf16x8 kr[2][NC], vr[2][NC];
+  lookup(k0, pg);
+  lookup(k0 + step, pn);
+  fetch(kbase, k0, pg, kr);
+  fetch(vbase, k0, pg, vr);
+  for (; k0 < k_end; k0 += step) {
+    const bool all = __all(pg[0] >= 0 && pg[1] >= 0), partial = k0 + PT_KEYS > lo;
+    lookup(k0 + 2 * step, pnn);
+    // ---- S^T = K Q^T; K's registers then take the next tile's
+    f32x4 S[2];
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      S[jt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NC; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[jt][i], qb[i], S[jt], 0, 0, 0);
+    }
+    fetch(kbase, k0 + step, pn, kr);
+    // ---- V -> LDS (row = key, padded by 16 bytes: no bank conflict in either direction); V's registers likewise
+    bool odd = false;
+    if (partial) {
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) odd |= !(fabsf((float)vr[jt][i][e]) < INFINITY);
+      odd = __any(odd);
+    }
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int i = 0; i < NC; ++i) *(bf16x8*)(Vs + (jt * 16 + li) * LD + i * 32 + g * 8) = vr[jt][i];
+    fetch(vbase, k0 + step, pn, vr);
+    // ---- softmax
+    float mx = -INFINITY;
+    if (all && !partial) {
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          S[jt][r] *= a.scale_log2;
+          mx = fmaxf(mx, S[jt][r]);
+        }
+    } else {
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt) {
+        const unsigned on = (unsigned)__ballot(pg[jt] >= 0) >> (4 * g);   // (lanes 0..15 hold the tile's 16 keys)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool use = ((on >> r) & 1) && k0 + jt * 16 + 4 * g + r < seen;
+          S[jt][r] = use ? S[jt][r] * a.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, S[jt][r]);
+        }
+      }
+    }
+    mx = quad_max(mx);
+    if (__any(mx > m + kSlack)) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) O[i] *= alpha;
+    }
+    const float mz = m == -INFINITY ? 0.f : m;   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
+    bf16x8 pb;
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        S[jt][r] = __builtin_amdgcn_exp2f(S[jt][r] - mz);
+        l += S[jt][r];
+        pb[jt * 4 + r] = (bf16_t)S[jt][r];   // (rounded for the matrix instruction: relative 2^-8 a weight)
+      }
+    // ---- O^T += V^T P^T
+    wave_fence();   // lanes read what other lanes of the wave have written
+    if (odd) {
+      bf16x8 ind;
+#pragma unroll
+      for (int jj = 0; jj < 8; ++jj) ind[jj] = S[jj >> 2][jj & 3] > 0.f ? (bf16_t)1.f : (bf16_t)0.f;
+#pragma unroll
+      for (int dt = 0; dt < HD / 16; ++dt) {
+        const bf16x8 v = read_vt<LD>(Vs, li, g, dt);
+        bf16x8 vs = v, vc;
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) {
+          const float c = odd_code((float)v[jj]);
+          vc[jj] = (bf16_t)c;
+          vs[jj] = c == 0.f ? v[jj] : (bf16_t)0.f;
+        }
+        const f32x4 code = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, ind, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vs, pb, O[dt], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) O[dt][r] = odd_apply(O[dt][r], code[r]);
+      }
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < HD / 16; ++dt)
+        O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(read_vt<LD>(Vs, li, g, dt), pb, O[dt], 0, 0, 0);
+    }
+    wave_fence();
+    pg[0] = pn[0]; pg[1] = pn[1];
+    pn[0] = pnn[0]; pn[1] = pnn[1];
+  }
+  l = quad_sum(l);
+  const bool parts = n_parts > 1 && a.n_split > 1;
+  const int64_t at = ((int64_t)split * a.T + tok) * a.H + hq;
+  if constexpr (WPP == 1) {
+    if (!live) return;
+    write_row<bf16_t, HD>(a, parts, at, tok, hq, g, O, m, l);
+  } else {
+    // ---- join the waves: O [16][HD] fp32, then m and l of the 16 rows, in the wave's own LDS
+    float* mine = (float*)Vs;
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) *(f32x4*)(mine + li * HD + dt * 16 + 4 * g) = O[dt];
+    if (g == 0) { mine[16 * HD + li] = m; mine[16 * HD + 16 + li] = l; }
+    __syncthreads();
+    if (wave >= 4) return;      // 4 waves join: wave w the rows 4w .. 4w+3, a lane 4 (of 64) columns at a time
+    for (int r = wave * 4 + (lane >> 4); r < wave * 4 + 4; r += 4) {
+      if (row0 + r >= rows) continue;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WPP; ++w) mm = fmaxf(mm, ((const float*)Vall[w])[16 * HD + r]);
+      const float mz = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f;
+      f32x4 acc[(HD + 63) / 64] = {};
+      for (int w = 0; w < WPP; ++w) {
+        const float* o = (const float*)Vall[w];
+        const float f = __builtin_amdgcn_exp2f(o[16 * HD + r] - mz);
+        ll += o[16 * HD + 16 + r] * f;
+#pragma unroll
+        for (int c = 0; c < (HD + 63) / 64; ++c)
+          if (c * 64 + li * 4 < HD) acc[c] += *(const f32x4*)(o + r * HD + c * 64 + li * 4) * f;
+      }
+      const int tk = t0 + (int)((row0 + r) / a.G), h = hk * a.G + (int)((row0 + r) % a.G);
+      const int64_t pa = ((int64_t)split * a.T + tk) * a.H + h;
+      const float inv = parts ? 1.f : norm_of(ll);
+#pragma unroll
+      for (int c = 0; c < (HD + 63) / 64; ++c)
+        if (c * 64 + li * 4 < HD) {
+          if (parts) *(f32x4*)(a.part_o + pa * HD + c * 64 + li * 4) = acc[c];
+          else store4((bf16_t*)a.out + tk * a.o_ts + h * a.o_hs + c * 64 + li * 4,
+                      make_float4(acc[c][0] * inv, acc[c][1] * inv, acc[c][2] * inv, acc[c][3] * inv));
+        }
+      if (li == 0) {
+        if (parts) { a.part_ml[pa * 2] = mm; a.part_ml[pa * 2 + 1] = ll; }
+        else if (a.lse) a.lse[(int64_t)tk * a.H + h] = lse_of(mm, ll);
+      }
+    }
+  }
+}
+
+// ---- many rows (chunks of a prompt): 128 rows of one key head (32 a wave) against tiles of 64 keys that the workgroup's
+// four waves share through LDS, on 32 x 32 x 16 matrix instructions.  Two tile buffers: the next tile is written into LDS by
+// the memory pipe itself while this one is computed; one barrier a tile.
+// LDS rows are not padded (the direct writes are linear), their 16-byte chunks are permuted instead: by the row's number,
+// so that the 16 rows a K read touches at once, and the 4 rows of a transposed V read, lie in different banks.
+template <int HD> struct TileSwz {
+  static constexpr int CH = HD / 8;   // chunks of a row
+  // 128: 16 chunks = all banks; 64: two rows are; 96: rows start 4 chunks apart, K's chunks are rotated, V's are apart as is
+  __device__ static __forceinline__ int k_pos(int r, int c) {
+    if constexpr (HD == 96) { const int x = c + ((r >> 2) & 3); return x >= CH ? x - CH : x; }
+    else return c ^ (HD == 128 ? r & 15 : (r >> 1) & 7);
+  }
+  __device__ static __forceinline__ int k_chunk(int r, int pos) {
+    if constexpr (HD == 96) { const int x = pos - ((r >> 2) & 3); return x < 0 ? x + CH : x; }
+    else return k_pos(r, pos);
+  }
+  __device__ static __forceinline__ int v_pos(int r, int c) {
+    return HD == 96 ? c : c ^ (HD == 128 ? (r & 7) * 2 : ((r >> 1) & 3) * 2);
+  }
+};
+
+__device__ __attribute__((aligned(16))) const unsigned kZeroRow[64] = {};   // 256 bytes: the row of a key that is left out
+
+constexpr int TT_ROWS = 128, TT_KEYS = 64;
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
+  typedef TileSwz<HD> Z;
+  typedef __attribute__((address_space(3))) void lds_void;
+  typedef const __attribute__((address_space(1))) void gl_void;
+  typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+  constexpr int CH = Z::CH, TILE = TT_KEYS * HD * 2, NI = CH / 4;   // NI: 1-KB pieces of a tile that a wave brings in
+  extern __shared__ __attribute__((aligned(16))) char smem[];       // [2][K tile | V tile]
+  __shared__ int red[8];
+
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, c32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t id = blockIdx.x;
+  const int split = (int)(id % a.n_split); id /= a.n_split;
+  const int tile = (int)(id % a.n_tiles); id /= a.n_tiles;
+  const int hk = (int)(id % a.Hk), b = (int)(id / a.Hk);
+  int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
+  t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
+  t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
+  const int64_t rows = (int64_t)(t1 - t0) * a.G;
+  const int64_t row0 = (int64_t)tile * TT_ROWS;
+  if (row0 >= rows) return;
+  const int len = seq_len(a, b);
+  const int64_t row = row0 + wave * 32 + c32;
+  const bool live = row < rows;
+  const int tok = t0 + (int)((live ? row : row0) / a.G), hq = hk * a.G + (int)((live ? row : row0) % a.G);
+  int seen = live ? len : 0;   // keys this lane's row may look at
+  if (a.causal && live) {
+    const int64_t last = a.q_index ? (int64_t)a.q_index[tok] : (int64_t)len - (t1 - tok);
+    seen = last + 1 < len ? (last + 1 < 0 ? 0 : (int)(last + 1)) : len;
+  }
+  int whi = seen, wlo = live ? seen : 0x7fffffff;   // largest and smallest bound of the wave's rows, then the workgroup's
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    whi = max(whi, __shfl_xor(whi, o, 64));
+    wlo = min(wlo, __shfl_xor(wlo, o, 64));
+  }
+  whi = __builtin_amdgcn_readfirstlane(whi);
+  wlo = __builtin_amdgcn_readfirstlane(wlo);
+  if (lane == 0) { red[wave] = whi; red[4 + wave] = wlo; }
+  __syncthreads();
+  const int hi = __builtin_amdgcn_readfirstlane(max(max(red[0], red[1]), max(red[2], red[3])));
+  const int lo = __builtin_amdgcn_readfirstlane(min(min(red[4], red[5]), min(red[6], red[7])));
+  const int n_parts = len <= 0 ? 1 : (len + a.split_keys - 1) / a.split_keys;
+  if (split >= n_parts) return;
+  const int k_begin = split * a.split_keys;
+  const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
+
+  const bf16_t* qrow = (const bf16_t*)a.q + tok * a.q_ts + hq * a.q_hs;
+  bf16x8 qb[HD / 16];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i) qb[i] = *(const bf16x8*)(qrow + i * 16 + h * 8);
+
+  const int32_t* tab = a.table + b * a.table_stride;
+  const uint8_t* km = a.kmask ? a.kmask + b * a.mask_stride : nullptr;
+  const char* kbase = (const char*)((const bf16_t*)a.k + (int64_t)hk * a.head_stride);
+  const char* vbase = (const char*)((const bf16_t*)a.v + (int64_t)hk * a.head_stride);
+  const int pmask = (1 << a.page_log2) - 1;
+  // the page and the mask of key k0 + lane as they stand in memory (looked at one tile later, so that nothing waits here) ...
+  int raw_page = -1, raw_mask = 1;
+  auto look = [&](int k0) {
+    const int key = min(k0 + lane, k_end - 1);
+    raw_page = tab[key >> a.page_log2];
+    if (km) raw_mask = km[key];
+  };
+  // ... and where its row lies, in 16-byte units from its head's first; ~0: left out
+  auto place = [&](int k0) -> unsigned {
+    const int key = k0 + lane;
+    const bool on = key < k_end && raw_page >= 0 && raw_page < a.n_pages && raw_mask != 0;
+    return on ? (unsigned)(((int64_t)raw_page * a.page_stride + (int64_t)(key & pmask) * a.slot_stride) >> 3) : ~0u;
+  };
+  // this wave's pieces of a tile: lane l of piece n fills chunk (n * 4 + wave) * 64 + l of the tile
+  auto stage = [&](int buf, unsigned off) {
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int at = (n * 4 + wave) * 64 + lane, r = at / CH, pos = at - r * CH;
+      const unsigned o = __shfl(off, r, 64);
+      const bool on = o != ~0u;
+      const char* zr = (const char*)kZeroRow;
+      const char* kp = (on ? kbase + ((uint64_t)o << 4) : zr) + Z::k_chunk(r, pos) * 16;
+      const char* vp = (on ? vbase + ((uint64_t)o << 4) : zr) + Z::v_pos(r, pos) * 16;
+      char* to = smem + buf * (2 * TILE) + (n * 4 + wave) * 1024;
+      __builtin_amdgcn_global_load_lds((gl_void*)kp, (lds_void*)to, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gl_void*)vp, (lds_void*)(to + TILE), 16, 0, 0);
+    }
+  };
+
+  f32x16 O[HD / 32];
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) O[i] = (f32x16){};
+  float m = -INFINITY, l = 0.f;
+
+  // this lane's places in a tile: K chunk 2i + h of row c32, V rows 4h + li / 4, columns 16 x + 4 (li & 3) of 32
+  const int vr = 4 * h + (li >> 2), x = (lane >> 4) & 1;
+  int k_at[HD / 16], v_at[HD / 32];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i) k_at[i] = c32 * (HD * 2) + Z::k_pos(c32, 2 * i + h) * 16;
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) v_at[i] = TILE + vr * (HD * 2) + Z::v_pos(vr, 4 * i + 2 * x + ((li & 3) >> 1)) * 16 + (li & 1) * 8;
+
+  uint64_t on = 0, on_next = 0;   // which keys of the tile are used at all
+  if (k_begin < k_end) {          // (no direct write may be under way when the workgroup ends)
+    look(k_begin);
+    const unsigned off = place(k_begin);
+    on = __ballot(off != ~0u);
+    stage(0, off);
+    look(k_begin + TT_KEYS);
+  }
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += TT_KEYS, buf ^= 1) {
+    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): this wave's pieces of the tile are in LDS, its reads are done;
+    __builtin_amdgcn_s_barrier();         // everybody's are: the tile may be read, the other buffer refilled
+    if (k0 + TT_KEYS < k_end) {
+      const unsigned off = place(k0 + TT_KEYS);
+      on_next = __ballot(off != ~0u);
+      stage(buf ^ 1, off);
+      look(k0 + 2 * TT_KEYS);
+    }
+    const char* tl = smem + buf * (2 * TILE);
+    int odd = 0;
+    if (k0 + TT_KEYS > lo) {   // some row does not see all of this tile: infinities and NaN in V have to be looked for
+#pragma unroll
+      for (int n = 0; n < CH / 4; ++n) {
+        const bf16x8 v = *(const bf16x8*)(tl + TILE + (n * 256 + tid) * 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) odd |= !(fabsf((float)v[e]) < INFINITY);
+      }
+      odd = __syncthreads_or(odd);
+    }
+    // ---- S^T = K Q^T (a wave whose rows see nothing of the tile passes it by, but for the barriers)
+    f32x16 S[2];
+    if (k0 < whi) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        S[t] = (f32x16){};
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(tl + t * 32 * HD * 2 + k_at[i]), qb[i], S[t], 0, 0, 0);
+      }
+    }
+    if (odd) {   // (rare) V's infinities and NaN out of the tile, their codes in K's place
+      __syncthreads();
+#pragma unroll 1
+      for (int n = 0; n < CH / 4; ++n) {
+        bf16x8* pv = (bf16x8*)(smem + buf * (2 * TILE) + TILE + (n * 256 + tid) * 16);
+        bf16x8 v = *pv, c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float code = odd_code((float)v[e]);
+          c[e] = (bf16_t)code;
+          v[e] = code == 0.f ? v[e] : (bf16_t)0.f;
+        }
+        *pv = v;
+        *(bf16x8*)(smem + buf * (2 * TILE) + (n * 256 + tid) * 16) = c;
+      }
+      __syncthreads();
+    }
+    if (k0 < whi) {
+      // ---- softmax: this lane's keys are 32 t + (i & 3) + 8 (i >> 2) + 4 h
+      if (on != ~0ull || k0 + TT_KEYS > wlo) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const unsigned w = (unsigned)(on >> (32 * t)) >> (4 * h);
+          const int room = seen - (k0 + 32 * t + 4 * h);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = (i & 3) + 8 * (i >> 2);
+            if (!((w >> j) & 1) || j >= room) S[t][i] = -INFINITY;
+          }
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[t][i]);
+      mx = pair_max(mx) * a.scale_log2;
+      if (__any(mx > m + kSlack)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) O[i] *= alpha;
+      }
+      const float mz = m == -INFINITY ? 0.f : m;
+      bf16x8 pb[4];   // P^T, 16 keys each: rounded for the matrix instruction (relative 2^-8 a weight)
+      float ls[2] = {0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i], a.scale_log2, -mz));
+          ls[i & 1] += e;
+          pb[2 * t + (i >> 3)][i & 7] = (bf16_t)e;
+        }
+      l += ls[0] + ls[1];
+      // ---- O^T += V^T P^T
+      auto read_v = [&](const char* at, int s, int dt) {
+        const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at + s * 16 * HD * 2 + v_at[dt]));
+        const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(at + (s * 16 + 8) * HD * 2 + v_at[dt]));
+        return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt) O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_v(tl, s, dt), pb[s], O[dt], 0, 0, 0);
+      if (odd) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int jj = 0; jj < 8; ++jj) pb[s][jj] = (float)pb[s][jj] > 0.f ? (bf16_t)1.f : (bf16_t)0.f;
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt) {
+          f32x16 code = {};
+#pragma unroll
+          for (int s = 0; s < 4; ++s) code = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_v(tl - TILE, s, dt), pb[s], code, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) O[dt][i] = odd_apply(O[dt][i], code[i]);
+        }
+      }
+    }
+    on = on_next;
+  }
+  l = pair_sum(l);
+  if (!live) return;
+  const bool parts = n_parts > 1 && a.n_split > 1;
+  const int64_t at = ((int64_t)split * a.T + tok) * a.H + hq;
+  const float inv = norm_of(l);
+  bf16_t* orow = (bf16_t*)a.out + tok * a.o_ts + hq * a.o_hs;
+#pragma unroll
+  for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = dt * 32 + 8 * i + 4 * h;
+      const f32x4 o = {O[dt][4 * i], O[dt][4 * i + 1], O[dt][4 * i + 2], O[dt][4 * i + 3]};
+      if (parts) *(f32x4*)(a.part_o + at * HD + d) = o;
+      else store4(orow + d, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
+    }
+  if (h == 0) {
+    if (parts) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = l; }
+    else if (a.lse) a.lse[(int64_t)tok * a.H + hq] = lse_of(m, l);
+  }
 }
 
 // ---- joins the parts of a split key axis: one wave per (token, head)
@@ -294,40 +823,45 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
       o[1] += v.y * f;
     }
   }
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  const float inv = norm_of(l);
   if (lane * 2 < HD) {
     T* d = (T*)a.out + tok * a.o_ts + h * a.o_hs + lane * 2;
     d[0] = ElemTraits<T>::from_f32(o[0] * inv);
     d[1] = ElemTraits<T>::from_f32(o[1] * inv);
   }
-  if (a.lse && lane == 0) a.lse[row] = l > 0.f ? (m + log2f(l)) * 0.69314718055994530942f : (l == 0.f ? -INFINITY : l);
+  if (a.lse && lane == 0) a.lse[row] = lse_of(m, l);
 }
 
 struct PagedPlan {
+  int few;               // waves a problem in paged_few_kernel, 0 = paged_attn_kernel
   int n_tiles, n_split, split_keys;
   int64_t ws_o, ws_ml;   // bytes
 };
 
 static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   PagedPlan s;
-  const int G = p->n_heads / p->kv.n_kv_heads;
-  s.n_tiles = (int)(((int64_t)p->max_q * G + PT_ROWS - 1) / PT_ROWS);
+  const int64_t rows = (int64_t)p->max_q * (p->n_heads / p->kv.n_kv_heads);
+  const int64_t heads = (int64_t)p->kv.n_kv_heads * p->n_seqs;
+  s.few = 0;
+  if (p->kv.dtype == DARK_BF16 && rows <= 16) s.few = p->max_kv <= 128 ? 1 : (heads <= 64 && p->max_kv <= 1024) ? 8 : 4;
+  const int tile_rows = s.few ? 16 : p->kv.dtype == DARK_BF16 ? TT_ROWS : PT_ROWS;
+  s.n_tiles = (int)((rows + tile_rows - 1) / tile_rows);
   if (s.n_tiles < 1) s.n_tiles = 1;
-  const int64_t wgs = (int64_t)s.n_tiles * p->kv.n_kv_heads * p->n_seqs;
+  const int64_t wgs = (int64_t)s.n_tiles * heads;
   // enough workgroups for 256 CUs x 4, parts of 256 keys at least
   int64_t want = (1024 + wgs - 1) / (wgs > 0 ? wgs : 1);
   const int64_t most = (p->max_kv + 255) / 256;
   if (want > most) want = most;
-  if (want < 1) want = 1;
+  if (want < 1 || s.few == 1 || s.few == 8) want = 1;
   s.split_keys = (int)(((p->max_kv + want - 1) / want + 63) / 64 * 64);
   if (s.split_keys < 64) s.split_keys = 64;
   s.n_split = (int)((p->max_kv + s.split_keys - 1) / s.split_keys);
   if (s.n_split < 1) s.n_split = 1;
   s.ws_o = s.ws_ml = 0;
   if (s.n_split > 1) {
-    const int64_t rows = (int64_t)s.n_split * p->n_tokens * p->n_heads;
-    s.ws_o = (int64_t)align_up((size_t)rows * p->kv.head_dim * 4, 256);
-    s.ws_ml = (int64_t)align_up((size_t)rows * 8, 256);
+    const int64_t n = (int64_t)s.n_split * p->n_tokens * p->n_heads;
+    s.ws_o = (int64_t)align_up((size_t)n * p->kv.head_dim * 4, 256);
+    s.ws_ml = (int64_t)align_up((size_t)n * 8, 256);
   }
   return s;
 }
@@ -340,7 +874,10 @@ static int check_paged_attention(const dark_paged_attention_args* p) {
                  "%s: n_heads=%d must be a multiple of n_kv_heads=%d", who, p->n_heads, p->kv.n_kv_heads);
   DARK_CHECK_ARG(p->n_tokens >= 0 && p->n_seqs >= 0 && p->table_width >= 0 && p->max_q >= 0 && p->max_kv >= 0 &&
                      p->n_tokens < (1 << 30), "%s: negative or too large size", who);
-  DARK_CHECK_ARG((int64_t)p->table_width * p->kv.page_size < (1ll << 31) - 64 && p->max_kv < 0x7fffffc0, "%s: more than 2^31 keys a sequence", who);
+  DARK_CHECK_ARG((int64_t)p->table_width * p->kv.page_size < (1ll << 30) && p->max_kv < (1 << 30), "%s: 2^30 keys a sequence or more", who);
+  // (rows are addressed by 32-bit offsets in 16-byte units: 64 GiB of keys a layer)
+  DARK_CHECK_ARG((double)p->kv.page_stride * (p->kv.n_pages > 0 ? p->kv.n_pages - 1 : 0) + (double)p->kv.slot_stride * p->kv.page_size <
+                     8.0 * 4294967295.0 / (p->kv.dtype == DARK_BF16 ? 1 : 2), "%s: the cache spans more than 64 GiB", who);
   DARK_CHECK_ARG(p->scale == p->scale && fabsf(p->scale) < INFINITY, "%s: scale is not finite", who);
   return DARK_OK;
 }
@@ -389,19 +926,34 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   a.scale_log2 = p->scale * 1.44269504088896340736f;
   const int64_t wgs = (int64_t)s.n_tiles * p->kv.n_kv_heads * p->n_seqs * s.n_split;
   DARK_CHECK_ARG(wgs < (1ll << 31), "%s: %lld workgroups", who, (long long)wgs);
-  const dim3 grid((unsigned)wgs), block(256), jgrid((unsigned)(((int64_t)p->n_tokens * p->n_heads + 3) / 4));
-#define DARK_PAGED(T, HDv)                                                                          \
+  a.n_units = wgs;
+  const dim3 grid((unsigned)(s.few == 1 ? (wgs + 3) / 4 : wgs)), block(s.few == 8 ? 512 : 256), jblock(256), jgrid((unsigned)(((int64_t)p->n_tokens * p->n_heads + 3) / 4));
+#define DARK_PAGED_BF16(HDv)                                                                        \
   do {                                                                                              \
-    hipLaunchKernelGGL((paged_attn_kernel<T, HDv>), grid, block, 0, st, a);                         \
-    if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<T, HDv>), jgrid, block, 0, st, a);     \
+    if (s.few == 1) hipLaunchKernelGGL((paged_few_kernel<HDv, 1>), grid, block, 0, st, a);          \
+    else if (s.few == 4) hipLaunchKernelGGL((paged_few_kernel<HDv, 4>), grid, block, 0, st, a);     \
+    else if (s.few == 8) hipLaunchKernelGGL((paged_few_kernel<HDv, 8>), grid, block, 0, st, a);     \
+    else {                                                                                          \
+      constexpr int lds = 4 * TT_KEYS * HDv * 2;                                                    \
+      static SmemOptIn optin;                                                                       \
+      DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv>, lds, st));                         \
+      hipLaunchKernelGGL((paged_tile_kernel<HDv>), grid, block, lds, st, a);                        \
+    }                                                                                               \
+    if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<bf16_t, HDv>), jgrid, jblock, 0, st, a); \
+  } while (0)
+#define DARK_PAGED_F32(HDv)                                                                         \
+  do {                                                                                              \
+    hipLaunchKernelGGL((paged_attn_kernel<HDv>), grid, block, 0, st, a);                            \
+    if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<float, HDv>), jgrid, jblock, 0, st, a); \
   } while (0)
   const int HD = p->kv.head_dim;
   if (p->kv.dtype == DARK_BF16) {
-    if (HD == 64) DARK_PAGED(bf16_t, 64); else if (HD == 96) DARK_PAGED(bf16_t, 96); else DARK_PAGED(bf16_t, 128);
+    if (HD == 64) DARK_PAGED_BF16(64); else if (HD == 96) DARK_PAGED_BF16(96); else DARK_PAGED_BF16(128);
   } else {
-    if (HD == 64) DARK_PAGED(float, 64); else if (HD == 96) DARK_PAGED(float, 96); else DARK_PAGED(float, 128);
+    if (HD == 64) DARK_PAGED_F32(64); else if (HD == 96) DARK_PAGED_F32(96); else DARK_PAGED_F32(128);
   }
-#undef DARK_PAGED
+#undef DARK_PAGED_BF16
+#undef DARK_PAGED_F32
   DARK_CHECK_LAUNCH();
   return DARK_OK;
 }

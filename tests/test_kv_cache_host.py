@@ -60,7 +60,7 @@ def test_kv_append_refuses(kw, msg):
 
 @pytest.mark.parametrize("kw,msg", [(dict(n_heads=9), "multiple"), (dict(kv=_kv(head_dim=32)), "head_dim"), (dict(q=None), "null pointer"),
                                     (dict(block_table=None), "null pointer"), (dict(max_kv=-1), "negative"), (dict(scale=math.inf), "scale"),
-                                    (dict(o_ts=4), "16 bytes"), (dict(table_stride=1), "table_stride"), (dict(table_width=1 << 28), "2^31"),
+                                    (dict(o_ts=4), "16 bytes"), (dict(table_stride=1), "table_stride"), (dict(table_width=1 << 28), "2^30"),
                                     (dict(max_kv=100000), "workspace")])
 def test_paged_attention_refuses(kw, msg):
     f = dict(kv=_kv(), q=4096, out=8192, block_table=4096, cu_q=4096, kv_len=4096, q_ts=768, q_hs=96, o_ts=768, o_hs=96,

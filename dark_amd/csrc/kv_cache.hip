@@ -2,10 +2,11 @@
 // key / value cache.  The three jobs are one kernel: a token's rows (heads of q, k and v) are read once, normed and
 // rotated in fp32 registers and stored once, wherever they belong.
 //
-// Bound by HBM: 2 * (heads read) * head_dim elements a token against ~8 flops an element.  One wave per token: a row is
-// held by LPR lanes, lane c of them with the 16 bytes at chunk c of the row's first half and of its second half -- the
-// two elements of every rotated pair in one lane -- so the 64 / LPR rows of one pass need no exchange but the norm's sum
-// (log2(LPR) xor-shuffles), and the token's cos / sin, read once, serve all its heads.
+// Bound by HBM: 2 * (heads read) * head_dim elements a token against ~8 flops an element.  A row is held by LPR lanes, lane
+// c of them with the 16 bytes at chunk c of the row's first half and of its second half -- the two elements of every rotated
+// pair in one lane -- so the 64 / LPR rows of a pass need no exchange but the norm's sum (log2(LPR) xor-shuffles).  A wave
+// keeps its pass (which heads, hence its pointers, strides and weights) and walks over the tokens, the next one's rows,
+// rotation and, one further, position on their way while it computes.
 #include "common.h"
 
 namespace dark {
@@ -21,7 +22,7 @@ struct RowsArgs {
   int64_t src_ts[3], src_hs[3], dst_ts[3], dst_hs[3];
   int64_t page_stride, n_slots;
   int32_t T, h_end[3];        // rows [0, h_end[0]) are q heads, then k heads, then v heads
-  int32_t max_pos, page_log2;
+  int32_t max_pos, page_log2, n_pass, t_step;   // passes of a token, tokens under way at a time
   float eps;
 };
 
@@ -50,85 +51,113 @@ template <> struct RowVec<float> {
   __device__ static __forceinline__ raw down(const float (&f)[4]) { return (raw){f[0], f[1], f[2], f[3]}; }
 };
 
-template <typename T, int HD>
+template <typename T, int HD, bool NORM>
 __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
   constexpr int N = RowVec<T>::N, HALF = HD / 2, CH = HALF / N;         // CH lanes hold a row
   constexpr int LPR = CH <= 4 ? 4 : CH <= 8 ? 8 : 16, RPP = 64 / LPR;   // lanes a row is given, rows of one pass
   typedef typename RowVec<T>::raw raw;
   const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= a.T) return;
-  const int c = lane & (LPR - 1), r0 = lane / LPR;
-  const bool on = c < CH;
-  const int cc = on ? c : 0;
-  float cs[N], sn[N], wq[2 * N], wk[2 * N];
+  const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pass = unit % a.n_pass, step = a.t_step;
+  int t = unit / a.n_pass;
+  if (t >= step || t >= a.T) return;
+  const int c = lane & (LPR - 1), r = pass * RPP + lane / LPR;
+  const bool on = c < CH && r < a.h_end[2];
+  const int role = r < a.h_end[0] ? 0 : r < a.h_end[1] ? 1 : 2;
+  const int h = on ? r - (role == 0 ? 0 : role == 1 ? a.h_end[0] : a.h_end[1]) : 0, at = on ? c * N : 0;
+  const T* src = (const T*)(role == 0 ? a.src[0] : role == 1 ? a.src[1] : a.src[2]) +
+                 h * (role == 0 ? a.src_hs[0] : role == 1 ? a.src_hs[1] : a.src_hs[2]) + at;
+  const int64_t src_ts = role == 0 ? a.src_ts[0] : role == 1 ? a.src_ts[1] : a.src_ts[2];
+  T* dst = (T*)(role == 0 ? a.dst[0] : role == 1 ? a.dst[1] : a.dst[2]) +
+           h * (role == 0 ? a.dst_hs[0] : role == 1 ? a.dst_hs[1] : a.dst_hs[2]) + at;
+  const int64_t dst_ts = role == 0 ? a.dst_ts[0] : role == 1 ? a.dst_ts[1] : a.dst_ts[2];
+  const bool paged = role > 0 && a.slots, turned = role < 2 && a.cosT;
+  const float* wp = role == 0 ? a.w[0] : role == 1 ? a.w[1] : nullptr;
+  float w[2 * N];
+  if constexpr (NORM) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
-  if (a.cosT) {
-    int p = a.pos[t];
-    p = p < 0 ? 0 : (p >= a.max_pos ? a.max_pos - 1 : p);
-    const float* cp = a.cosT + (int64_t)p * HALF + cc * N;
-    const float* sp = a.sinT + (int64_t)p * HALF + cc * N;
-#pragma unroll
-    for (int i = 0; i < N; ++i) { cs[i] = cp[i]; sn[i] = sp[i]; }
+    for (int i = 0; i < N; ++i) {
+      w[i] = wp ? wp[at + i] : 1.f;
+      w[N + i] = wp ? wp[HALF + at + i] : 1.f;
+    }
   }
-  int64_t slot = -1;
-  if (a.slots) {
-    slot = a.slots[t];
-    if (slot >= a.n_slots) slot = -1;
-  }
-  const int64_t in_cache = slot < 0 ? 0 : (slot >> a.page_log2) * a.page_stride;
-  const int64_t in_page = slot < 0 ? 0 : slot & (((int64_t)1 << a.page_log2) - 1);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    wq[i] = a.w[0] ? a.w[0][cc * N + i] : 1.f;
-    wq[N + i] = a.w[0] ? a.w[0][HALF + cc * N + i] : 1.f;
-    wk[i] = a.w[1] ? a.w[1][cc * N + i] : 1.f;
-    wk[N + i] = a.w[1] ? a.w[1][HALF + cc * N + i] : 1.f;
-  }
-  const int rows = a.h_end[2];
-  for (int r = r0; r < rows + r0; r += RPP) {   // (the same trip count for every lane: the shuffles need whole groups)
-    const bool live = r < rows;
-    const int role = !live ? 0 : (r < a.h_end[0] ? 0 : r < a.h_end[1] ? 1 : 2);
-    const int h = r - (role == 0 ? 0 : a.h_end[role - 1]);
-    raw x1 = {}, x2 = {};
-    if (live && on) {
-      const T* s = (const T*)a.src[role] + t * a.src_ts[role] + h * a.src_hs[role] + c * N;
+  raw x1 = {}, x2 = {};
+  float cs[N], sn[N];
+  int p = 0, p_next = 0;
+  int64_t slot = 0;
+  auto position = [&](int tt) {
+    if (!turned || tt >= a.T) return 0;
+    const int q = a.pos[tt];
+    return q < 0 ? 0 : (q >= a.max_pos ? a.max_pos - 1 : q);
+  };
+  auto fetch = [&](int tt, int pp) {
+    if (on) {
+      const T* s = src + tt * src_ts;
       x1 = *(const raw*)s;
       x2 = *(const raw*)(s + HALF);
     }
-    raw y1 = x1, y2 = x2;
-    if (role < 2) {
-      float f1[N], f2[N], o1[N], o2[N];
-      RowVec<T>::up(x1, f1);
-      RowVec<T>::up(x2, f2);
-      if (a.w[role]) {
-        float ss = 0.f;
+    if (paged) slot = a.slots[tt];
+    if (turned) {
+      const float* cp = a.cosT + (int64_t)pp * HALF + at;
+      const float* sp = a.sinT + (int64_t)pp * HALF + at;
 #pragma unroll
-        for (int i = 0; i < N; ++i) ss += f1[i] * f1[i] + f2[i] * f2[i];
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          f1[i] *= inv * (role ? wk[i] : wq[i]);
-          f2[i] *= inv * (role ? wk[N + i] : wq[N + i]);
-        }
+      for (int i = 0; i < N; i += 4) {
+        *(f32x4*)(cs + i) = *(const f32x4*)(cp + i);
+        *(f32x4*)(sn + i) = *(const f32x4*)(sp + i);
       }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < N; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
+  p = position(t);
+  p_next = position(t + step);
+  fetch(t, p);
+  while (true) {
+    // this token's rows and rotation, then its successor's take their place
+    raw y1 = x1, y2 = x2;
+    float cc[N], ss[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) { cc[i] = cs[i]; ss[i] = sn[i]; }
+    const int64_t to = slot;
+    const int tn = t + step;
+    if (tn < a.T) {
+      fetch(tn, p_next);
+      p_next = position(tn + step);
+    }
+    float f1[N], f2[N], o1[N], o2[N];
+    RowVec<T>::up(y1, f1);
+    RowVec<T>::up(y2, f2);
+    if constexpr (NORM) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum += f1[i] * f1[i] + f2[i] * f2[i];
+      if (!on) sum = 0.f;   // (lanes without a chunk of the row)
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      const float inv = wp ? 1.0f / sqrtf(sum / (float)HD + a.eps) : 1.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        o1[i] = f1[i] * cs[i] - f2[i] * sn[i];
-        o2[i] = f2[i] * cs[i] + f1[i] * sn[i];
+        f1[i] *= inv * w[i];
+        f2[i] *= inv * w[N + i];
       }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      o1[i] = f1[i] * cc[i] - f2[i] * ss[i];
+      o2[i] = f2[i] * cc[i] + f1[i] * ss[i];
+    }
+    if (role < 2) {   // (values are carried as they are)
       y1 = RowVec<T>::down(o1);
       y2 = RowVec<T>::down(o2);
     }
-    const bool paged = role > 0 && a.slots;
-    if (live && on && (!paged || slot >= 0)) {
-      T* d = (T*)a.dst[role] + (paged ? in_cache + in_page * a.dst_ts[role] : t * a.dst_ts[role]) + h * a.dst_hs[role] + c * N;
+    const bool kept = !paged || (to >= 0 && to < a.n_slots);
+    if (on && kept) {
+      T* d = dst + (paged ? (to >> a.page_log2) * a.page_stride + (to & (((int64_t)1 << a.page_log2) - 1)) * dst_ts : t * dst_ts);
       *(raw*)d = y1;
       *(raw*)(d + HALF) = y2;
     }
+    if (tn >= a.T) return;
+    t = tn;
   }
 }
 
@@ -163,10 +192,20 @@ int check_paged_kv(const dark_paged_kv* kv, const char* who) {
   return DARK_OK;
 }
 
-static int launch_head_rows(const RowsArgs& a, int dtype, int HD, hipStream_t st) {
+static int launch_head_rows(RowsArgs& a, int dtype, int HD, hipStream_t st) {
   DARK_TRY(check_stream_device(st));
-  const dim3 grid((unsigned)cdiv(a.T, 4)), block(256);
-#define DARK_ROWS(T, HDv) hipLaunchKernelGGL((head_rows_kernel<T, HDv>), grid, block, 0, st, a)
+  const int ch = HD / 2 / (dtype == DARK_BF16 ? 8 : 4), rpp = 64 / (ch <= 4 ? 4 : ch <= 8 ? 8 : 16);
+  a.n_pass = cdiv(a.h_end[2], rpp);
+  // 256 CUs x 32 waves walk over the tokens
+  const int most = cdiv(8192, a.n_pass);
+  a.t_step = a.T < most ? a.T : most;
+  const dim3 grid((unsigned)cdiv(a.t_step * a.n_pass, 4)), block(256);
+  const bool norm = a.w[0] || a.w[1];
+#define DARK_ROWS(T, HDv)                                                                           \
+  do {                                                                                              \
+    if (norm) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true>), grid, block, 0, st, a);          \
+    else hipLaunchKernelGGL((head_rows_kernel<T, HDv, false>), grid, block, 0, st, a);              \
+  } while (0)
   if (dtype == DARK_BF16) {
     if (HD == 64) DARK_ROWS(bf16_t, 64); else if (HD == 96) DARK_ROWS(bf16_t, 96); else DARK_ROWS(bf16_t, 128);
   } else {

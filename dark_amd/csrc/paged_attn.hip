@@ -27,10 +27,17 @@ struct PagedArgs {
   const uint8_t* kmask;
   float *part_o, *part_ml;     // [n_split][T][H][HD], [n_split][T][H][2]; null when n_split == 1
   int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride, page_stride, slot_stride, head_stride;
-  int32_t T, H, Hk, G, B, width, n_pages, page_log2, causal, n_split, split_keys, n_tiles, cap;
-  int64_t n_units;             // problems of the launch: sequences x key heads x row tiles x parts
+  int32_t T, H, Hk, G, B, width, n_pages, page_log2, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
   float scale_log2;            // scale * log2(e)
 };
+
+// Workgroups are handed to the eight XCDs, each with an L2 of its own, in turn.  `n_inner` units that follow each other and
+// read the same memory (row tiles of a key head; key heads of one token row) go to one XCD: unit number of this workgroup.
+__device__ __forceinline__ int unit_of_block(const PagedArgs& a) {
+  if (a.n_inner <= 1) return blockIdx.x;
+  const int xcd = blockIdx.x & 7, k = blockIdx.x >> 3, group = k / a.n_inner;
+  return (group * 8 + xcd) * a.n_inner + (k - group * a.n_inner);
+}
 
 // keys of a sequence: what it says, within the table and the caller's bound (hence within the mask's rows)
 __device__ __forceinline__ int seq_len(const PagedArgs& a, int b) {
@@ -104,7 +111,7 @@ __device__ __forceinline__ void write_row(const PagedArgs& a, bool parts, int64_
     return;
   }
   const float inv = norm_of(l);
-  T* orow = (T*)a.out + tok * a.o_ts + hq * a.o_hs;
+  T* orow = (T*)a.out + (int64_t)tok * a.o_ts + hq * a.o_hs;
 #pragma unroll
   for (int dt = 0; dt < HD / 16; ++dt)
     store4(orow + dt * 16 + 4 * g, make_float4(O[dt][0] * inv, O[dt][1] * inv, O[dt][2] * inv, O[dt][3] * inv));
@@ -116,6 +123,8 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+
+__device__ __attribute__((aligned(16))) const unsigned kZeroRow[64] = {};   // 256 bytes: the row of a key that is left out
 
 constexpr int PT_ROWS = 64, PT_KEYS = 32;   // rows of a workgroup (16 a wave), keys of a tile
 
@@ -130,21 +139,22 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
   __shared__ int red[8];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, g = lane >> 4;
-  int bid = blockIdx.x;
-  const int split = bid % a.n_split; bid /= a.n_split;
-  const int tile = bid % a.n_tiles; bid /= a.n_tiles;
-  const int hk = bid % a.Hk, b = bid / a.Hk;
+  int id = unit_of_block(a);
+  if (id < 0 || id >= a.n_units) return;
+  const int tile = id % a.n_tiles; id /= a.n_tiles;
+  const int split = id % a.n_split; id /= a.n_split;
+  const int hk = id % a.Hk, b = id / a.Hk;
   int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
   t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
-  const int64_t rows = (int64_t)(t1 - t0) * a.G;
-  const int64_t row0 = (int64_t)tile * PT_ROWS;
+  const int rows = (t1 - t0) * a.G;
+  const int row0 = tile * PT_ROWS;
   if (row0 >= rows) return;
   const int len = seq_len(a, b);
 
-  const int64_t row = row0 + wave * 16 + li;
+  const int row = row0 + wave * 16 + li;
   const bool live = row < rows;
-  const int tok = t0 + (int)((live ? row : row0) / a.G), hq = hk * a.G + (int)((live ? row : row0) % a.G);
+  const int ri = (live ? row : row0) / a.G, tok = t0 + ri, hq = hk * a.G + (live ? row : row0) - ri * a.G;
   int seen = live ? len : 0;   // keys this lane's row may look at
   if (a.causal && live) {
     const int64_t last = a.q_index ? (int64_t)a.q_index[tok] : (int64_t)len - (t1 - tok);
@@ -165,7 +175,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
   const int k_begin = split * a.split_keys;
   const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
 
-  const float* qrow = (const float*)a.q + tok * a.q_ts + hq * a.q_hs;
+  const float* qrow = (const float*)a.q + (int64_t)tok * a.q_ts + hq * a.q_hs;
   float qf[HD / 4];
 #pragma unroll
   for (int i = 0; i < HD / 4; ++i) qf[i] = qrow[i * 4 + g];
@@ -276,21 +286,22 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   bf16_t* Vs = Vall[wave];
-  int64_t id = WPP == 1 ? (int64_t)blockIdx.x * NW + wave : blockIdx.x;
-  if (WPP == 1 && id >= a.n_units) return;
-  const int split = (int)(id % a.n_split); id /= a.n_split;
-  const int tile = (int)(id % a.n_tiles); id /= a.n_tiles;
-  const int hk = (int)(id % a.Hk), b = (int)(id / a.Hk);
+  int id = unit_of_block(a);
+  if (WPP == 1) id = id * NW + wave;
+  if (id < 0 || id >= a.n_units) return;
+  const int hk = id % a.Hk; id /= a.Hk;      // (the key heads of a token lie next to each other)
+  const int tile = id % a.n_tiles; id /= a.n_tiles;
+  const int split = id % a.n_split, b = id / a.n_split;
   int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
   t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
-  const int64_t rows = (int64_t)(t1 - t0) * a.G;
-  const int64_t row0 = (int64_t)tile * 16;
+  const int rows = (t1 - t0) * a.G;
+  const int row0 = tile * 16;
   if (row0 >= rows) return;
   const int len = seq_len(a, b);
-  const int64_t row = row0 + li;
+  const int row = row0 + li;
   const bool live = row < rows;
-  const int tok = t0 + (int)((live ? row : row0) / a.G), hq = hk * a.G + (int)((live ? row : row0) % a.G);
+  const int ri = (live ? row : row0) / a.G, tok = t0 + ri, hq = hk * a.G + (live ? row : row0) - ri * a.G;
   int seen = live ? len : 0;   // keys this lane's row may look at
   int hi = len, lo = len;
   if (a.causal) {
@@ -313,7 +324,7 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
   const int k_begin = split * a.split_keys;
   const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
 
-  const bf16_t* qrow = (const bf16_t*)a.q + tok * a.q_ts + hq * a.q_hs;
+  const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)tok * a.q_ts + hq * a.q_hs;
   bf16x8 qb[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) qb[i] = *(const bf16x8*)(qrow + i * 32 + g * 8);
@@ -323,40 +334,31 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
   const bf16_t* kbase = (const bf16_t*)a.k + (int64_t)hk * a.head_stride + g * 8;
   const bf16_t* vbase = (const bf16_t*)a.v + (int64_t)hk * a.head_stride + g * 8;
   const int pmask = (1 << a.page_log2) - 1;
-  // pages of this lane's two keys of a tile, -1 where the key is left out
-  auto lookup = [&](int k0, int (&pg)[2]) {
+  // pages and masks of this lane's two keys of a tile as they stand in memory: looked at two tiles ahead and made sense of
+  // one tile ahead, so that nothing waits for them
+  int rp[2], rm[2] = {1, 1};
+  auto look = [&](int k0) {
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt) {
-      const int key = k0 + jt * 16 + li;
-      int p = -1;
-      if (key < k_end) {
-        p = tab[key >> a.page_log2];
-        if (km && km[key] == 0) p = -1;
-        if (p >= a.n_pages) p = -1;
-      }
-      pg[jt] = p;
+      const int key = min(k0 + jt * 16 + li, k_end - 1);
+      rp[jt] = tab[key >> a.page_log2];
+      if (km) rm[jt] = km[key];
     }
+  };
+  // page of a key, -1 where it is left out
+  auto place = [&](int k0, int (&pg)[2]) {
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+      pg[jt] = (k0 + jt * 16 + li < k_end && rp[jt] < a.n_pages && rm[jt] != 0) ? rp[jt] : -1;
   };
   // a lane's share of 32 rows (K or V); a key that is left out is read as zeros
   auto fetch = [&](const bf16_t* base, int k0, const int (&pg)[2], bf16x8 (&x)[2][NC]) {
-    if (__all(pg[0] >= 0 && pg[1] >= 0)) {
 #pragma unroll
-      for (int jt = 0; jt < 2; ++jt) {
-        const bf16_t* p = base + (int64_t)pg[jt] * a.page_stride + (int64_t)((k0 + jt * 16 + li) & pmask) * a.slot_stride;
+    for (int jt = 0; jt < 2; ++jt) {
+      const bf16_t* p = base + (int64_t)pg[jt] * a.page_stride + (int64_t)((k0 + jt * 16 + li) & pmask) * a.slot_stride;
+      if (pg[jt] < 0) p = (const bf16_t*)kZeroRow + g * 8;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) x[jt][i] = *(const bf16x8*)(p + i * 32);
-      }
-    } else {
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) x[jt][i] = (bf16x8){};
-        if (pg[jt] >= 0) {
-          const bf16_t* p = base + (int64_t)pg[jt] * a.page_stride + (int64_t)((k0 + jt * 16 + li) & pmask) * a.slot_stride;
-#pragma unroll
-          for (int i = 0; i < NC; ++i) x[jt][i] = *(const bf16x8*)(p + i * 32);
-        }
-      }
+      for (int i = 0; i < NC; ++i) x[jt][i] = *(const bf16x8*)(p + i * 32);
     }
   };
 
@@ -367,15 +369,18 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
 
   const int step = WPP * PT_KEYS;
   int k0 = k_begin + (WPP == 1 ? 0 : wave * PT_KEYS);
-  int pg[2], pn[2], pnn[2];
+  int pg[2], pn[2];
   bf16x8 kr[2][NC], vr[2][NC];
-  lookup(k0, pg);
-  lookup(k0 + step, pn);
-  fetch(kbase, k0, pg, kr);
-  fetch(vbase, k0, pg, vr);
+  if (k0 < k_end) {
+    look(k0);
+    place(k0, pg);
+    fetch(kbase, k0, pg, kr);
+    fetch(vbase, k0, pg, vr);
+    look(k0 + step);
+  }
   for (; k0 < k_end; k0 += step) {
     const bool all = __all(pg[0] >= 0 && pg[1] >= 0), partial = k0 + PT_KEYS > lo;
-    lookup(k0 + 2 * step, pnn);
+    place(k0 + step, pn);
     // ---- S^T = K Q^T; K's registers then take the next tile's
     f32x4 S[2];
 #pragma unroll
@@ -385,6 +390,7 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
       for (int i = 0; i < NC; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[jt][i], qb[i], S[jt], 0, 0, 0);
     }
     fetch(kbase, k0 + step, pn, kr);
+    look(k0 + 2 * step);
     // ---- V -> LDS (row = key, padded by 16 bytes: no bank conflict in either direction); V's registers likewise
     bool odd = false;
     if (partial) {
@@ -470,7 +476,6 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
     }
     wave_fence();
     pg[0] = pn[0]; pg[1] = pn[1];
-    pn[0] = pnn[0]; pn[1] = pnn[1];
   }
   l = quad_sum(l);
   const bool parts = n_parts > 1 && a.n_split > 1;
@@ -502,14 +507,14 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
         for (int c = 0; c < (HD + 63) / 64; ++c)
           if (c * 64 + li * 4 < HD) acc[c] += *(const f32x4*)(o + r * HD + c * 64 + li * 4) * f;
       }
-      const int tk = t0 + (int)((row0 + r) / a.G), h = hk * a.G + (int)((row0 + r) % a.G);
+      const int ti = (row0 + r) / a.G, tk = t0 + ti, h = hk * a.G + (row0 + r) - ti * a.G;
       const int64_t pa = ((int64_t)split * a.T + tk) * a.H + h;
       const float inv = parts ? 1.f : norm_of(ll);
 #pragma unroll
       for (int c = 0; c < (HD + 63) / 64; ++c)
         if (c * 64 + li * 4 < HD) {
           if (parts) *(f32x4*)(a.part_o + pa * HD + c * 64 + li * 4) = acc[c];
-          else store4((bf16_t*)a.out + tk * a.o_ts + h * a.o_hs + c * 64 + li * 4,
+          else store4((bf16_t*)a.out + (int64_t)tk * a.o_ts + h * a.o_hs + c * 64 + li * 4,
                       make_float4(acc[c][0] * inv, acc[c][1] * inv, acc[c][2] * inv, acc[c][3] * inv));
         }
       if (li == 0) {
@@ -541,8 +546,6 @@ template <int HD> struct TileSwz {
   }
 };
 
-__device__ __attribute__((aligned(16))) const unsigned kZeroRow[64] = {};   // 256 bytes: the row of a key that is left out
-
 constexpr int TT_ROWS = 128, TT_KEYS = 64;
 
 template <int HD>
@@ -557,20 +560,21 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
 
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, c32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int64_t id = blockIdx.x;
-  const int split = (int)(id % a.n_split); id /= a.n_split;
-  const int tile = (int)(id % a.n_tiles); id /= a.n_tiles;
-  const int hk = (int)(id % a.Hk), b = (int)(id / a.Hk);
+  int id = unit_of_block(a);
+  if (id < 0 || id >= a.n_units) return;
+  const int tile = id % a.n_tiles; id /= a.n_tiles;   // (the tiles of a key head read the same keys)
+  const int split = id % a.n_split; id /= a.n_split;
+  const int hk = id % a.Hk, b = id / a.Hk;
   int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
   t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
-  const int64_t rows = (int64_t)(t1 - t0) * a.G;
-  const int64_t row0 = (int64_t)tile * TT_ROWS;
+  const int rows = (t1 - t0) * a.G;
+  const int row0 = tile * TT_ROWS;
   if (row0 >= rows) return;
   const int len = seq_len(a, b);
-  const int64_t row = row0 + wave * 32 + c32;
+  const int row = row0 + wave * 32 + c32;
   const bool live = row < rows;
-  const int tok = t0 + (int)((live ? row : row0) / a.G), hq = hk * a.G + (int)((live ? row : row0) % a.G);
+  const int ri = (live ? row : row0) / a.G, tok = t0 + ri, hq = hk * a.G + (live ? row : row0) - ri * a.G;
   int seen = live ? len : 0;   // keys this lane's row may look at
   if (a.causal && live) {
     const int64_t last = a.q_index ? (int64_t)a.q_index[tok] : (int64_t)len - (t1 - tok);
@@ -593,7 +597,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   const int k_begin = split * a.split_keys;
   const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
 
-  const bf16_t* qrow = (const bf16_t*)a.q + tok * a.q_ts + hq * a.q_hs;
+  const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)tok * a.q_ts + hq * a.q_hs;
   bf16x8 qb[HD / 16];
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) qb[i] = *(const bf16x8*)(qrow + i * 16 + h * 8);
@@ -677,13 +681,25 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
     // ---- S^T = K Q^T (a wave whose rows see nothing of the tile passes it by, but for the barriers)
     f32x16 S[2];
     if (k0 < whi) {
+      bf16x8 kf[2][HD / 16];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        S[t] = (f32x16){};
+      for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
-          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(tl + t * 32 * HD * 2 + k_at[i]), qb[i], S[t], 0, 0, 0);
+        for (int t = 0; t < 2; ++t) kf[t][i] = *(const bf16x8*)(tl + t * 32 * HD * 2 + k_at[i]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) S[t] = (f32x16){};
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[t][i], qb[i], S[t], 0, 0, 0);
+      // four LDS reads ahead of the matrix instructions, then one for one
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < HD / 8 - 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
     if (odd) {   // (rare) V's infinities and NaN out of the tile, their codes in K's place
       __syncthreads();
@@ -774,7 +790,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   const bool parts = n_parts > 1 && a.n_split > 1;
   const int64_t at = ((int64_t)split * a.T + tok) * a.H + hq;
   const float inv = norm_of(l);
-  bf16_t* orow = (bf16_t*)a.out + tok * a.o_ts + hq * a.o_hs;
+  bf16_t* orow = (bf16_t*)a.out + (int64_t)tok * a.o_ts + hq * a.o_hs;
 #pragma unroll
   for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
@@ -790,44 +806,54 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   }
 }
 
-// ---- joins the parts of a split key axis: one wave per (token, head)
-template <typename T, int HD>
+// ---- joins the parts of a split key axis: WPR waves a (token, head), each an equal share of the parts (4 where there are
+// many: the parts are then read side by side and not one after the other)
+template <typename T, int HD, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.T * a.H) return;
-  const int tok = (int)(row / a.H), h = (int)(row - (int64_t)tok * a.H);
-  // the token's sequence: the last b with cu_q[b] <= tok
-  int lo = 0, hi = a.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] <= tok) lo = mid; else hi = mid;
-  }
-  if (tok < a.cu_q[lo] || tok >= a.cu_q[lo + 1]) return;
-  const int len = seq_len(a, lo);
+  __shared__ float so[4][HD], sl[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = a.max_q * a.H, id = WPR == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+  const int b = id / per, r = id - b * per, i = r / a.H, h = r - i * a.H;
+  if (b >= a.B) return;
+  const int t0 = a.cu_q[b], t1 = a.cu_q[b + 1], len = seq_len(a, b);
+  const int tok = t0 + i;
+  if (tok < 0 || tok >= t1 || tok >= a.T) return;
   const int n_all = len <= 0 ? 1 : (len + a.split_keys - 1) / a.split_keys;
   if (n_all <= 1) return;                       // written whole by the first kernel
   const int n = min(n_all, a.n_split);
-  const int64_t step = (int64_t)a.T * a.H;
+  const int64_t step = (int64_t)a.T * a.H, row = (int64_t)tok * a.H + h;
   float m = -INFINITY;
-  for (int s = 0; s < n; ++s) m = fmaxf(m, a.part_ml[(s * step + row) * 2]);
+  for (int s = lane; s < n; s += 64) m = fmaxf(m, a.part_ml[(s * step + row) * 2]);
+  m = wave_max(m);
   const float mz = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[2] = {0.f, 0.f};
-  for (int s = 0; s < n; ++s) {                 // (in order: the same bits every time)
+  const bool on = lane * 2 < HD;
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 4
+  for (int s = WPR == 4 ? wave : 0; s < n; s += WPR) {   // (every part in its fixed place: the same bits every time)
     const int64_t at = s * step + row;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[at * 2] - mz);
-    l += a.part_ml[at * 2 + 1] * f;
-    if (lane * 2 < HD) {
-      const float2 v = *(const float2*)(a.part_o + at * HD + lane * 2);
-      o[0] += v.x * f;
-      o[1] += v.y * f;
+    const float2 ml = *(const float2*)(a.part_ml + at * 2);
+    const float2 v = on ? *(const float2*)(a.part_o + at * HD + lane * 2) : make_float2(0.f, 0.f);
+    const float f = __builtin_amdgcn_exp2f(ml.x - mz);
+    l += ml.y * f;
+    o0 += v.x * f;
+    o1 += v.y * f;
+  }
+  T* orow = (T*)a.out + (int64_t)tok * a.o_ts + h * a.o_hs;
+  if constexpr (WPR == 4) {
+    if (on) { so[wave][lane * 2] = o0; so[wave][lane * 2 + 1] = o1; }
+    if (lane == 0) sl[wave] = l;
+    __syncthreads();
+    if (wave > 0) return;
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    if (on) {
+      o0 = (so[0][lane * 2] + so[1][lane * 2]) + (so[2][lane * 2] + so[3][lane * 2]);
+      o1 = (so[0][lane * 2 + 1] + so[1][lane * 2 + 1]) + (so[2][lane * 2 + 1] + so[3][lane * 2 + 1]);
     }
   }
   const float inv = norm_of(l);
-  if (lane * 2 < HD) {
-    T* d = (T*)a.out + tok * a.o_ts + h * a.o_hs + lane * 2;
-    d[0] = ElemTraits<T>::from_f32(o[0] * inv);
-    d[1] = ElemTraits<T>::from_f32(o[1] * inv);
+  if (on) {
+    orow[lane * 2] = ElemTraits<T>::from_f32(o0 * inv);
+    orow[lane * 2 + 1] = ElemTraits<T>::from_f32(o1 * inv);
   }
   if (a.lse && lane == 0) a.lse[row] = lse_of(m, l);
 }
@@ -848,12 +874,17 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   s.n_tiles = (int)((rows + tile_rows - 1) / tile_rows);
   if (s.n_tiles < 1) s.n_tiles = 1;
   const int64_t wgs = (int64_t)s.n_tiles * heads;
-  // enough workgroups for 256 CUs x 4, parts of 256 keys at least
-  int64_t want = (1024 + wgs - 1) / (wgs > 0 ? wgs : 1);
-  const int64_t most = (p->max_kv + 255) / 256;
-  if (want > most) want = most;
-  if (want < 1 || s.few == 1 || s.few == 8) want = 1;
-  s.split_keys = (int)(((p->max_kv + want - 1) / want + 63) / 64 * 64);
+  // Parts of a key axis.  Few problems: 512 of them fill the card (2 x 4 over 131072, 16 problems: 191 us with parts of 4096
+  // to 8192 keys, 197 with 2048: the join costs more).  Many, as with one token for each of many sequences: parts of 1024,
+  // because lengths differ and the longest must not finish alone (64 x 1 over 16384: 517 us, 580 with parts of 2048, 637
+  // with 8192).  Never below 256 keys: a part's (O, m, l) is then 1/16 of the keys' bytes at most.
+  int64_t keys = p->max_kv;
+  if (s.few != 1 && s.few != 8) {
+    if (wgs < 512) keys = (p->max_kv * wgs + 511) / 512;
+    if (s.few && wgs >= 256 && keys > 1024) keys = 1024;
+    if (keys < 256) keys = 256;
+  }
+  s.split_keys = (int)((keys + 63) / 64 * 64);
   if (s.split_keys < 64) s.split_keys = 64;
   s.n_split = (int)((p->max_kv + s.split_keys - 1) / s.split_keys);
   if (s.n_split < 1) s.n_split = 1;
@@ -878,6 +909,8 @@ static int check_paged_attention(const dark_paged_attention_args* p) {
   // (rows are addressed by 32-bit offsets in 16-byte units: 64 GiB of keys a layer)
   DARK_CHECK_ARG((double)p->kv.page_stride * (p->kv.n_pages > 0 ? p->kv.n_pages - 1 : 0) + (double)p->kv.slot_stride * p->kv.page_size <
                      8.0 * 4294967295.0 / (p->kv.dtype == DARK_BF16 ? 1 : 2), "%s: the cache spans more than 64 GiB", who);
+  const int64_t G = p->n_heads / p->kv.n_kv_heads;
+  DARK_CHECK_ARG(p->n_tokens * G < (1ll << 31) - 128 && p->max_q * G < (1ll << 31) - 128, "%s: 2^31 rows of a key head or more", who);
   DARK_CHECK_ARG(p->scale == p->scale && fabsf(p->scale) < INFINITY, "%s: scale is not finite", who);
   return DARK_OK;
 }
@@ -925,9 +958,21 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   a.cap = (int)(cap < p->max_kv ? cap : p->max_kv);
   a.scale_log2 = p->scale * 1.44269504088896340736f;
   const int64_t wgs = (int64_t)s.n_tiles * p->kv.n_kv_heads * p->n_seqs * s.n_split;
-  DARK_CHECK_ARG(wgs < (1ll << 31), "%s: %lld workgroups", who, (long long)wgs);
-  a.n_units = wgs;
-  const dim3 grid((unsigned)(s.few == 1 ? (wgs + 3) / 4 : wgs)), block(s.few == 8 ? 512 : 256), jblock(256), jgrid((unsigned)(((int64_t)p->n_tokens * p->n_heads + 3) / 4));
+  DARK_CHECK_ARG(wgs < (1ll << 30), "%s: %lld workgroups", who, (long long)wgs);
+  a.n_units = (int)wgs;
+  // units that share memory on one XCD, where there are enough such groups for all eight
+  int blocks = s.few == 1 ? (int)((wgs + 3) / 4) : (int)wgs;
+  a.n_inner = s.few == 1 ? p->kv.n_kv_heads / 4 : s.few ? p->kv.n_kv_heads : s.n_tiles;
+  const int groups = a.n_inner > 1 ? cdiv(blocks, a.n_inner) : 0;
+  if (groups % 8 == 0 || groups >= 64) blocks = a.n_inner > 1 ? cdiv(groups, 8) * 8 * a.n_inner : blocks;
+  else a.n_inner = 1;
+  a.max_q = p->max_q;
+  DARK_CHECK_ARG(s.n_split == 1 || (int64_t)p->n_seqs * p->max_q * p->n_heads < (1ll << 31), "%s: too many rows", who);
+  const dim3 grid((unsigned)blocks), block(s.few == 8 ? 512 : 256), jblock(256);
+  const unsigned jrows = (unsigned)((int64_t)p->n_seqs * p->max_q * p->n_heads);
+#define DARK_JOIN(T, HDv)                                                                           \
+  if (s.n_split > 8) hipLaunchKernelGGL((paged_join_kernel<T, HDv, 4>), dim3(jrows), jblock, 0, st, a);  \
+  else if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<T, HDv, 1>), dim3((jrows + 3) / 4), jblock, 0, st, a)
 #define DARK_PAGED_BF16(HDv)                                                                        \
   do {                                                                                              \
     if (s.few == 1) hipLaunchKernelGGL((paged_few_kernel<HDv, 1>), grid, block, 0, st, a);          \
@@ -939,12 +984,12 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
       DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv>, lds, st));                         \
       hipLaunchKernelGGL((paged_tile_kernel<HDv>), grid, block, lds, st, a);                        \
     }                                                                                               \
-    if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<bf16_t, HDv>), jgrid, jblock, 0, st, a); \
+    DARK_JOIN(bf16_t, HDv);                                                                         \
   } while (0)
 #define DARK_PAGED_F32(HDv)                                                                         \
   do {                                                                                              \
     hipLaunchKernelGGL((paged_attn_kernel<HDv>), grid, block, 0, st, a);                            \
-    if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<float, HDv>), jgrid, jblock, 0, st, a); \
+    DARK_JOIN(float, HDv);                                                                          \
   } while (0)
   const int HD = p->kv.head_dim;
   if (p->kv.dtype == DARK_BF16) {
@@ -952,6 +997,7 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   } else {
     if (HD == 64) DARK_PAGED_F32(64); else if (HD == 96) DARK_PAGED_F32(96); else DARK_PAGED_F32(128);
   }
+#undef DARK_JOIN
 #undef DARK_PAGED_BF16
 #undef DARK_PAGED_F32
   DARK_CHECK_LAUNCH();

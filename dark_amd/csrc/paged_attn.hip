@@ -19,6 +19,27 @@ namespace dark {
 int check_paged_kv(const dark_paged_kv* kv, const char* who);
 int check_stream_device(hipStream_t st);
 
+// n / d for 0 <= n < 2^31 as one multiplication (a division by a run-time number is some 30 instructions, and a kernel of a
+// few microseconds is fetched from memory as it runs): m = ceil(2^(31 + s) / d), s = ceil(log2 d), n m / 2^(31 + s) is exact.
+struct Div {
+  uint32_t d, m, s;
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s); }
+  __device__ __forceinline__ int divmod(int& n) const {   // quotient; n becomes the remainder
+    const int q = div(n);
+    n -= q * (int)d;
+    return q;
+  }
+};
+static Div make_div(int d) {
+  Div x = {(uint32_t)d, 0, 0};
+  while ((1ll << x.s) < d) ++x.s;
+  if (d > 1) {
+    x.m = (uint32_t)(((1ull << (31 + x.s)) + d - 1) / d);
+    x.s -= 1;
+  }
+  return x;
+}
+
 struct PagedArgs {
   const void *q, *k, *v;
   void* out;
@@ -28,6 +49,7 @@ struct PagedArgs {
   float *part_o, *part_ml;     // [n_split][T][H][HD], [n_split][T][H][2]; null when n_split == 1
   int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride, page_stride, slot_stride, head_stride;
   int32_t T, H, Hk, G, B, width, n_pages, page_log2, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
+  Div by_hk, by_tiles, by_split, by_group, by_inner, by_heads, by_rows;   // by_rows: max_q * n_heads
   float scale_log2;            // scale * log2(e)
 };
 
@@ -35,8 +57,9 @@ struct PagedArgs {
 // read the same memory (row tiles of a key head; key heads of one token row) go to one XCD: unit number of this workgroup.
 __device__ __forceinline__ int unit_of_block(const PagedArgs& a) {
   if (a.n_inner <= 1) return blockIdx.x;
-  const int xcd = blockIdx.x & 7, k = blockIdx.x >> 3, group = k / a.n_inner;
-  return (group * 8 + xcd) * a.n_inner + (k - group * a.n_inner);
+  int k = blockIdx.x >> 3;
+  const int group = a.by_inner.divmod(k);
+  return (group * 8 + (blockIdx.x & 7)) * a.n_inner + k;
 }
 
 // keys of a sequence: what it says, within the table and the caller's bound (hence within the mask's rows)
@@ -48,7 +71,7 @@ __device__ __forceinline__ int seq_len(const PagedArgs& a, int b) {
 // Infinities and NaN of a V row that some row of the tile must not see (P = 0 there): 0 * inf would be NaN.  They are taken
 // out of the product and counted by a second one over P's indicator, +inf as 1, -inf as 128, NaN as both (at most 64 keys a
 // tile; 129 is a bf16), and added to the rows that do see them.
-__device__ __forceinline__ float odd_code(float x) { return x != x ? 129.f : x == INFINITY ? 1.f : x == -INFINITY ? 128.f : 0.f; }
+__device__ __forceinline__ float odd_code(float x) { return (x == INFINITY ? 1.f : 0.f) + (x == -INFINITY ? 128.f : 0.f) + (x != x ? 129.f : 0.f); }
 __device__ __forceinline__ float odd_apply(float acc, float code) {
   const float neg = floorf(code * 0.0078125f), pos = __builtin_fmaf(neg, -128.f, code);
   acc += pos > 0.f ? INFINITY : 0.f;
@@ -124,153 +147,101 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __attribute__((aligned(16))) const unsigned kZeroRow[64] = {};   // 256 bytes: the row of a key that is left out
+__device__ __attribute__((aligned(16))) const unsigned kZeroRow[128] = {};   // 512 bytes, the longest row: a key that is left out
 
-constexpr int PT_ROWS = 64, PT_KEYS = 32;   // rows of a workgroup (16 a wave), keys of a tile
+constexpr int PT_KEYS = 32;   // keys of a streamed tile
 
-// ---- fp32: 64 rows of one key head (16 a wave) against tiles of 32 keys in LDS, on 16 x 16 x 4 fp32 matrix instructions.
-template <int HD>
-__global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
-  constexpr int VEC = 4, LD = HD + VEC, CH = HD / VEC, NT = PT_KEYS / 16;
-  typedef f32x4 raw;
-  __shared__ __attribute__((aligned(16))) float Ks[PT_KEYS * LD];
-  __shared__ __attribute__((aligned(16))) float Vs[PT_KEYS * LD];
-  __shared__ float kbias[PT_KEYS];
-  __shared__ int red[8];
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, g = lane >> 4;
-  int id = unit_of_block(a);
-  if (id < 0 || id >= a.n_units) return;
-  const int tile = id % a.n_tiles; id /= a.n_tiles;
-  const int split = id % a.n_split; id /= a.n_split;
-  const int hk = id % a.Hk, b = id / a.Hk;
-  int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
+// ---- what a wave of the streaming kernels works on: 16 rows of one key head against a part of its sequence's keys
+struct Unit {
+  int b, hk, split, t0, row0, rows, tok, hq;   // row0: first of the 16; tok, hq: this lane's row (lane & 15)
+  int seen, lo, n_parts, k_begin, k_end;       // keys the row may look at; the fewest any row may; > 1: the axis is split
+  bool live;
+};
+__device__ __forceinline__ bool open_unit(const PagedArgs& a, int id, int li, Unit& u) {
+  int q = a.by_hk.divmod(id);
+  u.hk = id;                         // (the key heads of a token lie next to each other)
+  id = a.by_tiles.divmod(q);
+  const int tile = q;
+  u.b = a.by_split.divmod(id);
+  u.split = id;
+  int t0 = a.cu_q[u.b], t1 = a.cu_q[u.b + 1];
+  const int len = seq_len(a, u.b);
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
   t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
-  const int rows = (t1 - t0) * a.G;
-  const int row0 = tile * PT_ROWS;
-  if (row0 >= rows) return;
-  const int len = seq_len(a, b);
-
-  const int row = row0 + wave * 16 + li;
-  const bool live = row < rows;
-  const int ri = (live ? row : row0) / a.G, tok = t0 + ri, hq = hk * a.G + (live ? row : row0) - ri * a.G;
-  int seen = live ? len : 0;   // keys this lane's row may look at
-  if (a.causal && live) {
-    const int64_t last = a.q_index ? (int64_t)a.q_index[tok] : (int64_t)len - (t1 - tok);
-    seen = last + 1 < len ? (last + 1 < 0 ? 0 : (int)(last + 1)) : len;
-  }
-  int hi = seen, lo = live ? seen : 0x7fffffff;   // largest and smallest bound of the workgroup's rows
+  u.t0 = t0;
+  u.rows = (t1 - t0) * a.G;
+  u.row0 = tile * 16;
+  if (u.row0 >= u.rows) return false;
+  const int row = u.row0 + li;
+  u.live = row < u.rows;
+  const int rr = u.live ? row : u.row0, ri = a.by_group.div(rr);
+  u.tok = t0 + ri;
+  u.hq = u.hk * a.G + rr - ri * a.G;
+  u.seen = u.live ? len : 0;
+  int hi = len;
+  u.lo = len;
+  if (a.causal) {
+    auto clip = [&](int64_t last) { return last + 1 < len ? (last + 1 < 0 ? 0 : (int)(last + 1)) : len; };
+    if (a.q_index) {
+      u.seen = u.live ? clip(a.q_index[u.tok]) : 0;
+      hi = u.seen;
+      u.lo = u.live ? u.seen : 0x7fffffff;
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    hi = max(hi, __shfl_xor(hi, o, 64));
-    lo = min(lo, __shfl_xor(lo, o, 64));
-  }
-  if (lane == 0) { red[wave] = hi; red[4 + wave] = lo; }
-  __syncthreads();
-  hi = max(max(red[0], red[1]), max(red[2], red[3]));
-  lo = min(min(red[4], red[5]), min(red[6], red[7]));
-  const int n_parts = len <= 0 ? 1 : (len + a.split_keys - 1) / a.split_keys;   // parts of this sequence that hold keys
-  if (split >= n_parts) return;
-  const int k_begin = split * a.split_keys;
-  const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
-
-  const float* qrow = (const float*)a.q + (int64_t)tok * a.q_ts + hq * a.q_hs;
-  float qf[HD / 4];
-#pragma unroll
-  for (int i = 0; i < HD / 4; ++i) qf[i] = qrow[i * 4 + g];
-
-  f32x4 O[HD / 16];
-#pragma unroll
-  for (int i = 0; i < HD / 16; ++i) O[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  const int32_t* tab = a.table + b * a.table_stride;
-  const uint8_t* km = a.kmask ? a.kmask + b * a.mask_stride : nullptr;
-
-  for (int k0 = k_begin; k0 < k_end; k0 += PT_KEYS) {
-    // ---- K and V of the tile; a key that no row may use is stored as zeros
-    int odd = 0;
-    for (int it = tid; it < PT_KEYS * CH; it += 256) {
-      const int j = it / CH, c = it - j * CH;
-      const int key = k0 + j;
-      raw rk = {}, rv = {};
-      bool on = key < hi && (!km || km[key] != 0);
-      int page = on ? tab[key >> a.page_log2] : -1;
-      on = on && page >= 0 && page < a.n_pages;
-      if (on) {
-        const int64_t off = (int64_t)page * a.page_stride + (int64_t)(key & ((1 << a.page_log2) - 1)) * a.slot_stride +
-                            (int64_t)hk * a.head_stride + c * VEC;
-        rk = *(const raw*)((const float*)a.k + off);
-        rv = *(const raw*)((const float*)a.v + off);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) odd |= !(fabsf(rv[e]) < INFINITY);
+      for (int o = 1; o < 16; o <<= 1) {
+        hi = max(hi, __shfl_xor(hi, o, 64));
+        u.lo = min(u.lo, __shfl_xor(u.lo, o, 64));
       }
-      *(raw*)(Ks + j * LD + c * VEC) = rk;
-      *(raw*)(Vs + j * LD + c * VEC) = rv;
-      if (c == 0) kbias[j] = on ? 0.f : -INFINITY;
+      hi = __builtin_amdgcn_readfirstlane(hi);
+      u.lo = __builtin_amdgcn_readfirstlane(u.lo);
+    } else {   // the sequence's last places: rows see more and more
+      const int n = t1 - t0, last_row = min(u.row0 + 15, u.rows - 1);
+      if (u.live) u.seen = clip((int64_t)len - n + ri);
+      u.lo = clip((int64_t)len - n + a.by_group.div(u.row0));
+      hi = clip((int64_t)len - n + a.by_group.div(last_row));
     }
-    const bool partial = k0 + PT_KEYS > lo;   // some row does not see all of this tile
-    odd = __syncthreads_or(odd && partial);
-
-    f32x4 S[NT];
-    float mx = m;
-#pragma unroll
-    for (int jt = 0; jt < NT; ++jt) {
-      S[jt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      const float* kr = Ks + (jt * 16 + li) * LD;
-#pragma unroll
-      for (int i = 0; i < HD / 4; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i * 4 + g], qf[i], S[jt], 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = jt * 16 + 4 * g + r;
-        const float s = (kbias[j] == 0.f && k0 + j < seen) ? S[jt][r] * a.scale_log2 : -INFINITY;
-        S[jt][r] = s;
-        mx = fmaxf(mx, s);
-      }
-    }
-    mx = quad_max(mx);
-    const float mz = mx == -INFINITY ? 0.f : mx;   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
-    const float alpha = __builtin_amdgcn_exp2f(m - mz);
-    m = mx;
-    float sum = 0.f;
-#pragma unroll
-    for (int jt = 0; jt < NT; ++jt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        S[jt][r] = __builtin_amdgcn_exp2f(S[jt][r] - mz);
-        sum += S[jt][r];
-      }
-    l = l * alpha + sum;   // (this lane's keys only: the four lanes of a row are added up at the end)
-#pragma unroll
-    for (int i = 0; i < HD / 16; ++i) O[i] *= alpha;
-
-    // ---- O^T += V^T P^T
-#pragma unroll
-    for (int dt = 0; dt < HD / 16; ++dt) {
-      f32x4 code = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int jt = 0; jt < NT; ++jt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v = Vs[(jt * 16 + 4 * g + r) * LD + dt * 16 + li];
-          if (odd) {
-            const float c = odd_code(v);
-            code = __builtin_amdgcn_mfma_f32_16x16x4f32(c, S[jt][r] > 0.f ? 1.f : 0.f, code, 0, 0, 0);
-            v = c == 0.f ? v : 0.f;
-          }
-          O[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, S[jt][r], O[dt], 0, 0, 0);
-        }
-      if (odd) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) O[dt][r] = odd_apply(O[dt][r], code[r]);
-      }
-    }
-    __syncthreads();
   }
+  u.n_parts = len <= a.split_keys ? 1 : 2;   // (one, or more)
+  u.k_begin = u.split * a.split_keys;
+  if (u.split > 0 && u.k_begin >= len) return false;
+  u.k_end = min(hi, u.split == a.n_split - 1 ? hi : u.k_begin + a.split_keys);
+  return true;
+}
 
-  l = quad_sum(l);
-  if (!live) return;
-  write_row<float, HD>(a, n_parts > 1 && a.n_split > 1, ((int64_t)split * a.T + tok) * a.H + hq, tok, hq, g, O, m, l);
+// ---- joins the WPP waves of a workgroup, whose (O [16][HD], m [16], l [16]) lie where `of(wave)` says: wave w of the first
+// four the rows 4 w .. 4 w + 3, a lane four columns of each 64
+template <typename T, int HD, int WPP, typename Of>
+__device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit& u, bool parts, int wave, int lane, Of of) {
+  const int li = lane & 15, r = wave * 4 + (lane >> 4);
+  if (wave >= 4 || u.row0 + r >= u.rows) return;
+  float mm = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < WPP; ++w) mm = fmaxf(mm, of(w)[16 * HD + r]);
+  const float mz = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f;
+  f32x4 acc[(HD + 63) / 64] = {};
+#pragma unroll
+  for (int w = 0; w < WPP; ++w) {
+    const float* o = of(w);
+    const float f = __builtin_amdgcn_exp2f(o[16 * HD + r] - mz);
+    ll += o[16 * HD + 16 + r] * f;
+#pragma unroll
+    for (int c = 0; c < (HD + 63) / 64; ++c)
+      if (c * 64 + li * 4 < HD) acc[c] += *(const f32x4*)(o + r * HD + c * 64 + li * 4) * f;
+  }
+  const int ti = a.by_group.div(u.row0 + r), tk = u.t0 + ti, h = u.hk * a.G + (u.row0 + r) - ti * a.G;
+  const int64_t pa = ((int64_t)u.split * a.T + tk) * a.H + h;
+  const float inv = parts ? 1.f : norm_of(ll);
+#pragma unroll
+  for (int c = 0; c < (HD + 63) / 64; ++c)
+    if (c * 64 + li * 4 < HD) {
+      if (parts) *(f32x4*)(a.part_o + pa * HD + c * 64 + li * 4) = acc[c];
+      else store4((T*)a.out + (int64_t)tk * a.o_ts + h * a.o_hs + c * 64 + li * 4,
+                  make_float4(acc[c][0] * inv, acc[c][1] * inv, acc[c][2] * inv, acc[c][3] * inv));
+    }
+  if (li == 0) {
+    if (parts) { a.part_ml[pa * 2] = mm; a.part_ml[pa * 2 + 1] = ll; }
+    else if (a.lse) a.lse[(int64_t)tk * a.H + h] = lse_of(mm, ll);
+  }
 }
 
 // ---- few rows (one token and its head group, a handful of masked positions): 16 rows of one key head against a stream of
@@ -280,7 +251,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedArgs a) {
 // memory into the first product's operand as they are, V through LDS of the wave's own for the transposed read.
 // WPP waves share one problem (tiles dealt out in turn, joined in LDS at the end); WPP = 1: four problems a workgroup.
 template <int HD, int WPP>
-__global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_few_kernel(const PagedArgs a) {
   constexpr int LD = HD + 8, NC = HD / 32, NW = WPP == 8 ? 8 : 4;   // NC: 16-byte chunks of a row a lane holds
   __shared__ __attribute__((aligned(16))) bf16_t Vall[NW][PT_KEYS * LD];
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
@@ -289,54 +260,23 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
   int id = unit_of_block(a);
   if (WPP == 1) id = id * NW + wave;
   if (id < 0 || id >= a.n_units) return;
-  const int hk = id % a.Hk; id /= a.Hk;      // (the key heads of a token lie next to each other)
-  const int tile = id % a.n_tiles; id /= a.n_tiles;
-  const int split = id % a.n_split, b = id / a.n_split;
-  int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
-  t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
-  t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
-  const int rows = (t1 - t0) * a.G;
-  const int row0 = tile * 16;
-  if (row0 >= rows) return;
-  const int len = seq_len(a, b);
-  const int row = row0 + li;
-  const bool live = row < rows;
-  const int ri = (live ? row : row0) / a.G, tok = t0 + ri, hq = hk * a.G + (live ? row : row0) - ri * a.G;
-  int seen = live ? len : 0;   // keys this lane's row may look at
-  int hi = len, lo = len;
-  if (a.causal) {
-    if (live) {
-      const int64_t last = a.q_index ? (int64_t)a.q_index[tok] : (int64_t)len - (t1 - tok);
-      seen = last + 1 < len ? (last + 1 < 0 ? 0 : (int)(last + 1)) : len;
-    }
-    hi = seen;
-    lo = live ? seen : 0x7fffffff;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      hi = max(hi, __shfl_xor(hi, o, 64));
-      lo = min(lo, __shfl_xor(lo, o, 64));
-    }
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    lo = __builtin_amdgcn_readfirstlane(lo);
-  }
-  const int n_parts = len <= 0 ? 1 : (len + a.split_keys - 1) / a.split_keys;
-  if (split >= n_parts) return;
-  const int k_begin = split * a.split_keys;
-  const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
+  Unit u;
+  if (!open_unit(a, id, li, u)) return;
+  const int k_begin = u.k_begin, k_end = u.k_end, seen = u.seen, lo = u.lo;
 
-  const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)tok * a.q_ts + hq * a.q_hs;
+  const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)u.tok * a.q_ts + u.hq * a.q_hs;
   bf16x8 qb[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) qb[i] = *(const bf16x8*)(qrow + i * 32 + g * 8);
 
-  const int32_t* tab = a.table + b * a.table_stride;
-  const uint8_t* km = a.kmask ? a.kmask + b * a.mask_stride : nullptr;
-  const bf16_t* kbase = (const bf16_t*)a.k + (int64_t)hk * a.head_stride + g * 8;
-  const bf16_t* vbase = (const bf16_t*)a.v + (int64_t)hk * a.head_stride + g * 8;
+  const int32_t* tab = a.table + u.b * a.table_stride;
+  const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
+  const bf16_t* kbase = (const bf16_t*)a.k + (int64_t)u.hk * a.head_stride + g * 8;
+  const bf16_t* vbase = (const bf16_t*)a.v + (int64_t)u.hk * a.head_stride + g * 8;
   const int pmask = (1 << a.page_log2) - 1;
   // pages and masks of this lane's two keys of a tile as they stand in memory: looked at two tiles ahead and made sense of
   // one tile ahead, so that nothing waits for them
-  int rp[2], rm[2] = {1, 1};
+  int rp[2] = {-1, -1}, rm[2] = {1, 1};
   auto look = [&](int k0) {
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt) {
@@ -367,161 +307,289 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256) void paged_few_kernel(const P
   for (int i = 0; i < HD / 16; ++i) O[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
 
+  // One turn of the loop brings tile t + 1 in and works on tile t; the first only brings (the code of both is there once:
+  // short kernels are fetched as they run).
   const int step = WPP * PT_KEYS;
-  int k0 = k_begin + (WPP == 1 ? 0 : wave * PT_KEYS);
-  int pg[2], pn[2];
+  int k0 = k_begin + (WPP == 1 ? 0 : wave * PT_KEYS) - step;
+  int pg[2] = {-1, -1}, pn[2];
   bf16x8 kr[2][NC], vr[2][NC];
-  if (k0 < k_end) {
-    look(k0);
-    place(k0, pg);
-    fetch(kbase, k0, pg, kr);
-    fetch(vbase, k0, pg, vr);
-    look(k0 + step);
-  }
-  for (; k0 < k_end; k0 += step) {
-    const bool all = __all(pg[0] >= 0 && pg[1] >= 0), partial = k0 + PT_KEYS > lo;
+  if (k0 + step < k_end) look(k0 + step);
+  for (bool work = false; k0 < k_end; k0 += step, work = true) {
+    if (k0 + step >= k_end && !work) break;
     place(k0 + step, pn);
+    if (k0 + 2 * step < k_end) look(k0 + 2 * step);   // (before the rows: who waits for it does not wait for them)
     // ---- S^T = K Q^T; K's registers then take the next tile's
     f32x4 S[2];
+    if (work) {
 #pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      S[jt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int jt = 0; jt < 2; ++jt) {
+        S[jt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < NC; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[jt][i], qb[i], S[jt], 0, 0, 0);
+        for (int i = 0; i < NC; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[jt][i], qb[i], S[jt], 0, 0, 0);
+      }
     }
     fetch(kbase, k0 + step, pn, kr);
-    look(k0 + 2 * step);
     // ---- V -> LDS (row = key, padded by 16 bytes: no bank conflict in either direction); V's registers likewise
     bool odd = false;
-    if (partial) {
+    const bool partial = k0 + PT_KEYS > lo;
+    if (work) {
+      if (partial) {
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) odd |= !(fabsf((float)vr[jt][i][e]) < INFINITY);
+        odd = __any(odd);
+      }
 #pragma unroll
       for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) odd |= !(fabsf((float)vr[jt][i][e]) < INFINITY);
-      odd = __any(odd);
+        for (int i = 0; i < NC; ++i) *(bf16x8*)(Vs + (jt * 16 + li) * LD + i * 32 + g * 8) = vr[jt][i];
     }
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-      for (int i = 0; i < NC; ++i) *(bf16x8*)(Vs + (jt * 16 + li) * LD + i * 32 + g * 8) = vr[jt][i];
     fetch(vbase, k0 + step, pn, vr);
-    // ---- softmax
-    float mx = -INFINITY;
-    if (all && !partial) {
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          S[jt][r] *= a.scale_log2;
-          mx = fmaxf(mx, S[jt][r]);
-        }
-    } else {
+    if (work) {
+      // ---- softmax
+      float mx = -INFINITY;
 #pragma unroll
       for (int jt = 0; jt < 2; ++jt) {
         const unsigned on = (unsigned)__ballot(pg[jt] >= 0) >> (4 * g);   // (lanes 0..15 hold the tile's 16 keys)
+        const int room = seen - (k0 + jt * 16 + 4 * g);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool use = ((on >> r) & 1) && k0 + jt * 16 + 4 * g + r < seen;
-          S[jt][r] = use ? S[jt][r] * a.scale_log2 : -INFINITY;
+          S[jt][r] = ((on >> r) & 1) && r < room ? S[jt][r] * a.scale_log2 : -INFINITY;
           mx = fmaxf(mx, S[jt][r]);
         }
       }
-    }
-    mx = quad_max(mx);
-    if (__any(mx > m + kSlack)) {
-      const float mn = fmaxf(m, mx);
-      const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-      m = mn;
-      l *= alpha;
+      mx = quad_max(mx);
+      if (__any(mx > m + kSlack)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) O[i] *= alpha;
-    }
-    const float mz = m == -INFINITY ? 0.f : m;   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
-    bf16x8 pb;
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        S[jt][r] = __builtin_amdgcn_exp2f(S[jt][r] - mz);
-        l += S[jt][r];
-        pb[jt * 4 + r] = (bf16_t)S[jt][r];   // (rounded for the matrix instruction: relative 2^-8 a weight)
+        for (int i = 0; i < HD / 16; ++i) O[i] *= alpha;
       }
-    // ---- O^T += V^T P^T
-    wave_fence();   // lanes read what other lanes of the wave have written
-    if (odd) {
-      bf16x8 ind;
+      const float mz = m == -INFINITY ? 0.f : m;   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
+      bf16x8 pb;
 #pragma unroll
-      for (int jj = 0; jj < 8; ++jj) ind[jj] = S[jj >> 2][jj & 3] > 0.f ? (bf16_t)1.f : (bf16_t)0.f;
+      for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
-      for (int dt = 0; dt < HD / 16; ++dt) {
-        const bf16x8 v = read_vt<LD>(Vs, li, g, dt);
-        bf16x8 vs = v, vc;
-#pragma unroll
-        for (int jj = 0; jj < 8; ++jj) {
-          const float c = odd_code((float)v[jj]);
-          vc[jj] = (bf16_t)c;
-          vs[jj] = c == 0.f ? v[jj] : (bf16_t)0.f;
+        for (int r = 0; r < 4; ++r) {
+          S[jt][r] = __builtin_amdgcn_exp2f(S[jt][r] - mz);
+          l += S[jt][r];
+          pb[jt * 4 + r] = (bf16_t)S[jt][r];   // (rounded for the matrix instruction: relative 2^-8 a weight)
         }
-        const f32x4 code = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, ind, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vs, pb, O[dt], 0, 0, 0);
+      // ---- O^T += V^T P^T
+      wave_fence();   // lanes read what other lanes of the wave have written
+      if (odd) {
+        bf16x8 ind;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) O[dt][r] = odd_apply(O[dt][r], code[r]);
+        for (int jj = 0; jj < 8; ++jj) ind[jj] = S[jj >> 2][jj & 3] > 0.f ? (bf16_t)1.f : (bf16_t)0.f;
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt) {
+          const bf16x8 v = read_vt<LD>(Vs, li, g, dt);
+          bf16x8 vs = v, vc;
+#pragma unroll
+          for (int jj = 0; jj < 8; ++jj) {
+            const float c = odd_code((float)v[jj]);
+            vc[jj] = (bf16_t)c;
+            vs[jj] = c == 0.f ? v[jj] : (bf16_t)0.f;
+          }
+          const f32x4 code = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, ind, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vs, pb, O[dt], 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) O[dt][r] = odd_apply(O[dt][r], code[r]);
+        }
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt)
+          O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(read_vt<LD>(Vs, li, g, dt), pb, O[dt], 0, 0, 0);
       }
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < HD / 16; ++dt)
-        O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(read_vt<LD>(Vs, li, g, dt), pb, O[dt], 0, 0, 0);
+      wave_fence();
     }
-    wave_fence();
     pg[0] = pn[0]; pg[1] = pn[1];
   }
   l = quad_sum(l);
-  const bool parts = n_parts > 1 && a.n_split > 1;
-  const int64_t at = ((int64_t)split * a.T + tok) * a.H + hq;
+  const bool parts = u.n_parts > 1 && a.n_split > 1;
   if constexpr (WPP == 1) {
-    if (!live) return;
-    write_row<bf16_t, HD>(a, parts, at, tok, hq, g, O, m, l);
+    if (!u.live) return;
+    write_row<bf16_t, HD>(a, parts, ((int64_t)u.split * a.T + u.tok) * a.H + u.hq, u.tok, u.hq, g, O, m, l);
   } else {
-    // ---- join the waves: O [16][HD] fp32, then m and l of the 16 rows, in the wave's own LDS
+    // O [16][HD] fp32, then m and l of the 16 rows, in the wave's own LDS
     float* mine = (float*)Vs;
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt) *(f32x4*)(mine + li * HD + dt * 16 + 4 * g) = O[dt];
     if (g == 0) { mine[16 * HD + li] = m; mine[16 * HD + 16 + li] = l; }
     __syncthreads();
-    if (wave >= 4) return;      // 4 waves join: wave w the rows 4w .. 4w+3, a lane 4 (of 64) columns at a time
-    for (int r = wave * 4 + (lane >> 4); r < wave * 4 + 4; r += 4) {
-      if (row0 + r >= rows) continue;
-      float mm = -INFINITY;
+    join_waves<bf16_t, HD, WPP>(a, u, parts, wave, lane, [&](int w) { return (const float*)Vall[w]; });
+  }
+}
+
+// ---- fp32: the same stream for any number of rows, 16 a workgroup, on 16 x 16 x 4 fp32 matrix instructions; nothing passes
+// through LDS.  The output's columns are dealt to the second product's rows so that a lane reads a V row's 16 bytes at
+// 64 c + 4 (lane & 15) -- 16 lanes a whole row piece -- and its four (HD 96: the last two) floats go to four instructions.
+template <int HD, int WPP>
+__global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const PagedArgs a) {
+  constexpr int NC = HD / 16, KEYS = 16, NV = (HD + 63) / 64;   // NV: pieces of a V row a lane reads
+  constexpr int E1 = HD == 96 ? 2 : 4;                                                      // floats of the second one
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  __shared__ __attribute__((aligned(16))) float Oall[WPP == 1 ? 1 : 4][WPP == 1 ? 4 : 16 * HD + 32];
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = unit_of_block(a);
+  if (WPP == 1) id = id * 4 + wave;
+  if (id < 0 || id >= a.n_units) return;
+  Unit u;
+  if (!open_unit(a, id, li, u)) return;
+  const int k_begin = u.k_begin, k_end = u.k_end, seen = u.seen, lo = u.lo;
+
+  const float* qrow = (const float*)a.q + (int64_t)u.tok * a.q_ts + u.hq * a.q_hs + g * 4;
+  f32x4 qf[NC];
 #pragma unroll
-      for (int w = 0; w < WPP; ++w) mm = fmaxf(mm, ((const float*)Vall[w])[16 * HD + r]);
-      const float mz = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f;
-      f32x4 acc[(HD + 63) / 64] = {};
-      for (int w = 0; w < WPP; ++w) {
-        const float* o = (const float*)Vall[w];
-        const float f = __builtin_amdgcn_exp2f(o[16 * HD + r] - mz);
-        ll += o[16 * HD + 16 + r] * f;
+  for (int i = 0; i < NC; ++i) qf[i] = *(const f32x4*)(qrow + 16 * i);
+  const int32_t* tab = a.table + u.b * a.table_stride;
+  const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
+  const float* kbase = (const float*)a.k + (int64_t)u.hk * a.head_stride + g * 4;
+  const float* vbase = (const float*)a.v + (int64_t)u.hk * a.head_stride;
+  const int pmask = (1 << a.page_log2) - 1;
+  int rp = -1, rm = 1;   // page and mask of key k0 + li as they stand in memory
+  auto look = [&](int k0) {
+    const int key = min(k0 + li, k_end - 1);
+    rp = tab[key >> a.page_log2];
+    if (km) rm = km[key];
+  };
+  auto place = [&](int k0) { return k0 + li < k_end && rp < a.n_pages && rm != 0 ? rp : -1; };   // -1: left out
+  f32x4 kr[NC], v0[4], v1[4];
+  auto fetch_k = [&](int k0, int pg) {
+    const float* p = kbase + (int64_t)pg * a.page_stride + (int64_t)((k0 + li) & pmask) * a.slot_stride;
+    if (pg < 0) p = (const float*)kZeroRow + g * 4;
 #pragma unroll
-        for (int c = 0; c < (HD + 63) / 64; ++c)
-          if (c * 64 + li * 4 < HD) acc[c] += *(const f32x4*)(o + r * HD + c * 64 + li * 4) * f;
-      }
-      const int ti = (row0 + r) / a.G, tk = t0 + ti, h = hk * a.G + (row0 + r) - ti * a.G;
-      const int64_t pa = ((int64_t)split * a.T + tk) * a.H + h;
-      const float inv = parts ? 1.f : norm_of(ll);
+    for (int i = 0; i < NC; ++i) kr[i] = *(const f32x4*)(p + i * 16);
+  };
+  auto fetch_v = [&](int k0, int pg) {   // rows 4 g + r: the keys whose weights this lane group holds
 #pragma unroll
-      for (int c = 0; c < (HD + 63) / 64; ++c)
-        if (c * 64 + li * 4 < HD) {
-          if (parts) *(f32x4*)(a.part_o + pa * HD + c * 64 + li * 4) = acc[c];
-          else store4((bf16_t*)a.out + (int64_t)tk * a.o_ts + h * a.o_hs + c * 64 + li * 4,
-                      make_float4(acc[c][0] * inv, acc[c][1] * inv, acc[c][2] * inv, acc[c][3] * inv));
-        }
-      if (li == 0) {
-        if (parts) { a.part_ml[pa * 2] = mm; a.part_ml[pa * 2 + 1] = ll; }
-        else if (a.lse) a.lse[(int64_t)tk * a.H + h] = lse_of(mm, ll);
+    for (int r = 0; r < 4; ++r) {
+      const int pv = __shfl(pg, 4 * g + r, 16);
+      const float* p = vbase + (int64_t)pv * a.page_stride + (int64_t)((k0 + 4 * g + r) & pmask) * a.slot_stride;
+      if (pv < 0) p = (const float*)kZeroRow;
+      v0[r] = *(const f32x4*)(p + li * 4);
+      if constexpr (E1 == 2) {
+        const f32x2 x = *(const f32x2*)(p + 64 + li * 2);
+        v1[r] = (f32x4){x[0], x[1], 0.f, 0.f};
+      } else if constexpr (NV == 2) {
+        v1[r] = *(const f32x4*)(p + 64 + li * 4);
       }
     }
+  };
+
+  f32x4 O[NC];   // [4 c + e]: column 64 c + 4 (4 g + r) + e (HD 96, c = 1: 64 + 2 (4 g + r) + e) in element r
+#pragma unroll
+  for (int i = 0; i < NC; ++i) O[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  // (one turn brings tile t + 1 in and works on tile t, as above)
+  const int step = WPP * KEYS;
+  int k0 = k_begin + (WPP == 1 ? 0 : wave * KEYS) - step, pg = -1, pn;
+  if (k0 + step < k_end) look(k0 + step);
+  for (bool work = false; k0 < k_end; k0 += step, work = true) {
+    if (k0 + step >= k_end && !work) break;
+    pn = place(k0 + step);
+    if (k0 + 2 * step < k_end) look(k0 + 2 * step);
+    f32x4 S = {0.f, 0.f, 0.f, 0.f};
+    if (work) {
+      f32x4 S2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          S = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][e], qf[i][e], S, 0, 0, 0);
+          S2 = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][e + 1], qf[i][e + 1], S2, 0, 0, 0);
+        }
+      S += S2;
+    }
+    fetch_k(k0 + step, pn);
+    if (work) {
+      float mx = -INFINITY;
+      const unsigned on = (unsigned)__ballot(pg >= 0) >> (4 * g);   // (lanes 0..15 hold the 16 keys)
+      const int room = seen - (k0 + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        S[r] = ((on >> r) & 1) && r < room ? S[r] * a.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, S[r]);
+      }
+      mx = quad_max(mx);
+      if (__any(mx > m + kSlack)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) O[i] *= alpha;
+      }
+      const float mz = m == -INFINITY ? 0.f : m;   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        S[r] = __builtin_amdgcn_exp2f(S[r] - mz);
+        l += S[r];   // (this lane's keys only: the four lanes of a row are added up at the end)
+      }
+      // ---- O^T += V^T P^T
+      if (k0 + KEYS > lo) {
+        bool odd = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < NC; ++i) odd |= !(fabsf(i < 4 ? v0[r][i & 3] : v1[r][i & 3]) < INFINITY);
+        if (__any(odd)) {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            f32x4 code = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float c = odd_code(i < 4 ? v0[r][i & 3] : v1[r][i & 3]);
+              code = __builtin_amdgcn_mfma_f32_16x16x4f32(c, S[r] > 0.f ? 1.f : 0.f, code, 0, 0, 0);
+              if (i < 4) v0[r][i & 3] = c == 0.f ? v0[r][i & 3] : 0.f;
+              else v1[r][i & 3] = c == 0.f ? v1[r][i & 3] : 0.f;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) O[i][x] = odd_apply(O[i][x], code[x]);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          O[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(i < 4 ? v0[r][i & 3] : v1[r][i & 3], S[r], O[i], 0, 0, 0);
+    }
+    fetch_v(k0 + step, pn);
+    pg = pn;
+  }
+  l = quad_sum(l);
+  const bool parts = u.n_parts > 1 && a.n_split > 1;
+  // four (two) neighbouring columns of this lane's row for each r
+  auto emit = [&](float* row, float inv) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      *(f32x4*)(row + 4 * (4 * g + r)) = (f32x4){O[0][r], O[1][r], O[2][r], O[3][r]} * inv;
+      if constexpr (E1 == 2) *(f32x2*)(row + 64 + 2 * (4 * g + r)) = (f32x2){O[4][r], O[5][r]} * inv;
+      else if constexpr (NV == 2) *(f32x4*)(row + 64 + 4 * (4 * g + r)) = (f32x4){O[NC - 4][r], O[NC - 3][r], O[NC - 2][r], O[NC - 1][r]} * inv;
+    }
+  };
+  if constexpr (WPP == 1) {
+    if (!u.live) return;
+    const int64_t at = ((int64_t)u.split * a.T + u.tok) * a.H + u.hq;
+    if (parts) {
+      emit(a.part_o + at * HD, 1.f);
+      if (g == 0) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = l; }
+    } else {
+      emit((float*)a.out + (int64_t)u.tok * a.o_ts + u.hq * a.o_hs, norm_of(l));
+      if (a.lse && g == 0) a.lse[(int64_t)u.tok * a.H + u.hq] = lse_of(m, l);
+    }
+  } else {
+    emit(Oall[wave] + li * HD, 1.f);
+    if (g == 0) { Oall[wave][16 * HD + li] = m; Oall[wave][16 * HD + 16 + li] = l; }
+    __syncthreads();
+    join_waves<float, HD, WPP>(a, u, parts, wave, lane, [&](int w) { return (const float*)Oall[w]; });
   }
 }
 
@@ -562,9 +630,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int id = unit_of_block(a);
   if (id < 0 || id >= a.n_units) return;
-  const int tile = id % a.n_tiles; id /= a.n_tiles;   // (the tiles of a key head read the same keys)
-  const int split = id % a.n_split; id /= a.n_split;
-  const int hk = id % a.Hk, b = id / a.Hk;
+  int rest = a.by_tiles.divmod(id);
+  const int tile = id;                                // (the tiles of a key head read the same keys)
+  id = a.by_split.divmod(rest);
+  const int split = rest, b = a.by_hk.divmod(id), hk = id;
   int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
   t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
@@ -574,7 +643,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   const int len = seq_len(a, b);
   const int row = row0 + wave * 32 + c32;
   const bool live = row < rows;
-  const int ri = (live ? row : row0) / a.G, tok = t0 + ri, hq = hk * a.G + (live ? row : row0) - ri * a.G;
+  const int ri = a.by_group.div(live ? row : row0), tok = t0 + ri, hq = hk * a.G + (live ? row : row0) - ri * a.G;
   int seen = live ? len : 0;   // keys this lane's row may look at
   if (a.causal && live) {
     const int64_t last = a.q_index ? (int64_t)a.q_index[tok] : (int64_t)len - (t1 - tok);
@@ -592,9 +661,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   __syncthreads();
   const int hi = __builtin_amdgcn_readfirstlane(max(max(red[0], red[1]), max(red[2], red[3])));
   const int lo = __builtin_amdgcn_readfirstlane(min(min(red[4], red[5]), min(red[6], red[7])));
-  const int n_parts = len <= 0 ? 1 : (len + a.split_keys - 1) / a.split_keys;
-  if (split >= n_parts) return;
+  const int n_parts = len <= a.split_keys ? 1 : 2;   // (one, or more)
   const int k_begin = split * a.split_keys;
+  if (split > 0 && k_begin >= len) return;
   const int k_end = min(hi, split == a.n_split - 1 ? hi : k_begin + a.split_keys);
 
   const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)tok * a.q_ts + hq * a.q_hs;
@@ -812,9 +881,10 @@ template <typename T, int HD, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   __shared__ float so[4][HD], sl[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int per = a.max_q * a.H, id = WPR == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
-  const int b = id / per, r = id - b * per, i = r / a.H, h = r - i * a.H;
+  int h = WPR == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+  const int b = a.by_rows.divmod(h);
   if (b >= a.B) return;
+  const int i = a.by_heads.divmod(h);
   const int t0 = a.cu_q[b], t1 = a.cu_q[b + 1], len = seq_len(a, b);
   const int tok = t0 + i;
   if (tok < 0 || tok >= t1 || tok >= a.T) return;
@@ -859,7 +929,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
 }
 
 struct PagedPlan {
-  int few;               // waves a problem in paged_few_kernel, 0 = paged_attn_kernel
+  int few;               // waves a problem in paged_few_kernel, 0 = tiles of rows
   int n_tiles, n_split, split_keys;
   int64_t ws_o, ws_ml;   // bytes
 };
@@ -869,8 +939,9 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   const int64_t rows = (int64_t)p->max_q * (p->n_heads / p->kv.n_kv_heads);
   const int64_t heads = (int64_t)p->kv.n_kv_heads * p->n_seqs;
   s.few = 0;
-  if (p->kv.dtype == DARK_BF16 && rows <= 16) s.few = p->max_kv <= 128 ? 1 : (heads <= 64 && p->max_kv <= 1024) ? 8 : 4;
-  const int tile_rows = s.few ? 16 : p->kv.dtype == DARK_BF16 ? TT_ROWS : PT_ROWS;
+  if (p->kv.dtype == DARK_F32) s.few = p->max_kv <= 128 ? 1 : 4;
+  else if (rows <= 16) s.few = p->max_kv <= 128 ? 1 : (heads <= 64 && p->max_kv <= 1024) ? 8 : 4;
+  const int tile_rows = s.few ? 16 : TT_ROWS;
   s.n_tiles = (int)((rows + tile_rows - 1) / tile_rows);
   if (s.n_tiles < 1) s.n_tiles = 1;
   const int64_t wgs = (int64_t)s.n_tiles * heads;
@@ -880,7 +951,7 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   // with 8192).  Never below 256 keys: a part's (O, m, l) is then 1/16 of the keys' bytes at most.
   int64_t keys = p->max_kv;
   if (s.few != 1 && s.few != 8) {
-    if (wgs < 512) keys = (p->max_kv * wgs + 511) / 512;
+    if (wgs < 256) keys = (p->max_kv * wgs + 511) / 512;
     if (s.few && wgs >= 256 && keys > 1024) keys = 1024;
     if (keys < 256) keys = 256;
   }
@@ -960,14 +1031,23 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   const int64_t wgs = (int64_t)s.n_tiles * p->kv.n_kv_heads * p->n_seqs * s.n_split;
   DARK_CHECK_ARG(wgs < (1ll << 30), "%s: %lld workgroups", who, (long long)wgs);
   a.n_units = (int)wgs;
+  a.max_q = p->max_q;
+  a.by_hk = make_div(a.Hk); a.by_tiles = make_div(s.n_tiles); a.by_split = make_div(s.n_split); a.by_group = make_div(a.G);
+  a.by_heads = make_div(a.H); a.by_rows = make_div((int)(s.n_split > 1 ? (int64_t)p->max_q * a.H : 1));
+  DARK_CHECK_ARG(s.n_split == 1 || (int64_t)p->n_seqs * p->max_q * p->n_heads < (1ll << 31), "%s: too many rows", who);
   // units that share memory on one XCD, where there are enough such groups for all eight
   int blocks = s.few == 1 ? (int)((wgs + 3) / 4) : (int)wgs;
-  a.n_inner = s.few == 1 ? p->kv.n_kv_heads / 4 : s.few ? p->kv.n_kv_heads : s.n_tiles;
-  const int groups = a.n_inner > 1 ? cdiv(blocks, a.n_inner) : 0;
-  if (groups % 8 == 0 || groups >= 64) blocks = a.n_inner > 1 ? cdiv(groups, 8) * 8 * a.n_inner : blocks;
-  else a.n_inner = 1;
-  a.max_q = p->max_q;
-  DARK_CHECK_ARG(s.n_split == 1 || (int64_t)p->n_seqs * p->max_q * p->n_heads < (1ll << 31), "%s: too many rows", who);
+  a.n_inner = 1;
+  for (int inner : {s.few ? p->kv.n_kv_heads * s.n_tiles : s.n_tiles, s.few ? p->kv.n_kv_heads : 1}) {
+    if (s.few == 1) inner /= 4;   // (four units a workgroup)
+    const int groups = inner > 1 ? cdiv(blocks, inner) : 0;
+    if (groups >= 64 || (groups > 0 && groups % 8 == 0)) {
+      a.n_inner = inner;
+      blocks = cdiv(groups, 8) * 8 * inner;
+      break;
+    }
+  }
+  a.by_inner = make_div(a.n_inner);
   const dim3 grid((unsigned)blocks), block(s.few == 8 ? 512 : 256), jblock(256);
   const unsigned jrows = (unsigned)((int64_t)p->n_seqs * p->max_q * p->n_heads);
 #define DARK_JOIN(T, HDv)                                                                           \
@@ -988,7 +1068,8 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   } while (0)
 #define DARK_PAGED_F32(HDv)                                                                         \
   do {                                                                                              \
-    hipLaunchKernelGGL((paged_attn_kernel<HDv>), grid, block, 0, st, a);                            \
+    if (s.few == 1) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1>), grid, block, 0, st, a);          \
+    else hipLaunchKernelGGL((paged_f32_kernel<HDv, 4>), grid, block, 0, st, a);                     \
     DARK_JOIN(float, HDv);                                                                          \
   } while (0)
   const int HD = p->kv.head_dim;

@@ -12,8 +12,9 @@ from .configuration_dream import DreamConfig
 from .generation_utils import DreamGenerationConfig, DreamGenerationMixin, DreamModelOutput
 from .modeling_dream_length import DreamModel_length
 from .modeling_dream import DreamModel
+from .kv_cache import PagedKVCache, append_kv, paged_attention, qk_norm_rope
 
-__all__ = ["DreamConfig", "DreamGenerationConfig", "DreamGenerationMixin", "DreamModelOutput",
+__all__ = ["PagedKVCache", "append_kv", "paged_attention", "qk_norm_rope", "DreamConfig", "DreamGenerationConfig", "DreamGenerationMixin", "DreamModelOutput",
            "DreamModel_length", "DreamModel", "install_akgr_alias"]
 
 

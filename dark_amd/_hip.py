@@ -27,7 +27,8 @@ SAMPLE_LDS_MAX_V = 32768   # DARK_SAMPLE_LDS_MAX_V: larger vocabularies sample f
 
 class LayerWeights(C.Structure):
     _fields_ = [("w_qkv", C.c_void_p), ("b_qkv", C.c_void_p), ("w_o", C.c_void_p), ("w_gu", C.c_void_p),
-                ("w_down", C.c_void_p), ("ln1", C.c_void_p), ("ln2", C.c_void_p)]
+                ("w_down", C.c_void_p), ("ln1", C.c_void_p), ("ln2", C.c_void_p), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p)]
 
 
 class ModelDesc(C.Structure):
@@ -35,7 +36,8 @@ class ModelDesc(C.Structure):
                 ("ff", C.c_int32), ("n_layers", C.c_int32), ("n_heads", C.c_int32), ("head_dim", C.c_int32),
                 ("max_pos", C.c_int32), ("rms_eps", C.c_float), ("resid_dtype", C.c_int32), ("embed", C.c_void_p),
                 ("final_norm", C.c_void_p), ("lm_head", C.c_void_p), ("rope_cos", C.c_void_p),
-                ("rope_sin", C.c_void_p), ("layers", C.POINTER(LayerWeights))]
+                ("rope_sin", C.c_void_p), ("layers", C.POINTER(LayerWeights)), ("ident_cos", C.c_void_p),
+                ("ident_sin", C.c_void_p)]
 
 
 class Gpt2LayerWeights(C.Structure):
@@ -62,7 +64,7 @@ class QkNormRopeArgs(C.Structure):
     _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_w", "k_w", "rope_cos", "rope_sin", "pos")] +
                 [(n, C.c_int64) for n in ("q_ts", "q_hs", "k_ts", "k_hs", "qo_ts", "qo_hs", "ko_ts", "ko_hs")] +
                 [(n, C.c_int32) for n in ("dtype", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "max_pos")] +
-                [("eps", C.c_float), ("reserved", C.c_int32)])
+                [("eps", C.c_float), ("pos_period", C.c_int32)])
 
 
 class KVAppendArgs(C.Structure):
@@ -80,6 +82,11 @@ class PagedAttentionArgs(C.Structure):
                                           "mask_stride")] +
                 [(n, C.c_int32) for n in ("n_tokens", "n_heads", "n_seqs", "table_width", "max_q", "max_kv", "causal")] +
                 [("scale", C.c_float)])
+
+
+class CachedTokens(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("pos", C.c_void_p), ("slots", C.c_void_p), ("layer_stride", C.c_int64),
+                ("attn", PagedAttentionArgs)]
 
 
 # name -> (restype, argtypes); every symbol include/dark_hip.h declares
@@ -193,6 +200,9 @@ SIGNATURES = {
     "dark_kv_append": (C.c_int, [C.c_void_p, C.c_void_p]),
     "dark_paged_attention_workspace_bytes": (C.c_size_t, [C.c_void_p]),
     "dark_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "dark_forward_cached_workspace_bytes": (C.c_size_t, [C.POINTER(ModelDesc), C.POINTER(CachedTokens)]),
+    "dark_forward_cached": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(CachedTokens), C.c_void_p, C.c_size_t, C.c_void_p,
+                                      C.c_void_p]),
     "dark_dbg_embed": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                  C.c_void_p]),
 }

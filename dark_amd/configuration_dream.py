@@ -14,6 +14,9 @@ from typing import Any, Dict
 
 class DreamConfig:
     model_type = "Dream"
+    # RMS norm of every query and key head before the rotation (weights self_attn.q_norm / k_norm [head_dim]); not in the
+    # reference's config, written to config.json only where it is on
+    qk_norm = False
 
     def __init__(self, vocab_size=151936, hidden_size=768, intermediate_size=3072, num_hidden_layers=10,
                  num_attention_heads=8, num_key_value_heads=8, hidden_act="silu", max_position_embeddings=64,
@@ -45,6 +48,8 @@ class DreamConfig:
         self.pad_token_id = pad_token_id
         self.bos_token_id = kwargs.pop("bos_token_id", None)
         self.eos_token_id = kwargs.pop("eos_token_id", None)
+        if kwargs.pop("qk_norm", False):
+            self.qk_norm = True
         for k, v in kwargs.items():  # HF configs keep unknown keys as attributes
             setattr(self, k, v)
         self._check_supported()

@@ -76,6 +76,22 @@ static int resid_gemm_norm(const dark_model_desc* m, const void* A, const void* 
   return DARK_OK;
 }
 
+// per-head norms + rotation of the q and k columns of a [M, 3d] projection, in place (pos == null: row index mod N)
+static int norm_heads(const dark_model_desc* m, const dark_layer_weights& L, void* qkv, const int32_t* pos, int M, int N,
+                      hipStream_t st) {
+  DARK_CHECK_ARG(L.k_norm && m->ident_cos && m->ident_sin, "q_norm without k_norm or the identity rotation");
+  const int64_t es = (int64_t)esize(m->dtype), d = m->d;
+  dark_qk_norm_rope_args a = {};
+  a.q = a.q_out = qkv;
+  a.k = a.k_out = (char*)qkv + d * es;
+  a.q_w = L.q_norm; a.k_w = L.k_norm; a.rope_cos = m->rope_cos; a.rope_sin = m->rope_sin; a.pos = pos;
+  a.q_ts = a.k_ts = a.qo_ts = a.ko_ts = 3 * d;
+  a.q_hs = a.k_hs = a.qo_hs = a.ko_hs = m->head_dim;
+  a.dtype = m->dtype; a.n_tokens = M; a.n_heads = a.n_kv_heads = m->n_heads; a.head_dim = m->head_dim;
+  a.max_pos = m->max_pos; a.eps = m->rms_eps; a.pos_period = N;
+  return dark_qk_norm_rope(&a, st);
+}
+
 // `tail_rows` = false: the whole body.  true: stop after the LAST layer's attention -- what is left of that layer
 // (o_proj, residual, norm, MLP, residual) only matters for the rows the head will read and is done by forward_tail.
 static int forward_hidden(const dark_model_desc* m, const int64_t* ids, const int32_t* pos,
@@ -101,8 +117,14 @@ static int forward_hidden(const dark_model_desc* m, const int64_t* ids, const in
     DARK_CHECK_ARG(L.w_qkv && L.b_qkv && L.w_o && L.w_gu && L.w_down && L.ln1 && L.ln2, "layer %d: null weight", l);
     // (w.xn = this layer's normalised input: from embed_norm for layer 0, from the previous down_proj's epilogue after)
     DARK_TRY(launch_gemm(m->dtype, EPI_BIAS, w.xn, L.w_qkv, L.b_qkv, w.qkv, M, 3 * d, d, 3 * d, st));
-    DARK_TRY(launch_attention(m->dtype, w.qkv, m->rope_cos, m->rope_sin, pos, key_mask, w.att, B, N, m->n_heads,
-                              m->head_dim, m->max_pos, st));
+    if (L.q_norm) {   // norms go between the projection and the rotation: both in one pass over q and k, in place
+      DARK_TRY(norm_heads(m, L, w.qkv, pos, M, N, st));
+      DARK_TRY(launch_attention(m->dtype, w.qkv, m->ident_cos, m->ident_sin, nullptr, key_mask, w.att, B, N, m->n_heads,
+                                m->head_dim, 1, st));
+    } else {
+      DARK_TRY(launch_attention(m->dtype, w.qkv, m->rope_cos, m->rope_sin, pos, key_mask, w.att, B, N, m->n_heads,
+                                m->head_dim, m->max_pos, st));
+    }
     if (tail_rows && l == m->n_layers - 1) break;
     DARK_TRY(resid_gemm_norm(m, w.att, L.w_o, hidden, L.ln2, w.xn, M, d, st));
     DARK_TRY(launch_gemm(m->dtype, EPI_SWIGLU, w.xn, L.w_gu, nullptr, w.act, M, 2 * m->ff, d, m->ff, st));
@@ -265,6 +287,57 @@ int dark_forward_hidden_begin(const dark_model_desc* m, const int64_t* ids, cons
 int dark_forward_hidden_rows(const dark_model_desc* m, int B, int N, const int32_t* rows, int n_rows, void* workspace,
                              size_t workspace_bytes, const void* hidden, void* hidden_rows, void* stream) {
   return forward_tail(m, B, N, rows, n_rows, workspace, workspace_bytes, hidden, hidden_rows, (hipStream_t)stream);
+}
+
+size_t dark_forward_cached_workspace_bytes(const dark_model_desc* m, const dark_cached_tokens* t) {
+  if (!m || !t || t->attn.n_tokens <= 0) return 0;
+  return carve_fwd(m, (size_t)t->attn.n_tokens, nullptr).total + align_up(dark_paged_attention_workspace_bytes(&t->attn), 256);
+}
+
+int dark_forward_cached(const dark_model_desc* m, const dark_cached_tokens* t, void* workspace, size_t ws_bytes, void* hidden,
+                        void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  DARK_TRY(check_model(m));
+  DARK_CHECK_ARG(t != nullptr, "forward_cached: null arguments");
+  const int T = t->attn.n_tokens, d = m->d;
+  if (T == 0) return DARK_OK;
+  DARK_CHECK_ARG(T > 0 && T < (1 << 30), "forward_cached: n_tokens=%d", T);
+  DARK_CHECK_ARG(t->ids && t->pos && t->slots && hidden && workspace, "forward_cached: null pointer");
+  DARK_CHECK_ARG(t->attn.kv.dtype == m->dtype && t->attn.kv.head_dim == m->head_dim && t->attn.kv.n_kv_heads == m->n_heads &&
+                     t->attn.n_heads == m->n_heads, "forward_cached: the cache's dtype or heads are not the model's");
+  const size_t es = esize(m->dtype), need = dark_forward_cached_workspace_bytes(m, t);
+  DARK_CHECK_ARG(ws_bytes >= need && ((uintptr_t)workspace & 15) == 0, "forward_cached: workspace %zu < required %zu bytes (or not aligned)", ws_bytes, need);
+  FwdWs w = carve_fwd(m, (size_t)T, (char*)workspace);
+  DARK_CHECK_ARG(m->n_layers == 0 || m->layers[0].ln1, "layer 0: null weight");
+  if (m->n_layers == 0) return launch_embed(m->dtype, m->resid_dtype, t->ids, m->embed, hidden, T, d, m->vocab, st);
+  DARK_TRY(launch_embed_norm(m->dtype, m->resid_dtype, t->ids, m->embed, hidden, T, d, m->vocab, m->layers[0].ln1, m->rms_eps, w.xn, st));
+  dark_kv_append_args ap = {};
+  dark_paged_attention_args at = t->attn;
+  ap.rope_cos = m->rope_cos; ap.rope_sin = m->rope_sin; ap.pos = t->pos; ap.slots = t->slots;
+  ap.q_ts = ap.k_ts = ap.v_ts = ap.qo_ts = 3 * (int64_t)d;
+  ap.q_hs = ap.k_hs = ap.v_hs = ap.qo_hs = m->head_dim;
+  ap.n_tokens = T; ap.n_heads = m->n_heads; ap.max_pos = m->max_pos; ap.eps = m->rms_eps;
+  ap.q = ap.q_out = w.qkv;                       // (the rotated queries take the projection's place)
+  ap.k = w.qkv + d * es; ap.v = w.qkv + 2 * d * es;
+  at.q = w.qkv; at.q_ts = 3 * (int64_t)d; at.q_hs = m->head_dim;
+  at.out = w.att; at.o_ts = d; at.o_hs = m->head_dim; at.lse = nullptr;
+  at.workspace = (char*)workspace + w.total; at.workspace_bytes = (int64_t)(ws_bytes - w.total);
+  for (int l = 0; l < m->n_layers; ++l) {
+    const dark_layer_weights& L = m->layers[l];
+    DARK_CHECK_ARG(L.w_qkv && L.b_qkv && L.w_o && L.w_gu && L.w_down && L.ln1 && L.ln2, "layer %d: null weight", l);
+    at.kv.k = (char*)t->attn.kv.k + (size_t)l * t->layer_stride * es;
+    at.kv.v = (char*)t->attn.kv.v + (size_t)l * t->layer_stride * es;
+    ap.kv = at.kv; ap.q_w = L.q_norm; ap.k_w = L.k_norm;
+    DARK_TRY(launch_gemm(m->dtype, EPI_BIAS, w.xn, L.w_qkv, L.b_qkv, w.qkv, T, 3 * d, d, 3 * d, st));
+    DARK_TRY(dark_kv_append(&ap, stream));
+    DARK_TRY(dark_paged_attention(&at, stream));
+    DARK_TRY(resid_gemm_norm(m, w.att, L.w_o, hidden, L.ln2, w.xn, T, d, st));
+    DARK_TRY(launch_gemm(m->dtype, EPI_SWIGLU, w.xn, L.w_gu, nullptr, w.act, T, 2 * m->ff, d, m->ff, st));
+    const float* ln_next = l + 1 < m->n_layers ? m->layers[l + 1].ln1 : nullptr;
+    DARK_CHECK_ARG(l + 1 >= m->n_layers || ln_next, "layer %d: null weight", l + 1);
+    DARK_TRY(resid_gemm_norm(m, w.act, L.w_down, hidden, ln_next, w.xn, T, m->ff, st));
+  }
+  return DARK_OK;
 }
 
 int dark_lm_head_rows(const dark_model_desc* m, const void* hidden, const int32_t* src_rows, int M, void* workspace,

@@ -22,7 +22,7 @@ struct RowsArgs {
   int64_t src_ts[3], src_hs[3], dst_ts[3], dst_hs[3];
   int64_t page_stride, n_slots;
   int32_t T, h_end[3];        // rows [0, h_end[0]) are q heads, then k heads, then v heads
-  int32_t max_pos, page_log2, n_pass, t_step;   // passes of a token, tokens under way at a time
+  int32_t max_pos, page_log2, n_pass, t_step, pos_period;   // passes of a token, tokens under way at a time
   float eps;
 };
 
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
   int64_t slot = 0;
   auto position = [&](int tt) {
     if (!turned || tt >= a.T) return 0;
-    const int q = a.pos[tt];
+    const int q = a.pos ? a.pos[tt] : tt % a.pos_period;
     return q < 0 ? 0 : (q >= a.max_pos ? a.max_pos - 1 : q);
   };
   auto fetch = [&](int tt, int pp) {
@@ -239,7 +239,7 @@ int dark_qk_norm_rope(const dark_qk_norm_rope_args* p, void* stream) {
   const int es = p->dtype == DARK_BF16 ? 2 : 4;
   DARK_CHECK_ARG((p->n_heads == 0 || (p->q && p->q_out)) && (p->n_kv_heads == 0 || (p->k && p->k_out)), "%s: null pointer", who);
   DARK_CHECK_ARG((p->rope_cos == nullptr) == (p->rope_sin == nullptr), "%s: rope_cos and rope_sin go together", who);
-  DARK_CHECK_ARG(!p->rope_cos || (p->pos && p->max_pos >= 1), "%s: a rotation needs positions and a table", who);
+  DARK_CHECK_ARG(!p->rope_cos || ((p->pos || p->pos_period > 0) && p->max_pos >= 1), "%s: a rotation needs positions and a table", who);
   DARK_CHECK_ARG(aligned16(p->q, p->q_ts, p->q_hs, es) && aligned16(p->k, p->k_ts, p->k_hs, es) &&
                      aligned16(p->q_out, p->qo_ts, p->qo_hs, es) && aligned16(p->k_out, p->ko_ts, p->ko_hs, es),
                  "%s: pointers and strides must be multiples of 16 bytes", who);
@@ -248,7 +248,7 @@ int dark_qk_norm_rope(const dark_qk_norm_rope_args* p, void* stream) {
   a.w[0] = p->q_w; a.w[1] = p->k_w; a.cosT = p->rope_cos; a.sinT = p->rope_sin; a.pos = p->pos;
   a.src_ts[0] = p->q_ts; a.src_hs[0] = p->q_hs; a.src_ts[1] = p->k_ts; a.src_hs[1] = p->k_hs;
   a.dst_ts[0] = p->qo_ts; a.dst_hs[0] = p->qo_hs; a.dst_ts[1] = p->ko_ts; a.dst_hs[1] = p->ko_hs;
-  a.T = p->n_tokens; a.max_pos = p->max_pos; a.eps = p->eps;
+  a.T = p->n_tokens; a.max_pos = p->max_pos; a.eps = p->eps; a.pos_period = p->pos_period > 0 ? p->pos_period : 1;
   a.h_end[0] = p->n_heads; a.h_end[1] = a.h_end[2] = p->n_heads + p->n_kv_heads;
   return launch_head_rows(a, p->dtype, p->head_dim, (hipStream_t)stream);
 }

@@ -139,6 +139,8 @@ class _LoopCtx:
     state_hook: Optional[Callable] = None    # parity tests: teacher forcing, (step, x) -> x
     count_reduce: Optional[Callable] = None  # dispatch.generate_sharded(exact_ragged_k=True)
     trace: Optional[dict] = None             # parity tests: receives per-step k / conf / x0
+    cache_interval: int = 0         # > 0: cached forwards, a whole one every that many (kv_cache.WindowCache)
+    window: Optional[Any] = None    # the kv_cache.WindowCache of this call
     head: Optional[Any] = None               # vocab_shard.ShardedHead: head + sampling split over a process group
 
 
@@ -221,7 +223,12 @@ class DreamGenerationMixin:
         # stream (same generator state, same values as the [M, V] `exponential_` fill the reference makes) instead
         # of being written to and read back from HBM; False materialises them with torch.
         # _count_reduce (dispatch.generate_sharded): (count tensor, B_local) -> (global masks, global rows)
-        ctx = _LoopCtx(skip_noop=bool(kwargs.pop("skip_noop_steps", True)),
+        # cache_interval = R > 0: forwards run against a paged key / value cache, R - 1 of R of them for the positions that
+        # may still change only (kv_cache.WindowCache); R = 1 computes every position every time
+        interval = kwargs.pop("cache_interval", 0) or 0
+        if int(interval) != interval or interval < 0:
+            raise ValueError(f"cache_interval={interval!r}: a whole number of forwards, 0 = no cache")
+        ctx = _LoopCtx(skip_noop=bool(kwargs.pop("skip_noop_steps", True)), cache_interval=int(interval),
                        lazy_noise=bool(kwargs.pop("lazy_noise", True)),
                        noise_fn=kwargs.pop("_noise_fn", None), rand_fn=kwargs.pop("_rand_fn", None),
                        rank_noise_fn=kwargs.pop("_rank_noise_fn", None),
@@ -306,6 +313,12 @@ class DreamGenerationMixin:
         rank_temp = float(alg_temp) if (alg_temp is not None and alg_temp != 0) else 0.0
         if ctx.head is not None and (not fast or alg == "origin"):
             raise NotImplementedError("the vocabulary-sharded head serves the confidence algorithms with default hooks")
+        if ctx.cache_interval:
+            if not fast or alg == "origin" or ctx.head is not None:
+                raise NotImplementedError("cache_interval serves the confidence algorithms with default hooks, without "
+                                          "think_sample and without a sharded head")
+            from .kv_cache import WindowCache
+            ctx.window = WindowCache(self, B, N, pos, key_mask, ctx.cache_interval)
         # the reference filters iff `top_p is not None and top_p < 1` (:62): 0 keeps the top-1 token only; < 0 = off
         top_p_f = max(float(top_p), 0.0) if (top_p is not None and top_p < 1) else -1.0
         top_k_i = int(min(top_k, self.config.vocab_size)) if top_k is not None else 0
@@ -337,6 +350,8 @@ class DreamGenerationMixin:
             if ctx.state_hook is not None:
                 x.copy_(ctx.state_hook(i, x).to(x.device))
                 st.hidden_valid = False
+                if ctx.window is not None:
+                    ctx.window.expire()
             if histories is not None:
                 histories.append(x.clone())
 
@@ -416,7 +431,10 @@ class DreamGenerationMixin:
             st.mask_rows(x, mask_id)              # row_index / src_rows / count, then async count read-back
             # enqueued before the host waits for the count: everything up to the last layer's attention; the rest of
             # that layer is only needed for the M rows the head reads and follows once M is known (forward_rows)
-            st.forward_begin(x, pos, key_mask)
+            if ctx.window is not None:
+                ctx.window.forward(st, x, mask_id)
+            else:
+                st.forward_begin(x, pos, key_mask)
             st.hidden_valid = True                # ... for as long as x does not change
         M = st.wait_count()
         Mg, Bg = (M, B) if ctx.count_reduce is None else ctx.count_reduce(st.count[:1], B)
@@ -437,7 +455,7 @@ class DreamGenerationMixin:
                 noise = self._draw_noise(step, M, V, x.device, noise_fn)
         if skip and k == 0:
             return  # nothing is committed: the draw above was this step's only effect
-        if not st.rows_valid and M > 0:
+        if not st.rows_valid and M > 0 and ctx.window is None:
             st.forward_rows(M)
         if ctx.head is not None:
             conf, x0 = ctx.head.head_and_sample(st, M, temperature, top_p, top_k, conf_mode, noise, philox)
@@ -459,6 +477,8 @@ class DreamGenerationMixin:
             else:
                 st.commit(x, mask_id, M, conf, x0, k)
             st.hidden_valid = False
+            if ctx.window is not None:
+                ctx.window.committed(k)
 
     def _step_general(self, st, x, pos, key_mask, mask_id, temperature, top_p, top_k, alg, alg_temp, t, s, last, step,
                       tokens_hook, logits_hook, ctx: _LoopCtx) -> torch.Tensor:

@@ -260,3 +260,183 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         _WORKSPACE.pack_into(packed, _WORKSPACE_AT, ws.data_ptr(), need)
     _call(lib.dark_paged_attention, bytes(packed), dev)
     return (out, lse) if return_lse else out
+
+
+class PagedKVCache:
+    """The pages of every layer of a model and who holds them.  ``k(l)`` / ``v(l)`` are layer ``l``'s ``[n_pages, page_size,
+    n_kv_heads, head_dim]`` (a head's slots of a page lie together in memory: what the attention reads)."""
+
+    def __init__(self, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype,
+                 device) -> None:
+        _need(dtype in _DTYPES, f"dtype {dtype}: float32 and bfloat16 only")
+        _need(page_size >= 1 and page_size & (page_size - 1) == 0, f"page size {page_size} must be a power of two")
+        _need(n_layers >= 0 and n_pages >= 0 and n_kv_heads >= 1 and head_dim >= 1, "negative size")
+        self.n_layers, self.n_pages, self.page_size = n_layers, n_pages, page_size
+        self.n_kv_heads, self.head_dim, self.dtype = n_kv_heads, head_dim, dtype
+        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
+        self._k, self._v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def device(self) -> torch.device:
+        return self._k.device
+
+    def k(self, layer: int) -> torch.Tensor:
+        return self._k[layer].transpose(1, 2)
+
+    def v(self, layer: int) -> torch.Tensor:
+        return self._v[layer].transpose(1, 2)
+
+    def pages_for(self, n_tokens: int) -> int:
+        return -(-n_tokens // self.page_size)
+
+    def allocate(self, n_tokens: int) -> list:
+        """Page ids for ``n_tokens`` tokens of a sequence; MemoryError (nothing taken) if there are not enough."""
+        n = self.pages_for(n_tokens)
+        if n > len(self._free):
+            raise MemoryError(f"{n} pages wanted, {len(self._free)} of {self.n_pages} free")
+        out = [self._free.pop() for _ in range(n)]
+        return out
+
+    def free(self, pages) -> None:
+        held = set(self._free)
+        for p in pages:
+            p = int(p)
+            _need(0 <= p < self.n_pages and p not in held, f"page {p} is not held")
+            held.add(p)
+            self._free.append(p)
+
+    def slots(self, block_table: torch.Tensor, seq: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
+        """Slot (int64) of token ``index[t]`` of sequence ``seq[t]``; -1 where the table names no page for it."""
+        at = torch.div(index, self.page_size, rounding_mode="floor").long()
+        inside = (at >= 0) & (at < block_table.shape[1])
+        page = block_table[seq.long(), at.clamp(0, block_table.shape[1] - 1)].long()
+        return torch.where(inside & (page >= 0) & (page < self.n_pages), page * self.page_size + index % self.page_size, -1)
+
+    def _fields(self):
+        """dark_paged_kv of layer 0, elements between layers."""
+        e = self._k.stride()
+        return _hip.PagedKV(k=self._k.data_ptr(), v=self._v.data_ptr(), page_stride=e[1], slot_stride=e[3], head_stride=e[2],
+                            dtype=_DTYPES[self.dtype], n_pages=self.n_pages, page_size=self.page_size,
+                            n_kv_heads=self.n_kv_heads, head_dim=self.head_dim), e[0]
+
+
+def forward_cached(model, cache: PagedKVCache, input_ids: torch.Tensor, seq: torch.Tensor, index: torch.Tensor,
+                   block_table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, max_q: int, max_kv: int, *,
+                   position_ids: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None, causal: bool = False,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The body of a ``DreamModel_length`` for new tokens (``input_ids [T]`` int64, token ``t`` = place ``index[t]`` of sequence
+    ``seq[t]``, the tokens of a sequence together as ``cu_q`` says) against ``cache``: their keys and values are written to
+    their slots, every new token attends over all ``kv_len`` keys of its sequence (``causal``: up to its own place).
+    ``position_ids [T]`` default to ``index``.  Returns the residual stream ``[T, hidden_size]`` (``out`` if given) for the LM
+    head."""
+    pk = model.packed()
+    dev = pk.device
+    T, B = input_ids.shape[0], kv_len.shape[0]
+    if not isinstance(cache, PagedKVCache) or cache.device != dev or cache.dtype != pk.dtype:
+        raise ValueError("the cache is not on the model's device or not of its dtype")
+    cfg = model.config
+    if cache.n_layers < cfg.num_hidden_layers or cache.n_kv_heads != cfg.num_attention_heads or cache.head_dim != cfg.head_dim:
+        raise ValueError("the cache is not the model's: layers, heads or head_dim differ")
+    if position_ids is None and max_kv > pk.max_pos:
+        raise ValueError(f"max_kv={max_kv} exceeds the rotation tables ({pk.max_pos} rows: max_position_embeddings)")
+    i32 = torch.int32
+    for name, t, dt, n in (("input_ids", input_ids, torch.int64, T), ("seq", seq, None, T), ("index", index, i32, T),
+                           ("cu_q", cu_q, i32, B + 1), ("kv_len", kv_len, i32, B), ("position_ids", position_ids, i32, T)):
+        if t is not None:
+            _refuse(name, t, dev.index, dt, 1)
+            _need(t.shape[0] == n and t.is_contiguous(), f"{name} must be contiguous with {n} elements")
+    _refuse("block_table", block_table, dev.index, i32, 2)
+    _need(block_table.shape[0] == B and block_table.is_contiguous(), f"block_table must be contiguous with {B} rows")
+    if key_mask is not None:
+        _refuse("key_mask", key_mask, dev.index, torch.uint8, 2)
+        _need(key_mask.shape[0] == B and key_mask.shape[1] >= max_kv and key_mask.is_contiguous(),
+              f"key_mask must be contiguous [{B}, >= {max_kv}] uint8")
+    hidden = torch.empty((T, cfg.hidden_size), dtype=pk.resid_dtype, device=dev) if out is None else out
+    _refuse("out", hidden, dev.index, pk.resid_dtype, 2)
+    _need(tuple(hidden.shape) == (T, cfg.hidden_size) and hidden.is_contiguous(), f"out must be contiguous [{T}, {cfg.hidden_size}]")
+    if T == 0:
+        return hidden
+    lib = _hip.load()
+    kv, layer_stride = cache._fields()
+    with torch.cuda.device(dev):
+        slots = cache.slots(block_table, seq, index)
+        attn = _hip.PagedAttentionArgs(
+            kv=kv, block_table=block_table.data_ptr(), cu_q=cu_q.data_ptr(), kv_len=kv_len.data_ptr(),
+            q_index=index.data_ptr() if causal else None, key_mask=_hip.ptr(key_mask), table_stride=block_table.shape[1],
+            mask_stride=0 if key_mask is None else key_mask.shape[1], n_tokens=T, n_heads=cfg.num_attention_heads, n_seqs=B,
+            table_width=block_table.shape[1], max_q=max_q, max_kv=max_kv, causal=int(bool(causal)), scale=cfg.head_dim ** -0.5)
+        tokens = _hip.CachedTokens(ids=input_ids.data_ptr(), pos=(index if position_ids is None else position_ids).data_ptr(),
+                                   slots=slots.data_ptr(), layer_stride=layer_stride, attn=attn)
+        need = lib.dark_forward_cached_workspace_bytes(pk.ref, tokens)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _hip.check(lib.dark_forward_cached(pk.ref, tokens, ws.data_ptr(), need, hidden.data_ptr(), _hip.stream_ptr(dev)))
+    return hidden
+
+
+class WindowCache:
+    """Cached denoise steps of one batch of windows ``[B, N]`` (``diffusion_generate(..., cache_interval=R)``).
+
+    Every R-th forward is a whole one: all positions are new tokens, their keys and values fill the cache.  The forwards
+    between compute only the positions that may have changed since or that a sampler may read: the ones masked at the last
+    whole forward and their left neighbours (the logit shift, generation_utils.py:496).  The other positions' keys and values
+    stay those of that forward -- an approximation for bidirectional attention (they would change with the tokens committed
+    meanwhile), exact for R = 1."""
+
+    PAGE = 16
+
+    def __init__(self, model, B: int, N: int, pos: Optional[torch.Tensor], key_mask: Optional[torch.Tensor], interval: int) -> None:
+        cfg, dev = model.config, model.device
+        self.model, self.B, self.N, self.interval = model, B, N, interval
+        per = -(-N // self.PAGE)
+        self.cache = PagedKVCache(cfg.num_hidden_layers, B * per, self.PAGE, cfg.num_attention_heads, cfg.head_dim,
+                                  model.packed().dtype, dev)
+        i32 = torch.int32
+        self.table = torch.arange(B * per, dtype=i32, device=dev).view(B, per)
+        self.kv_len = torch.full((B,), N, dtype=i32, device=dev)
+        self.all_cu = torch.arange(0, B * N + 1, N, dtype=i32, device=dev)
+        self.all_seq = torch.arange(B, device=dev).repeat_interleave(N)
+        self.all_index = torch.arange(N, dtype=i32, device=dev).repeat(B)
+        self.pos = None if pos is None else pos.reshape(-1)
+        self.key_mask = key_mask
+        self.rows = None          # flat positions the forwards between compute; None: a whole one is due
+        self.done = 0             # forwards since the last whole one
+        self.min_masked = 0       # fewest masks a row holds
+
+    def expire(self) -> None:
+        """The windows changed in a way the cache does not know of: the next forward is a whole one."""
+        self.rows = None
+
+    def committed(self, k: int) -> None:
+        """k positions of every row were committed.  A row with fewer masks than k gets positions re-masked that were not
+        (generation_utils.py:531-534): they may lie outside the rows computed, so a whole forward is due."""
+        if k > self.min_masked:
+            self.expire()
+        self.min_masked -= k
+
+    def forward(self, st, x: torch.Tensor, mask_id: int) -> None:
+        """Leaves the residual stream of every position a sampler may read in ``st.hidden``."""
+        st.rows_valid = False
+        if self.rows is None or self.done + 1 >= self.interval:
+            forward_cached(self.model, self.cache, x.view(-1), self.all_seq, self.all_index, self.table, self.all_cu, self.kv_len,
+                           self.N, self.N, position_ids=self.pos, key_mask=self.key_mask, out=st.hidden)
+            self.done = 0
+            if self.interval > 1:
+                self._choose(x == mask_id)
+            return
+        self.done += 1
+        if self.rows.shape[0] > 0:
+            hidden = forward_cached(self.model, self.cache, x.view(-1)[self.rows], self.seq, self.index, self.table, self.cu,
+                                    self.kv_len, self.max_q, self.N, position_ids=self.rows_pos, key_mask=self.key_mask)
+            st.hidden.index_copy_(0, self.rows, hidden)
+
+    def _choose(self, masked: torch.Tensor) -> None:
+        act = masked.clone()
+        act[:, :-1] |= masked[:, 1:]
+        n = act.sum(1)
+        self.rows = act.view(-1).nonzero().flatten()
+        self.min_masked, self.max_q = torch.stack([masked.sum(1).min(), n.max()]).tolist()
+        self.cu = torch.zeros(self.B + 1, dtype=torch.int32, device=masked.device)
+        self.cu[1:] = n.cumsum(0)
+        self.seq, self.index = self.all_seq[self.rows], self.all_index[self.rows].contiguous()
+        self.rows_pos = None if self.pos is None else self.pos[self.rows].contiguous()

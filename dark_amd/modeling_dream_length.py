@@ -112,6 +112,9 @@ class PackedWeights:
             lw.w_down = dev(_pad_rows(sd[p + "mlp.down_proj.weight"])).data_ptr()
             lw.ln1 = dev(sd[p + "input_layernorm.weight"], torch.float32).data_ptr()
             lw.ln2 = dev(sd[p + "post_attention_layernorm.weight"], torch.float32).data_ptr()
+            if cfg.qk_norm:
+                lw.q_norm = dev(sd[a + "q_norm.weight"], torch.float32).data_ptr()
+                lw.k_norm = dev(sd[a + "k_norm.weight"], torch.float32).data_ptr()
         head = _pad_rows(sd["lm_head.weight"])
         self.desc = _hip.ModelDesc(
             dtype=_hip.DARK_BF16 if dtype == torch.bfloat16 else _hip.DARK_F32,
@@ -123,7 +126,9 @@ class PackedWeights:
             final_norm=dev(sd["model.norm.weight"], torch.float32).data_ptr(),
             lm_head=dev(head).data_ptr(),
             rope_cos=dev(cos, torch.float32).data_ptr(), rope_sin=dev(sin, torch.float32).data_ptr(),
-            layers=C.cast(self.layers, C.POINTER(_hip.LayerWeights)))
+            layers=C.cast(self.layers, C.POINTER(_hip.LayerWeights)),
+            ident_cos=dev(torch.ones(cfg.head_dim // 2), torch.float32).data_ptr(),
+            ident_sin=dev(torch.zeros(cfg.head_dim // 2), torch.float32).data_ptr())
         self.ref = C.byref(self.desc)
         self.elem = 2 if dtype == torch.bfloat16 else 4
 
@@ -375,10 +380,12 @@ class _Weight(nn.Module):
 
 
 class _Attn(nn.Module):
-    def __init__(self, d):
+    def __init__(self, d, norm_dim=0):
         super().__init__()
         self.q_proj, self.k_proj, self.v_proj = _Linear(d, d, True), _Linear(d, d, True), _Linear(d, d, True)
         self.o_proj = _Linear(d, d, False)
+        if norm_dim:
+            self.q_norm, self.k_norm = _Weight(norm_dim), _Weight(norm_dim)
 
 
 class _MLP(nn.Module):
@@ -388,9 +395,9 @@ class _MLP(nn.Module):
 
 
 class _Layer(nn.Module):
-    def __init__(self, d, ff):
+    def __init__(self, d, ff, norm_dim=0):
         super().__init__()
-        self.self_attn, self.mlp = _Attn(d), _MLP(d, ff)
+        self.self_attn, self.mlp = _Attn(d, norm_dim), _MLP(d, ff)
         self.input_layernorm, self.post_attention_layernorm = _Weight(d), _Weight(d)
 
 
@@ -398,7 +405,7 @@ class _Base(nn.Module):
     def __init__(self, cfg: DreamConfig):
         super().__init__()
         self.embed_tokens = _Weight(cfg.vocab_size, cfg.hidden_size)
-        self.layers = nn.ModuleList([_Layer(cfg.hidden_size, cfg.intermediate_size)
+        self.layers = nn.ModuleList([_Layer(cfg.hidden_size, cfg.intermediate_size, cfg.head_dim if cfg.qk_norm else 0)
                                      for _ in range(cfg.num_hidden_layers)])
         self.norm = _Weight(cfg.hidden_size)
 
@@ -565,3 +572,32 @@ class DreamModel_length(DreamGenerationMixin, nn.Module):
         # the reference's lm_head returns the model's dtype (modeling_dream_length.py:809: bf16 logits from a bf16 model,
         # e.g. under the autocast of custom_grpo2.py:409-418); the head GEMM here accumulates and stores fp32
         return MaskedLMOutput(logits=logits.to(self.dtype) if self.dtype == torch.bfloat16 else logits.clone())
+
+    # ---- a paged key / value cache (no counterpart in the reference, which recomputes every window)
+    def make_cache(self, n_tokens: int, page_size: int = 16):
+        """A ``kv_cache.PagedKVCache`` with pages for ``n_tokens`` tokens (of whole pages: count a sequence's last one whole)."""
+        from .kv_cache import PagedKVCache
+        pk = self.packed()
+        return PagedKVCache(self.config.num_hidden_layers, -(-n_tokens // page_size), page_size, self.config.num_attention_heads,
+                            self.config.head_dim, pk.dtype, pk.device)
+
+    @torch.no_grad()
+    def forward_cached(self, cache, input_ids: torch.LongTensor, seq: torch.Tensor, index: torch.Tensor, block_table: torch.Tensor,
+                       cu_q: torch.Tensor, kv_len: torch.Tensor, max_q: int, max_kv: int, *,
+                       position_ids: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None, causal: bool = False
+                       ) -> MaskedLMOutput:
+        """``forward`` for new tokens against ``cache`` (arguments of ``kv_cache.forward_cached``): ``.logits [T, V]`` in the
+        model's dtype.  Windows of any length, in chunks of any length."""
+        from .kv_cache import forward_cached
+        if self.device.type != "cuda":
+            raise RuntimeError("dark_amd runs on a HIP device only: move the model with .to('cuda')")
+        hidden = forward_cached(self, cache, input_ids, seq, index, block_table, cu_q, kv_len, max_q, max_kv,
+                                position_ids=position_ids, key_mask=key_mask, causal=causal)
+        T, V, pk, lib = hidden.shape[0], self.config.vocab_size, self._packed, _hip.load()
+        logits = torch.empty((T, V), dtype=torch.float32, device=pk.device)
+        if T > 0:
+            with torch.cuda.device(pk.device):
+                ws = torch.empty(lib.dark_head_workspace_bytes(pk.ref, T), dtype=torch.uint8, device=pk.device)
+                _hip.check(lib.dark_lm_head_rows(pk.ref, _hip.ptr(hidden), None, T, _hip.ptr(ws), ws.numel(), _hip.ptr(logits), V,
+                                                 _hip.stream_ptr(pk.device)))
+        return MaskedLMOutput(logits=logits.to(self.dtype) if self.dtype == torch.bfloat16 else logits)

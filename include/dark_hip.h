@@ -53,6 +53,8 @@ typedef struct dark_layer_weights {
   const void* w_down;  /* [d, ff]                                                          */
   const float* ln1;    /* input_layernorm.weight [d] fp32                                  */
   const float* ln2;    /* post_attention_layernorm.weight [d] fp32                         */
+  const float* q_norm; /* [head_dim] fp32: per-head RMS norm of the queries / keys before the rotation, NULL (both) = none: */
+  const float* k_norm; /* the reference has none; DreamConfig(qk_norm=True), names self_attn.q_norm.weight / k_norm.weight  */
 } dark_layer_weights;
 
 /* Whole model (DreamConfig shape contract, configuration_dream.py:29-50). */
@@ -77,6 +79,8 @@ typedef struct dark_model_desc {
   const float* rope_cos;    /* [max_pos, head_dim/2] fp32 (DreamRotaryEmbedding.forward, :151-171) */
   const float* rope_sin;    /* [max_pos, head_dim/2] fp32 */
   const dark_layer_weights* layers; /* HOST array of n_layers entries */
+  const float* ident_cos;   /* [head_dim/2] fp32, all 1 / all 0: the rotation of the attention kernel where q and k come */
+  const float* ident_sin;   /* normed and rotated (layers with q_norm); may be NULL for models without */
 } dark_model_desc;
 
 int dark_hip_abi_version(void);
@@ -382,7 +386,8 @@ typedef struct dark_paged_kv {
  * pointers and strides multiples of 16 bytes.  q_out = q (same strides) runs in place, k_out = k likewise; any other
  * overlap of an output with an input is not allowed.
  *   q_w, k_w [head_dim] fp32, NULL = no norm for that operand
- *   rope_cos, rope_sin [max_pos, head_dim/2] fp32, both NULL = no rotation; pos [n_tokens] int32, clamped to the table */
+ *   rope_cos, rope_sin [max_pos, head_dim/2] fp32, both NULL = no rotation; pos [n_tokens] int32, or NULL with
+ *   pos_period = N > 0: token t stands at t mod N (rows of windows of N); clamped to the table */
 typedef struct dark_qk_norm_rope_args {
   const void *q, *k;
   void *q_out, *k_out;
@@ -391,7 +396,7 @@ typedef struct dark_qk_norm_rope_args {
   int64_t q_ts, q_hs, k_ts, k_hs, qo_ts, qo_hs, ko_ts, ko_hs;
   int32_t dtype, n_tokens, n_heads, n_kv_heads, head_dim, max_pos;
   float eps;
-  int32_t reserved;
+  int32_t pos_period;
 } dark_qk_norm_rope_args;
 int dark_qk_norm_rope(const dark_qk_norm_rope_args* a, void* stream);
 
@@ -446,6 +451,26 @@ typedef struct dark_paged_attention_args {
 } dark_paged_attention_args;
 size_t dark_paged_attention_workspace_bytes(const dark_paged_attention_args* a);
 int dark_paged_attention(const dark_paged_attention_args* a, void* stream);
+
+/* The transformer body for new tokens against a paged cache (all layers): embedding + norm, per layer [q/k/v projection,
+ * kv_append (rotation, norms where the layer has them), paged_attention, o_proj + residual, norm, SwiGLU MLP + residual].
+ * With every position of a window as a new token it computes what dark_forward_hidden does (window length not limited);
+ * with some of them, what follows from the others' cached keys and values.
+ *   kv: layer 0's cache; layer l's k and v lie layer_stride elements further each.  n_kv_heads must be n_heads.
+ *   ids, pos, slots, q_index, hidden: one entry (row) a new token; pos, slots as in dark_kv_append, the rest as in
+ *   dark_paged_attention (q, out, lse, workspace and their strides are not read)
+ *   hidden [n_tokens, d] m->resid_dtype OUT: the residual stream after the last layer (pre final norm), for
+ *   dark_lm_head_rows.  Workspace: dark_forward_cached_workspace_bytes(...) bytes, 256-byte aligned. */
+typedef struct dark_cached_tokens {
+  const int64_t* ids;      /* [n_tokens] */
+  const int32_t* pos;      /* [n_tokens] */
+  const int64_t* slots;    /* [n_tokens] */
+  int64_t layer_stride;
+  dark_paged_attention_args attn;
+} dark_cached_tokens;
+size_t dark_forward_cached_workspace_bytes(const dark_model_desc* m, const dark_cached_tokens* t);
+int dark_forward_cached(const dark_model_desc* m, const dark_cached_tokens* t, void* workspace, size_t workspace_bytes,
+                        void* hidden, void* stream);
 
 /* ---- GPT-2 backbone of the legacy denoiser: akgr/abduction_model/model/custom_gpt.py:25-114,
  * `DiffusionModel(GPT2LMHeadModel)` built by create_gpt2_transformer (:446-472).  Weights are packed by

@@ -117,3 +117,53 @@ def test_checker_against_dense_attention():
         want = torch.einsum("bhij,bjhd->bihd", s.softmax(-1), v.repeat_interleave(2, 2))
         torch.testing.assert_close(out.view(B, n, H, D), want, rtol=0, atol=1e-12)
         torch.testing.assert_close(lse.view(B, n, H), s.logsumexp(-1).transpose(1, 2), rtol=0, atol=1e-12)
+
+
+# --------------------------------------------------------------------------- pages and windows
+def test_pages_and_slots():
+    c = kv_cache.PagedKVCache(2, 7, 16, 4, 64, torch.float32, "cpu")
+    assert c.k(1).shape == (7, 16, 4, 64) and c.k(1).stride() == c.v(0).stride() and c.pages_for(0) == 0
+    a, b = c.allocate(33), c.allocate(16)
+    assert len(a) == 3 and len(b) == 1 and len(set(a + b)) == 4
+    with pytest.raises(MemoryError):
+        c.allocate(49)
+    assert len(c.allocate(48)) == 3
+    c.free(a)
+    for bad in ([a[0]], [99], [b[0], b[0]]):
+        with pytest.raises(ValueError, match="not held"):
+            c.free(bad)
+    table = torch.tensor([[5, -1], [2, 9]], dtype=torch.int32)
+    seq, index = torch.tensor([0, 0, 0, 1, 1, 1, 1]), torch.tensor([0, 15, 16, 3, 17, 32, -1], dtype=torch.int32)
+    assert c.slots(table, seq, index).tolist() == [80, 95, -1, 35, -1, -1, -1]
+    with pytest.raises(ValueError, match="power of two"):
+        kv_cache.PagedKVCache(1, 1, 24, 1, 64, torch.float32, "cpu")
+
+
+def test_window_cache_schedule(monkeypatch):
+    """Whole forwards every third time; a row that runs out of masks, or a change from outside, brings one forward."""
+    from types import SimpleNamespace
+    seen = []
+    monkeypatch.setattr(kv_cache, "forward_cached", lambda m, c, ids, seq, index, *a, out=None, **k: (
+        seen.append(ids.shape[0]), out if out is not None else torch.zeros(ids.shape[0], 64))[1])
+    cfg = SimpleNamespace(num_hidden_layers=1, num_attention_heads=1, head_dim=64)
+    model = SimpleNamespace(config=cfg, device=torch.device("cpu"), packed=lambda: SimpleNamespace(dtype=torch.float32))
+    x = torch.full((2, 20), 9)
+    x[0, 5:9], x[1, 0:7] = 6, 6
+    wc = kv_cache.WindowCache(model, 2, 20, None, None, 3)
+    st = SimpleNamespace(hidden=torch.zeros(40, 64), rows_valid=True)
+    for k in (1, 1, 1):
+        wc.forward(st, x, 6)
+        wc.committed(k)
+    assert seen == [40, 12, 12] and not st.rows_valid and wc.min_masked == 1
+    assert wc.cu.tolist() == [0, 5, 12] and wc.max_q == 7
+    assert wc.rows.tolist() == [4, 5, 6, 7, 8] + [20 + j for j in range(7)]
+    wc.forward(st, x, 6)                       # the third since the whole one: whole again
+    wc.committed(4)
+    wc.forward(st, x, 6)
+    assert seen[3:] == [40, 12]
+    wc.committed(1)                            # row 0 had none left
+    wc.forward(st, x, 6)
+    wc.expire()
+    wc.forward(st, x, 6)
+    assert seen[5:] == [40, 40]
+    assert kv_cache.WindowCache(model, 2, 20, None, None, 1).forward(st, x, 6) is None and seen[-1] == 40

@@ -195,11 +195,10 @@ SIGNATURES = {
                                          C.c_void_p, C.c_int64, C.c_void_p]),
     "dark_dbg_layernorm": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                      C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p]),
-    # (the argument structs go as the bytes of their fields: kv_cache.py packs them, one call converts one pointer)
-    "dark_qk_norm_rope": (C.c_int, [C.c_void_p, C.c_void_p]),
-    "dark_kv_append": (C.c_int, [C.c_void_p, C.c_void_p]),
-    "dark_paged_attention_workspace_bytes": (C.c_size_t, [C.c_void_p]),
-    "dark_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "dark_qk_norm_rope": (C.c_int, [C.POINTER(QkNormRopeArgs), C.c_void_p]),
+    "dark_kv_append": (C.c_int, [C.POINTER(KVAppendArgs), C.c_void_p]),
+    "dark_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
+    "dark_paged_attention": (C.c_int, [C.POINTER(PagedAttentionArgs), C.c_void_p]),
     "dark_forward_cached_workspace_bytes": (C.c_size_t, [C.POINTER(ModelDesc), C.POINTER(CachedTokens)]),
     "dark_forward_cached": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(CachedTokens), C.c_void_p, C.c_size_t, C.c_void_p,
                                       C.c_void_p]),

@@ -11,7 +11,7 @@ synchronise, and have no backward: a tensor that asks for gradients is refused w
 """
 from __future__ import annotations
 
-import struct
+import ctypes as C
 from typing import Optional, Tuple
 
 import torch
@@ -19,14 +19,29 @@ import torch
 from . import _hip
 
 _DTYPES = {torch.float32: _hip.DARK_F32, torch.bfloat16: _hip.DARK_BF16}
-_SIZE = {torch.float32: 4, torch.bfloat16: 2}
-_KV = "2Q3q6i"                                            # dark_paged_kv
-_NORM_ROPE = struct.Struct("=9Q8q6ifi")                   # dark_qk_norm_rope_args
-_APPEND = struct.Struct(f"={_KV}10Q8q3if")                # dark_kv_append_args
-_ATTEND = struct.Struct(f"={_KV}9Q7q7if")                 # dark_paged_attention_args
-_WORKSPACE = struct.Struct("=Qq")                         # its workspace, workspace_bytes
-_WORKSPACE_AT = struct.calcsize(f"={_KV}8Q")
 _raw_stream = torch._C._cuda_getCurrentRawStream          # hipStream_t of torch's current stream on a device
+_bind = None
+
+
+def _ops():
+    """The compiled binding (csrc/bind.cpp): checks operands, fills the argument structs of include/dark_hip.h."""
+    global _bind
+    if _bind is None:
+        try:
+            from . import _bind as mod
+        except ImportError as e:
+            raise ImportError(f"dark_amd/_bind.so cannot be loaded ({e}): build it with `make -C dark_amd/csrc`") from e
+        lib = _hip.load()
+        mod.init(_hip.DarkHipError, *(C.cast(getattr(lib, n), C.c_void_p).value for n in (
+            "dark_qk_norm_rope", "dark_kv_append", "dark_paged_attention", "dark_paged_attention_workspace_bytes",
+            "dark_hip_last_error")))
+        _bind = mod
+    return _bind
+
+
+def _stream(t: torch.Tensor) -> int:
+    dev = t.get_device()
+    return _raw_stream(dev) if dev >= 0 else 0
 
 
 def _need(cond: bool, msg: str) -> None:
@@ -34,10 +49,8 @@ def _need(cond: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
-# A served step calls these functions once a layer, and a step of single tokens is over in microseconds: the checks
-# below are one expression a tensor, and only a call that fails one is taken apart for its message.
 def _refuse(name: str, t, dev: int, dtype, dim: int) -> None:
-    """Says what is wrong with an operand that a quick check has found wrong (or returns: nothing is)."""
+    """Returns if t is a tensor of this device, dtype and number of dimensions."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.get_device() != dev:
@@ -48,116 +61,6 @@ def _refuse(name: str, t, dev: int, dtype, dim: int) -> None:
         raise ValueError(f"{name} has {t.dim()} dimensions, expected {dim}")
 
 
-def _no_grad(**tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.requires_grad:
-            raise RuntimeError(f"{name} requires gradients: the cache's operators have no backward (use torch.no_grad())")
-
-
-def _device(t) -> int:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise RuntimeError("dark_amd runs on a HIP device only")
-    if t.dtype not in _DTYPES:
-        raise ValueError(f"dtype {t.dtype}: float32 and bfloat16 only")
-    return t.get_device()
-
-
-def _rows(name: str, t: torch.Tensor, dev: int, dtype, T: int, HD: int) -> Tuple[torch.Tensor, int, int, int, int]:
-    """(tensor, pointer, token stride, head stride, heads) of a [T, heads, HD] input, copied only where its strides or its
-    alignment do not fit the kernels' 16-byte accesses."""
-    if t.dtype != dtype or t.get_device() != dev or t.dim() != 3:
-        _refuse(name, t, dev, dtype, 3)
-    n, heads, d = t.shape
-    if n != T or d != HD:
-        raise ValueError(f"{name} is {tuple(t.shape)}, expected [{T}, heads, {HD}]")
-    ts, hs, one = t.stride()
-    p = t.data_ptr()
-    if one != 1 or (p | (ts | hs) * _SIZE[dtype]) & 15:
-        t = t.clone(memory_format=torch.contiguous_format)
-        ts, hs, _ = t.stride()
-        p = t.data_ptr()
-    return t, p, ts, hs, heads
-
-
-def _out(name: str, t: Optional[torch.Tensor], like: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
-    if t is None:
-        t = torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    elif t is not like and (t.dtype != like.dtype or t.get_device() != like.get_device() or t.dim() != 3):
-        _refuse(name, t, like.get_device(), like.dtype, 3)
-    _need(t.shape == like.shape, f"{name} is {tuple(t.shape)}, expected {tuple(like.shape)}")
-    ts, hs, one = t.stride()
-    p = t.data_ptr()
-    if one != 1 or (p | (ts | hs) * _SIZE[t.dtype]) & 15 or ts == 0 or hs == 0:
-        _fits(name, t)
-    return t, p, ts, hs
-
-
-def _fits(name: str, t: torch.Tensor) -> None:
-    """What is written: 16-byte pointer and strides, contiguous last dimension, no two elements in one place (dimensions of
-    one have no stride of their own)."""
-    if t.numel() == 0:
-        return
-    es = t.element_size()
-    st = [s for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1]
-    _need(t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in st),
-          f"{name}: pointer and strides must be multiples of 16 bytes, the last dimension contiguous")
-    _need(all(st), f"{name}: an expanded tensor cannot be written")
-
-
-def _vec(name: str, t: Optional[torch.Tensor], dev: int, dtype, n: int) -> int:
-    if t is None:
-        return 0
-    if t.dtype != dtype or t.get_device() != dev or t.dim() != 1:
-        _refuse(name, t, dev, dtype, 1)
-    if t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous with {n} elements")
-    return t.data_ptr()
-
-
-def _tables(cos, sin, pos, dev: int, T: int, HD: int) -> Tuple[int, int, int, int]:
-    if cos is None and sin is None:
-        return 0, 0, 0, 0
-    _need(cos is not None and sin is not None and pos is not None, "cos, sin and pos go together")
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype != torch.float32 or t.get_device() != dev or t.dim() != 2:
-            _refuse(name, t, dev, torch.float32, 2)
-    n, half = cos.shape
-    if n < 1 or half * 2 != HD or sin.shape != cos.shape or not (cos.is_contiguous() and sin.is_contiguous()):
-        raise ValueError(f"cos and sin must be contiguous [max_pos, {HD // 2}]")
-    return cos.data_ptr(), sin.data_ptr(), _vec("pos", pos, dev, torch.int32, T), n
-
-
-def _cache(k: torch.Tensor, v: torch.Tensor, dev: int, dtype):
-    """The fields of dark_paged_kv."""
-    if k.dtype != dtype or k.get_device() != dev or k.dim() != 4:
-        _refuse("k_cache", k, dev, dtype, 4)
-    if v.dtype != dtype or v.get_device() != dev or v.dim() != 4:
-        _refuse("v_cache", v, dev, dtype, 4)
-    n_pages, page, Hk, HD = k.shape
-    ps, ss, hs, one = st = k.stride()
-    if v.shape != k.shape or v.stride() != st:
-        raise ValueError("k_cache and v_cache must have the same shape and strides")
-    if page < 1 or page & (page - 1):
-        raise ValueError(f"page size {page} must be a power of two")
-    kp, vp = k.data_ptr(), v.data_ptr()
-    if one != 1 or (kp | vp | (ps | ss | hs) * _SIZE[dtype]) & 15 or not (ps and ss and hs):
-        _fits("k_cache", k)
-        _fits("v_cache", v)
-        # (a dimension of one has no stride of its own)
-        ps, ss, hs = ps if n_pages > 1 else 0, ss if page > 1 else 0, hs if Hk > 1 else 0
-    return kp, vp, ps, ss, hs, _DTYPES[dtype], n_pages, page, Hk, HD, 0
-
-
-def _call(fn, packed: bytes, dev: int) -> None:
-    if dev != torch._C._cuda_getDevice():                 # the library launches on the CURRENT device
-        with torch.cuda.device(dev):
-            _hip.check(fn(packed, _raw_stream(dev)))
-        return
-    rc = fn(packed, _raw_stream(dev))
-    if rc:
-        _hip.check(rc)
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
                  cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], pos: Optional[torch.Tensor], eps: float = 1e-6,
                  q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -165,20 +68,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     fp32, None = no norm), then the rotation by row ``pos[t]`` (int32, clamped) of the fp32 tables ``cos`` / ``sin
     [max_pos, head_dim/2]`` (both None = no rotation); fp32 inside, one rounding.  ``q_out`` / ``k_out`` may be ``q`` /
     ``k`` themselves.  Returns ``(q_out, k_out)``."""
-    dev, dt = _device(q), q.dtype
-    if torch.is_grad_enabled():
-        _no_grad(q=q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, q_out=q_out, k_out=k_out)
-    T, _, HD = q.shape if q.dim() == 3 else (0, 0, 0)
-    qi, qp, q_ts, q_hs, Hq = _rows("q", q, dev, dt, T, HD)
-    ki, kp, k_ts, k_hs, Hk = _rows("k", k, dev, dt, T, HD)
-    q_out, qop, qo_ts, qo_hs = _out("q_out", q_out, q)
-    k_out, kop, ko_ts, ko_hs = _out("k_out", k_out, k)
-    c, s, p, n = _tables(cos, sin, pos, dev, T, HD)
-    _call(_hip.load().dark_qk_norm_rope,
-          _NORM_ROPE.pack(qp, kp, qop, kop, _vec("q_weight", q_weight, dev, torch.float32, HD),
-                          _vec("k_weight", k_weight, dev, torch.float32, HD), c, s, p, q_ts, q_hs, k_ts, k_hs, qo_ts, qo_hs,
-                          ko_ts, ko_hs, _DTYPES[dt], T, Hq, Hk, HD, n, eps, 0), dev)
-    return q_out, k_out
+    return (_bind or _ops()).qk_norm_rope(_stream(q), q, k, q_weight, k_weight, cos, sin, pos, eps, q_out, k_out)
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
@@ -189,27 +79,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     head_dim]`` of new tokens into the cache: token ``t`` into slot ``slots[t]`` (int64, ``page * page_size + slot``;
     a negative one, or one beyond the cache, is not stored).  The slots of one call must differ.  ``q`` is normed and
     rotated in the same pass into ``q_out`` (which may be ``q``), the return value."""
-    dev, dt = _device(k), k.dtype
-    if torch.is_grad_enabled():
-        _no_grad(k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q, q_out=q_out, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin)
-    T, Hk, HD = k.shape if k.dim() == 3 else (0, 0, 0)
-    kv = _cache(k_cache, v_cache, dev, dt)
-    ki, kp, k_ts, k_hs, _ = _rows("k", k, dev, dt, T, HD)
-    vi, vp, v_ts, v_hs, Hv = _rows("v", v, dev, dt, T, HD)
-    if kv[8] != Hk or kv[9] != HD or Hv != Hk:
-        raise ValueError(f"k is {tuple(k.shape)}, v {tuple(v.shape)}, the cache holds {kv[8]} heads of {kv[9]}")
-    qi, qp, q_ts, q_hs, Hq, qop, qo_ts, qo_hs = None, 0, 0, 0, 0, 0, 0, 0
-    if q is not None:
-        qi, qp, q_ts, q_hs, Hq = _rows("q", q, dev, dt, T, HD)
-        q_out, qop, qo_ts, qo_hs = _out("q_out", q_out, q)
-    else:
-        _need(q_out is None, "q_out without q")
-    c, s, p, n = _tables(cos, sin, pos, dev, T, HD)
-    _call(_hip.load().dark_kv_append,
-          _APPEND.pack(*kv, qp, kp, vp, qop, _vec("q_weight", q_weight, dev, torch.float32, HD),
-                       _vec("k_weight", k_weight, dev, torch.float32, HD), c, s, p, _vec("slots", slots, dev, torch.int64, T),
-                       q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, qo_ts, qo_hs, T, Hq, n, eps), dev)
-    return q_out
+    return (_bind or _ops()).append_kv(_stream(k), k, v, k_cache, v_cache, slots, cos, sin, pos, q, q_out, q_weight, k_weight, eps)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -222,44 +92,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (uint8 or bool) is 0 and, with ``causal``, keys behind the token's own place ``q_index[t]`` (int32; default: the
     sequence's last places).  A token with no key left gets zeros (lse -inf).  ``max_q`` / ``max_kv``: the most new tokens /
     keys of a sequence.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out``, or ``(out, lse [T, n_heads] fp32)``."""
-    dev, dt = _device(q), q.dtype
-    if torch.is_grad_enabled():
-        _no_grad(q=q, k_cache=k_cache, v_cache=v_cache, out=out)
-    T, _, HD = q.shape if q.dim() == 3 else (0, 0, 0)
-    kv = _cache(k_cache, v_cache, dev, dt)
-    qi, qp, q_ts, q_hs, H = _rows("q", q, dev, dt, T, HD)
-    if kv[9] != HD or kv[8] < 1 or H % kv[8]:
-        raise ValueError(f"q is {tuple(q.shape)}, the cache holds {kv[8]} heads of {kv[9]}")
-    if block_table.dtype != torch.int32 or block_table.get_device() != dev or block_table.dim() != 2:
-        _refuse("block_table", block_table, dev, torch.int32, 2)
-    B, width = block_table.shape
-    t_row, one = block_table.stride()
-    _need(width <= 1 or one == 1, "block_table rows must be contiguous")
-    mask, mask_row = 0, 0
-    if key_mask is not None:
-        if key_mask.dtype not in (torch.uint8, torch.bool) or key_mask.get_device() != dev or key_mask.dim() != 2:
-            _refuse("key_mask", key_mask, dev, None, 2)
-            raise ValueError(f"key_mask is {key_mask.dtype}, expected uint8 or bool")
-        n, w = key_mask.shape
-        mask_row, one = key_mask.stride()
-        _need(n == B and w >= max_kv and (w <= 1 or one == 1),
-              f"key_mask is {tuple(key_mask.shape)}, expected [{B}, >= {max_kv}] with contiguous rows")
-        mask = key_mask.data_ptr()
-    if max_q < 0 or max_kv < 0:
-        raise ValueError(f"max_q={max_q}, max_kv={max_kv}")
-    out, op, o_ts, o_hs = _out("out", out, q)
-    lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
-    lib = _hip.load()
-    packed = bytearray(_ATTEND.pack(
-        *kv, qp, op, lse.data_ptr() if return_lse else 0, block_table.data_ptr(), _vec("cu_q", cu_q, dev, torch.int32, B + 1),
-        _vec("kv_len", kv_len, dev, torch.int32, B), _vec("q_index", q_index, dev, torch.int32, T), mask, 0, 0, q_ts, q_hs, o_ts, o_hs,
-        t_row if B > 1 else width, mask_row, T, H, B, width, max_q, max_kv, 1 if causal else 0, HD ** -0.5 if scale is None else scale))
-    need = lib.dark_paged_attention_workspace_bytes(bytes(packed))
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _WORKSPACE.pack_into(packed, _WORKSPACE_AT, ws.data_ptr(), need)
-    _call(lib.dark_paged_attention, bytes(packed), dev)
-    return (out, lse) if return_lse else out
+    return (_bind or _ops()).paged_attention(_stream(q), q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_kv, q_index,
+                                            key_mask, causal, scale, out, return_lse)
 
 
 class PagedKVCache:

@@ -406,3 +406,56 @@ def test_nothing_to_do():
     none = z(0, 16, 8, 96)
     out, lse = kv_cache.paged_attention(z(2, 8, 96) + 1, none, none, z(1, 0, dtype=torch.int32), i32(0, 2), i32(7), 2, 7, return_lse=True)
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_refused_operands():
+    """What a call cannot be given: said by name before anything is enqueued."""
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device=DEV)
+    q, k, cache = z(2, 8, 96), z(2, 4, 96), z(3, 16, 4, 96)
+    slots = torch.arange(2, device=DEV)
+    cos, sin, pos = z(64, 48), z(64, 48), z(2, dtype=torch.int32)
+    norm = lambda **kw: kv_cache.qk_norm_rope(*[{**dict(q=q, k=k, w=None, x=None, cos=cos, sin=sin, pos=pos), **kw}[n] for n in ("q", "k", "w", "x", "cos", "sin", "pos")])
+    for kw, msg in ((dict(q=q.double()), "float32 and bfloat16"), (dict(k=k.bfloat16()), "k is torch.bfloat16"), (dict(k=z(3, 4, 96)), r"k is \(3, 4, 96\)"),
+                    (dict(q=z(2, 8 * 96)), "q has 2 dimensions"), (dict(w=z(95)), "q_weight must be contiguous with 96"),
+                    (dict(sin=None), "go together"), (dict(pos=pos.long()), "pos is torch.int64"), (dict(pos=z(3, dtype=torch.int32)), "pos must be"),
+                    (dict(cos=z(64, 47)), "max_pos, 48"), (dict(k=k.cpu()), "k is on cpu")):
+        with pytest.raises(ValueError, match=msg):
+            norm(**kw)
+    with pytest.raises(TypeError, match="k must be a tensor"):
+        norm(k=None)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        norm(q=q.cpu())
+    with pytest.raises(RuntimeError, match="q requires gradients"):
+        norm(q=z(2, 8, 96).requires_grad_())
+    with torch.no_grad():
+        norm(q=z(2, 8, 96).requires_grad_())
+    with pytest.raises(ValueError, match="expanded"):
+        kv_cache.qk_norm_rope(q, k, None, None, None, None, None, q_out=z(1, 8, 96).expand(2, 8, 96))
+    with pytest.raises(ValueError, match="q_out is"):
+        kv_cache.qk_norm_rope(q, k, None, None, None, None, None, q_out=z(2, 7, 96))
+    with pytest.raises(_hip.DarkHipError, match="head_dim"):
+        kv_cache.qk_norm_rope(z(1, 2, 80), z(1, 2, 80), None, None, None, None, None)
+    app = lambda **kw: kv_cache.append_kv(*[{**dict(k=k, v=k, kc=cache, vc=cache.clone(), slots=slots), **kw}[n] for n in ("k", "v", "kc", "vc", "slots")])
+    for kw, msg in ((dict(slots=slots.int()), "slots is torch.int32"), (dict(kc=z(3, 12, 4, 96), vc=z(3, 12, 4, 96)), "power of two"),
+                    (dict(vc=z(3, 4, 16, 96).transpose(1, 2)), "same shape and strides"), (dict(kc=z(3, 16, 5, 96), vc=z(3, 16, 5, 96)), "heads of 96"),
+                    (dict(kc=z(1, 16, 4, 96).expand(3, 16, 4, 96), vc=z(1, 16, 4, 96).expand(3, 16, 4, 96)), "expanded"),
+                    (dict(v=z(2, 3, 96)), "the cache holds")):
+        with pytest.raises(ValueError, match=msg):
+            app(**kw)
+    with pytest.raises(TypeError, match="slots"):
+        app(slots=None)
+    with pytest.raises(ValueError, match="q_out without q"):
+        kv_cache.append_kv(k, k, cache, cache.clone(), slots, q_out=q)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    base = dict(q=q, kc=cache, vc=cache, table=z(1, 3, dtype=torch.int32), cu=i32(0, 2), kv=i32(5))
+    att = lambda mq=2, mk=5, **kw: kv_cache.paged_attention(*[{**base, **kw}[n] for n in ("q", "kc", "vc", "table", "cu", "kv")], mq, mk,
+                                                            **{n: v for n, v in kw.items() if n not in base})
+    assert att().shape == (2, 8, 96)
+    for kw, msg in ((dict(q=z(2, 6, 96)), "q is"), (dict(cu=i32(0, 1, 2)), "cu_q must be"), (dict(kv=i32(5).long()), "kv_len is torch.int64"),
+                    (dict(table=z(1, 3)), "block_table is torch.float32"), (dict(key_mask=z(1, 4, dtype=torch.uint8)), "key_mask is"),
+                    (dict(key_mask=z(1, 5)), "uint8 or bool"), (dict(mk=-1), "max_kv=-1"), (dict(q_index=i32(0)), "q_index must be"),
+                    (dict(out=z(2, 8, 96).bfloat16()), "out is torch.bfloat16")):
+        with pytest.raises(ValueError, match=msg):
+            att(**kw)
+    with pytest.raises(_hip.DarkHipError, match="scale"):
+        att(scale=math.nan)

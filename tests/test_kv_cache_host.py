@@ -10,15 +10,22 @@ from dark_amd import _hip, kv_cache
 from oracle import kv_cache_oracle as O
 
 
-def test_packed_structs_match_the_header():
-    assert kv_cache._NORM_ROPE.size == C.sizeof(_hip.QkNormRopeArgs)
-    assert kv_cache._APPEND.size == C.sizeof(_hip.KVAppendArgs)
-    assert kv_cache._ATTEND.size == C.sizeof(_hip.PagedAttentionArgs)
-    names = [n for n, _ in _hip.PagedKV._fields_] + [n for n, _ in _hip.PagedAttentionArgs._fields_[1:]]
-    vals = list(range(1, len(names) + 1))
-    a = _hip.PagedAttentionArgs.from_buffer_copy(kv_cache._ATTEND.pack(*vals))
-    got = [getattr(a.kv, n) for n, _ in _hip.PagedKV._fields_] + [getattr(a, n) for n, _ in _hip.PagedAttentionArgs._fields_[1:]]
-    assert got == vals
+def test_structs_match_the_header(tmp_path):
+    """Sizes and last fields of the ctypes structs against what a C compiler makes of include/dark_hip.h."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = {"dark_paged_kv": _hip.PagedKV, "dark_qk_norm_rope_args": _hip.QkNormRopeArgs, "dark_kv_append_args": _hip.KVAppendArgs,
+             "dark_paged_attention_args": _hip.PagedAttentionArgs, "dark_cached_tokens": _hip.CachedTokens,
+             "dark_layer_weights": _hip.LayerWeights, "dark_model_desc": _hip.ModelDesc}
+    src = '#include "dark_hip.h"\n#include <stdio.h>\nint main(void) {\n' + "".join(
+        f'  printf("{n} %zu %zu\\n", sizeof({n}), offsetof({n}, {s._fields_[-1][0]}));\n' for n, s in names.items()) + "  return 0;\n}\n"
+    (tmp_path / "s.c").write_text(src)
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
+    for line in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.splitlines():
+        n, size, last = line.split()
+        s = names[n]
+        assert C.sizeof(s) == int(size) and getattr(s, s._fields_[-1][0]).offset == int(last), n
 
 
 def _kv(**kw):

@@ -12,6 +12,8 @@
 // A long key axis is split over workgroups where there are few rows; parts (O, m, l) are joined by a second kernel.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace dark {
@@ -48,7 +50,7 @@ struct PagedArgs {
   const uint8_t* kmask;
   float *part_o, *part_ml;     // [n_split][T][H][HD], [n_split][T][H][2]; null when n_split == 1
   int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride, page_stride, slot_stride, head_stride;
-  int32_t T, H, Hk, G, B, width, n_pages, page_log2, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
+  int32_t T, H, Hk, G, B, width, n_pages, page_log2, unit, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
   Div by_hk, by_tiles, by_split, by_group, by_inner, by_heads, by_rows;   // by_rows: max_q * n_heads
   float scale_log2;            // scale * log2(e)
 };
@@ -163,7 +165,11 @@ __device__ __forceinline__ bool open_unit(const PagedArgs& a, int id, int li, Un
   id = a.by_tiles.divmod(q);
   const int tile = q;
   u.b = a.by_split.divmod(id);
-  u.split = id;
+  // each sequence begins its round of the XCDs with another part: the first parts, which short sequences have as well, would
+  // all fall to the same XCDs (64 x 1 over up to 16384: 462 us without, 404 with)
+  int shift = (int)(((uint32_t)u.b * 0x9E3779B1u) >> 16);
+  a.by_split.divmod(shift);
+  u.split = id + shift - (id + shift >= a.n_split ? a.n_split : 0);
   int t0 = a.cu_q[u.b], t1 = a.cu_q[u.b + 1];
   const int len = seq_len(a, u.b);
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
@@ -247,12 +253,15 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit& u, bo
 // ---- few rows (one token and its head group, a handful of masked positions): 16 rows of one key head against a stream of
 // keys that is read once.  Bound by HBM; what counts is bytes in flight, so every wave streams tiles of its own -- tile t's
 // successor is on its way into the registers t is done with, the pages of the one behind it are looked up -- and waits for
-// nobody: K rows go from
-// memory into the first product's operand as they are, V through LDS of the wave's own for the transposed read.
+// nobody.  K and V rows are read whole (16 lanes a row of 256 bytes) and turned into operands by way of LDS of the wave's
+// own: read from memory as the first product wants them, 64 bytes of each of 16 rows an instruction, every line is asked for
+// twice (64 x 1 over up to 16384: 518 us so, 440 whole, 402 = 6.1 TB/s whole and past the caches, see NT; a plain stream of
+// such rows reads 6.0 and 6.8 TB/s).  Two waves a SIMD: 502 us with three, 522 with one.
 // WPP waves share one problem (tiles dealt out in turn, joined in LDS at the end); WPP = 1: four problems a workgroup.
-template <int HD, int WPP>
+template <int HD, int WPP, bool ODD, bool NT>
 __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_few_kernel(const PagedArgs a) {
-  constexpr int LD = HD + 8, NC = HD / 32, NW = WPP == 8 ? 8 : 4;   // NC: 16-byte chunks of a row a lane holds
+  constexpr int LD = HD + 8, NC = HD / 32, NW = WPP == 8 ? 8 : 4;   // NC: 32-dim steps of the first product
+  constexpr int CH = HD / 8, NL = CH / 2;   // 16-byte chunks of a row; of a tile's K or V that a lane loads
   __shared__ __attribute__((aligned(16))) bf16_t Vall[NW][PT_KEYS * LD];
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -271,8 +280,8 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
 
   const int32_t* tab = a.table + u.b * a.table_stride;
   const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
-  const bf16_t* kbase = (const bf16_t*)a.k + (int64_t)u.hk * a.head_stride + g * 8;
-  const bf16_t* vbase = (const bf16_t*)a.v + (int64_t)u.hk * a.head_stride + g * 8;
+  const bf16_t* kbase = (const bf16_t*)a.k + (int64_t)u.hk * a.head_stride;
+  const bf16_t* vbase = (const bf16_t*)a.v + (int64_t)u.hk * a.head_stride;
   const int pmask = (1 << a.page_log2) - 1;
   // pages and masks of this lane's two keys of a tile as they stand in memory: looked at two tiles ahead and made sense of
   // one tile ahead, so that nothing waits for them
@@ -291,14 +300,34 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
     for (int jt = 0; jt < 2; ++jt)
       pg[jt] = (k0 + jt * 16 + li < k_end && rp[jt] < a.n_pages && rm[jt] != 0) ? rp[jt] : -1;
   };
-  // a lane's share of 32 rows (K or V); a key that is left out is read as zeros
-  auto fetch = [&](const bf16_t* base, int k0, const int (&pg)[2], bf16x8 (&x)[2][NC]) {
+  // where a lane's chunks of 32 rows lie: chunk n is number n * 64 + lane of the tile, its row's place comes from the lane that
+  // looked it up.  Rows are read whole, 1 KB an instruction.
+  auto spread = [&](int k0, const int (&pg)[2], int64_t (&off)[NL]) {
+    int64_t at[2];
 #pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      const bf16_t* p = base + (int64_t)pg[jt] * a.page_stride + (int64_t)((k0 + jt * 16 + li) & pmask) * a.slot_stride;
-      if (pg[jt] < 0) p = (const bf16_t*)kZeroRow + g * 8;
+    for (int jt = 0; jt < 2; ++jt)
+      at[jt] = pg[jt] < 0 ? -1 : (int64_t)pg[jt] * a.page_stride + (int64_t)((k0 + jt * 16 + li) & pmask) * a.slot_stride;
 #pragma unroll
-      for (int i = 0; i < NC; ++i) x[jt][i] = *(const bf16x8*)(p + i * 32);
+    for (int n = 0; n < NL; ++n) {
+      const int c = n % (NL / 2) * 64 + lane, row = c / CH, jt = n / (NL / 2);
+      const unsigned lo32 = (unsigned)__builtin_amdgcn_ds_bpermute(row * 4, (int)(uint32_t)at[jt]);
+      const int hi32 = __builtin_amdgcn_ds_bpermute(row * 4, (int)(at[jt] >> 32));
+      off[n] = (int64_t)hi32 << 32 | lo32;
+    }
+  };
+  auto fetch = [&](const bf16_t* base, const int64_t (&off)[NL], bf16x8 (&x)[NL]) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int col = (n % (NL / 2) * 64 + lane) % CH * 8;
+      const bf16_t* p = off[n] < 0 ? (const bf16_t*)kZeroRow : base + off[n];   // a key that is left out is read as zeros
+      x[n] = NT ? __builtin_nontemporal_load((const bf16x8*)(p + col)) : *(const bf16x8*)(p + col);
+    }
+  };
+  auto to_lds = [&](const bf16x8 (&x)[NL]) {   // (row = key, padded by 16 bytes: no bank conflict in either direction)
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int c = n * 64 + lane;
+      *(bf16x8*)(Vs + c / CH * LD + c % CH * 8) = x[n];
     }
   };
 
@@ -312,42 +341,42 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
   const int step = WPP * PT_KEYS;
   int k0 = k_begin + (WPP == 1 ? 0 : wave * PT_KEYS) - step;
   int pg[2] = {-1, -1}, pn[2];
-  bf16x8 kr[2][NC], vr[2][NC];
+  bf16x8 kr[NL], vr[NL];
+  int64_t off[NL];
   if (k0 + step < k_end) look(k0 + step);
   for (bool work = false; k0 < k_end; k0 += step, work = true) {
     if (k0 + step >= k_end && !work) break;
     place(k0 + step, pn);
     if (k0 + 2 * step < k_end) look(k0 + 2 * step);   // (before the rows: who waits for it does not wait for them)
-    // ---- S^T = K Q^T; K's registers then take the next tile's
+    spread(k0 + step, pn, off);
+    // ---- S^T = K Q^T by way of LDS; K's registers then take the next tile's
     f32x4 S[2];
+    if (work) to_lds(kr);
+    fetch(kbase, off, kr);
     if (work) {
+      wave_fence();   // lanes read what other lanes of the wave have written
 #pragma unroll
       for (int jt = 0; jt < 2; ++jt) {
         S[jt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < NC; ++i) S[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[jt][i], qb[i], S[jt], 0, 0, 0);
+        for (int i = 0; i < NC; ++i)
+          S[jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)(Vs + (jt * 16 + li) * LD + i * 32 + g * 8), qb[i], S[jt], 0, 0, 0);
       }
+      wave_fence();
     }
-    fetch(kbase, k0 + step, pn, kr);
-    // ---- V -> LDS (row = key, padded by 16 bytes: no bank conflict in either direction); V's registers likewise
+    // ---- V -> LDS in K's place; V's registers likewise
     bool odd = false;
-    const bool partial = k0 + PT_KEYS > lo;
     if (work) {
-      if (partial) {
+      if (ODD && k0 + PT_KEYS > lo && lo < k_end) {   // some row does not see a key that others do
 #pragma unroll
-        for (int jt = 0; jt < 2; ++jt)
+        for (int n = 0; n < NL; ++n)
 #pragma unroll
-          for (int i = 0; i < NC; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) odd |= !(fabsf((float)vr[jt][i][e]) < INFINITY);
+          for (int e = 0; e < 8; ++e) odd |= !(fabsf((float)vr[n][e]) < INFINITY);
         odd = __any(odd);
       }
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-        for (int i = 0; i < NC; ++i) *(bf16x8*)(Vs + (jt * 16 + li) * LD + i * 32 + g * 8) = vr[jt][i];
+      to_lds(vr);
     }
-    fetch(vbase, k0 + step, pn, vr);
+    fetch(vbase, off, vr);
     if (work) {
       // ---- softmax
       float mx = -INFINITY;
@@ -381,8 +410,8 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
           pb[jt * 4 + r] = (bf16_t)S[jt][r];   // (rounded for the matrix instruction: relative 2^-8 a weight)
         }
       // ---- O^T += V^T P^T
-      wave_fence();   // lanes read what other lanes of the wave have written
-      if (odd) {
+      wave_fence();
+      if (ODD && odd) {
         bf16x8 ind;
 #pragma unroll
         for (int jj = 0; jj < 8; ++jj) ind[jj] = S[jj >> 2][jj & 3] > 0.f ? (bf16_t)1.f : (bf16_t)0.f;
@@ -429,7 +458,7 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
 // ---- fp32: the same stream for any number of rows, 16 a workgroup, on 16 x 16 x 4 fp32 matrix instructions; nothing passes
 // through LDS.  The output's columns are dealt to the second product's rows so that a lane reads a V row's 16 bytes at
 // 64 c + 4 (lane & 15) -- 16 lanes a whole row piece -- and its four (HD 96: the last two) floats go to four instructions.
-template <int HD, int WPP>
+template <int HD, int WPP, bool ODD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const PagedArgs a) {
   constexpr int NC = HD / 16, KEYS = 16, NV = (HD + 63) / 64;   // NV: pieces of a V row a lane reads
   constexpr int E1 = HD == 96 ? 2 : 4;                                                      // floats of the second one
@@ -533,7 +562,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
         l += S[r];   // (this lane's keys only: the four lanes of a row are added up at the end)
       }
       // ---- O^T += V^T P^T
-      if (k0 + KEYS > lo) {
+      if (ODD && k0 + KEYS > lo && lo < k_end) {
         bool odd = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -616,7 +645,7 @@ template <int HD> struct TileSwz {
 
 constexpr int TT_ROWS = 128, TT_KEYS = 64;
 
-template <int HD>
+template <int HD, bool ODD>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   typedef TileSwz<HD> Z;
   typedef __attribute__((address_space(3))) void lds_void;
@@ -631,7 +660,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   int id = unit_of_block(a);
   if (id < 0 || id >= a.n_units) return;
   int rest = a.by_tiles.divmod(id);
-  const int tile = id;                                // (the tiles of a key head read the same keys)
+  const int tile = a.n_tiles - 1 - id;                // (the tiles of a key head read the same keys; the last see most and come
+                                                      // first: 2 chunks of 4096 tokens, causal, 343 -> 302 us)
   id = a.by_split.divmod(rest);
   const int split = rest, b = a.by_hk.divmod(id), hk = id;
   int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
@@ -683,11 +713,11 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
     raw_page = tab[key >> a.page_log2];
     if (km) raw_mask = km[key];
   };
-  // ... and where its row lies, in 16-byte units from its head's first; ~0: left out
+  // ... and where its row lies, in units of 2^unit elements from its head's first; ~0: left out
   auto place = [&](int k0) -> unsigned {
     const int key = k0 + lane;
     const bool on = key < k_end && raw_page >= 0 && raw_page < a.n_pages && raw_mask != 0;
-    return on ? (unsigned)(((int64_t)raw_page * a.page_stride + (int64_t)(key & pmask) * a.slot_stride) >> 3) : ~0u;
+    return on ? (unsigned)(((int64_t)raw_page * a.page_stride + (int64_t)(key & pmask) * a.slot_stride) >> a.unit) : ~0u;
   };
   // this wave's pieces of a tile: lane l of piece n fills chunk (n * 4 + wave) * 64 + l of the tile
   auto stage = [&](int buf, unsigned off) {
@@ -697,8 +727,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
       const unsigned o = __shfl(off, r, 64);
       const bool on = o != ~0u;
       const char* zr = (const char*)kZeroRow;
-      const char* kp = (on ? kbase + ((uint64_t)o << 4) : zr) + Z::k_chunk(r, pos) * 16;
-      const char* vp = (on ? vbase + ((uint64_t)o << 4) : zr) + Z::v_pos(r, pos) * 16;
+      const char* kp = (on ? kbase + ((uint64_t)o << (a.unit + 1)) : zr) + Z::k_chunk(r, pos) * 16;
+      const char* vp = (on ? vbase + ((uint64_t)o << (a.unit + 1)) : zr) + Z::v_pos(r, pos) * 16;
       char* to = smem + buf * (2 * TILE) + (n * 4 + wave) * 1024;
       __builtin_amdgcn_global_load_lds((gl_void*)kp, (lds_void*)to, 16, 0, 0);
       __builtin_amdgcn_global_load_lds((gl_void*)vp, (lds_void*)(to + TILE), 16, 0, 0);
@@ -726,8 +756,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
     stage(0, off);
     look(k_begin + TT_KEYS);
   }
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += TT_KEYS, buf ^= 1) {
+  // PART: some row may not see a key of the tile that others do
+  auto turn = [&](auto part_tag, int k0, int buf) {
+    constexpr bool PART = decltype(part_tag)::value;
     __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): this wave's pieces of the tile are in LDS, its reads are done;
     __builtin_amdgcn_s_barrier();         // everybody's are: the tile may be read, the other buffer refilled
     if (k0 + TT_KEYS < k_end) {
@@ -738,7 +769,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
     }
     const char* tl = smem + buf * (2 * TILE);
     int odd = 0;
-    if (k0 + TT_KEYS > lo) {   // some row does not see all of this tile: infinities and NaN in V have to be looked for
+    if (PART) {   // look for infinities and NaN in V
 #pragma unroll
       for (int n = 0; n < CH / 4; ++n) {
         const bf16x8 v = *(const bf16x8*)(tl + TILE + (n * 256 + tid) * 16);
@@ -770,7 +801,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
       }
       __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
-    if (odd) {   // (rare) V's infinities and NaN out of the tile, their codes in K's place
+    if (PART && odd) {   // (rare) V's infinities and NaN out of the tile, their codes in K's place
       __syncthreads();
 #pragma unroll 1
       for (int n = 0; n < CH / 4; ++n) {
@@ -789,7 +820,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
     }
     if (k0 < whi) {
       // ---- softmax: this lane's keys are 32 t + (i & 3) + 8 (i >> 2) + 4 h
-      if (on != ~0ull || k0 + TT_KEYS > wlo) {
+      if (on != ~0ull || (PART && k0 + TT_KEYS > wlo)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const unsigned w = (unsigned)(on >> (32 * t)) >> (4 * h);
@@ -837,7 +868,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) O[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_v(tl, s, dt), pb[s], O[dt], 0, 0, 0);
-      if (odd) {
+      if (PART && odd) {
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -853,7 +884,11 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
       }
     }
     on = on_next;
-  }
+  };
+  int k0 = k_begin, buf = 0;
+  for (const int whole = ODD && lo < k_end ? lo - TT_KEYS : k_end - 1; k0 <= whole; k0 += TT_KEYS, buf ^= 1) turn(std::false_type(), k0, buf);
+  if constexpr (ODD)
+    for (; k0 < k_end; k0 += TT_KEYS, buf ^= 1) turn(std::true_type(), k0, buf);
   l = pair_sum(l);
   if (!live) return;
   const bool parts = n_parts > 1 && a.n_split > 1;
@@ -934,6 +969,13 @@ struct PagedPlan {
   int64_t ws_o, ws_ml;   // bytes
 };
 
+// The row tiles' kernel hands a key's place from lane to lane as 32 bits: in units of the largest power of two that divides
+// the cache's strides (256 bytes for one head of 128 bf16, a cache of 1 TiB then).
+static int place_unit(const dark_paged_kv& kv) {
+  const uint64_t strides = (uint64_t)kv.page_stride | (uint64_t)kv.slot_stride | 1ull << 20;
+  return __builtin_ctzll(strides);
+}
+
 static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   PagedPlan s;
   const int64_t rows = (int64_t)p->max_q * (p->n_heads / p->kv.n_kv_heads);
@@ -945,12 +987,12 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   s.n_tiles = (int)((rows + tile_rows - 1) / tile_rows);
   if (s.n_tiles < 1) s.n_tiles = 1;
   const int64_t wgs = (int64_t)s.n_tiles * heads;
-  // Parts of a key axis.  Few problems: 512 of them fill the card (2 x 4 over 131072, 16 problems: 191 us with parts of 4096
-  // to 8192 keys, 197 with 2048: the join costs more).  Many, as with one token for each of many sequences: parts of 1024,
-  // because lengths differ and the longest must not finish alone (64 x 1 over 16384: 517 us, 580 with parts of 2048, 637
-  // with 8192).  Never below 256 keys: a part's (O, m, l) is then 1/16 of the keys' bytes at most.
+  // Parts of a key axis.  Few problems: 512 of them fill the card once (2 x 4 over 131072, 16 problems: 166 us; 172 with 1024
+  // parts, 184 with 768, 183 with 2048).  Many, as with one token for each of many sequences: parts of 1024, because lengths
+  // differ and the longest must not finish alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with
+  // 4096).  Never below 256 keys: a part's (O, m, l) is then 1/16 of the keys' bytes at most.
   int64_t keys = p->max_kv;
-  if (s.few != 1 && s.few != 8) {
+  if (s.few == 0 || s.few == 4) {
     if (wgs < 256) keys = (p->max_kv * wgs + 511) / 512;
     if (s.few && wgs >= 256 && keys > 1024) keys = 1024;
     if (keys < 256) keys = 256;
@@ -977,9 +1019,6 @@ static int check_paged_attention(const dark_paged_attention_args* p) {
   DARK_CHECK_ARG(p->n_tokens >= 0 && p->n_seqs >= 0 && p->table_width >= 0 && p->max_q >= 0 && p->max_kv >= 0 &&
                      p->n_tokens < (1 << 30), "%s: negative or too large size", who);
   DARK_CHECK_ARG((int64_t)p->table_width * p->kv.page_size < (1ll << 30) && p->max_kv < (1 << 30), "%s: 2^30 keys a sequence or more", who);
-  // (rows are addressed by 32-bit offsets in 16-byte units: 64 GiB of keys a layer)
-  DARK_CHECK_ARG((double)p->kv.page_stride * (p->kv.n_pages > 0 ? p->kv.n_pages - 1 : 0) + (double)p->kv.slot_stride * p->kv.page_size <
-                     8.0 * 4294967295.0 / (p->kv.dtype == DARK_BF16 ? 1 : 2), "%s: the cache spans more than 64 GiB", who);
   const int64_t G = p->n_heads / p->kv.n_kv_heads;
   DARK_CHECK_ARG(p->n_tokens * G < (1ll << 31) - 128 && p->max_q * G < (1ll << 31) - 128, "%s: 2^31 rows of a key head or more", who);
   DARK_CHECK_ARG(p->scale == p->scale && fabsf(p->scale) < INFINITY, "%s: scale is not finite", who);
@@ -1010,6 +1049,10 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   DARK_CHECK_ARG(p->table_stride >= p->table_width || p->n_seqs == 1, "%s: table_stride %lld < table_width %d", who, (long long)p->table_stride, p->table_width);
   hipStream_t st = (hipStream_t)stream;
   const PagedPlan s = plan_paged(p);
+  const int unit = place_unit(p->kv);
+  DARK_CHECK_ARG(s.few || (double)p->kv.page_stride * (p->kv.n_pages > 0 ? p->kv.n_pages - 1 : 0) +
+                              (double)p->kv.slot_stride * (p->kv.page_size - 1) < 4294967295.0 * (double)(1ll << unit),
+                 "%s: the cache spans more than 2^32 times the power of two in its strides (%lld elements)", who, 1ll << unit);
   DARK_CHECK_ARG(s.ws_o + s.ws_ml == 0 || (p->workspace && ((uintptr_t)p->workspace & 15) == 0 && p->workspace_bytes >= s.ws_o + s.ws_ml),
                  "%s: workspace %lld < required %lld bytes (or not 16-byte aligned)", who, (long long)p->workspace_bytes, (long long)(s.ws_o + s.ws_ml));
   DARK_TRY(check_stream_device(st));
@@ -1024,7 +1067,7 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   a.page_stride = p->kv.page_stride; a.slot_stride = p->kv.slot_stride; a.head_stride = p->kv.head_stride;
   a.T = p->n_tokens; a.H = p->n_heads; a.Hk = p->kv.n_kv_heads; a.G = p->n_heads / p->kv.n_kv_heads; a.B = p->n_seqs;
   a.width = p->table_width; a.n_pages = p->kv.n_pages; a.page_log2 = __builtin_ctz((unsigned)p->kv.page_size);
-  a.causal = p->causal != 0; a.n_split = s.n_split; a.split_keys = s.split_keys; a.n_tiles = s.n_tiles;
+  a.unit = unit; a.causal = p->causal != 0; a.n_split = s.n_split; a.split_keys = s.split_keys; a.n_tiles = s.n_tiles;
   const int64_t cap = (int64_t)p->table_width * p->kv.page_size;
   a.cap = (int)(cap < p->max_kv ? cap : p->max_kv);
   a.scale_log2 = p->scale * 1.44269504088896340736f;
@@ -1055,28 +1098,43 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   else if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<T, HDv, 1>), dim3((jrows + 3) / 4), jblock, 0, st, a)
 #define DARK_PAGED_BF16(HDv)                                                                        \
   do {                                                                                              \
-    if (s.few == 1) hipLaunchKernelGGL((paged_few_kernel<HDv, 1>), grid, block, 0, st, a);          \
-    else if (s.few == 4) hipLaunchKernelGGL((paged_few_kernel<HDv, 4>), grid, block, 0, st, a);     \
-    else if (s.few == 8) hipLaunchKernelGGL((paged_few_kernel<HDv, 8>), grid, block, 0, st, a);     \
+    if (s.few == 1) hipLaunchKernelGGL((paged_few_kernel<HDv, 1, ODD, false>), grid, block, 0, st, a);     \
+    else if (s.few == 4 && past) hipLaunchKernelGGL((paged_few_kernel<HDv, 4, ODD, true>), grid, block, 0, st, a); \
+    else if (s.few == 4) hipLaunchKernelGGL((paged_few_kernel<HDv, 4, ODD, false>), grid, block, 0, st, a); \
+    else if (s.few == 8) hipLaunchKernelGGL((paged_few_kernel<HDv, 8, ODD, false>), grid, block, 0, st, a); \
     else {                                                                                          \
       constexpr int lds = 4 * TT_KEYS * HDv * 2;                                                    \
       static SmemOptIn optin;                                                                       \
-      DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv>, lds, st));                         \
-      hipLaunchKernelGGL((paged_tile_kernel<HDv>), grid, block, lds, st, a);                        \
+      DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv, ODD>, lds, st));                    \
+      hipLaunchKernelGGL((paged_tile_kernel<HDv, ODD>), grid, block, lds, st, a);                   \
     }                                                                                               \
     DARK_JOIN(bf16_t, HDv);                                                                         \
   } while (0)
 #define DARK_PAGED_F32(HDv)                                                                         \
   do {                                                                                              \
-    if (s.few == 1) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1>), grid, block, 0, st, a);          \
-    else hipLaunchKernelGGL((paged_f32_kernel<HDv, 4>), grid, block, 0, st, a);                     \
+    if (s.few == 1) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1, ODD>), grid, block, 0, st, a);     \
+    else hipLaunchKernelGGL((paged_f32_kernel<HDv, 4, ODD>), grid, block, 0, st, a);                \
     DARK_JOIN(float, HDv);                                                                          \
   } while (0)
   const int HD = p->kv.head_dim;
-  if (p->kv.dtype == DARK_BF16) {
-    if (HD == 64) DARK_PAGED_BF16(64); else if (HD == 96) DARK_PAGED_BF16(96); else DARK_PAGED_BF16(128);
+  // NT: keys that cannot stay in the 256 MB behind the L2s until somebody reads them again go past the caches (64 x 1 over up
+  // to 16384, 2.5 GB: 402 us, 440 without; 1024 x 11 over 46, 178 MB read again and again: 36.8 and 29.5 the other way)
+  const bool past = (int64_t)p->n_seqs * a.cap * p->kv.n_kv_heads * HD * es * 2 > (int64_t)256 << 20;
+  // rows of one tile see different keys only where a token's own place bounds them and a tile holds several tokens
+  if (p->causal && p->max_q > 1) {
+    constexpr bool ODD = true;
+    if (p->kv.dtype == DARK_BF16) {
+      if (HD == 64) DARK_PAGED_BF16(64); else if (HD == 96) DARK_PAGED_BF16(96); else DARK_PAGED_BF16(128);
+    } else {
+      if (HD == 64) DARK_PAGED_F32(64); else if (HD == 96) DARK_PAGED_F32(96); else DARK_PAGED_F32(128);
+    }
   } else {
-    if (HD == 64) DARK_PAGED_F32(64); else if (HD == 96) DARK_PAGED_F32(96); else DARK_PAGED_F32(128);
+    constexpr bool ODD = false;
+    if (p->kv.dtype == DARK_BF16) {
+      if (HD == 64) DARK_PAGED_BF16(64); else if (HD == 96) DARK_PAGED_BF16(96); else DARK_PAGED_BF16(128);
+    } else {
+      if (HD == 64) DARK_PAGED_F32(64); else if (HD == 96) DARK_PAGED_F32(96); else DARK_PAGED_F32(128);
+    }
   }
 #undef DARK_JOIN
 #undef DARK_PAGED_BF16

@@ -51,7 +51,7 @@ template <> struct RowVec<float> {
   __device__ static __forceinline__ raw down(const float (&f)[4]) { return (raw){f[0], f[1], f[2], f[3]}; }
 };
 
-template <typename T, int HD, bool NORM>
+template <typename T, int HD, bool NORM, bool PAST>
 __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
   constexpr int N = RowVec<T>::N, HALF = HD / 2, CH = HALF / N;         // CH lanes hold a row
   constexpr int LPR = CH <= 4 ? 4 : CH <= 8 ? 8 : 16, RPP = 64 / LPR;   // lanes a row is given, rows of one pass
@@ -153,8 +153,13 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
     const bool kept = !paged || (to >= 0 && to < a.n_slots);
     if (on && kept) {
       T* d = dst + (paged ? (to >> a.page_log2) * a.page_stride + (to & (((int64_t)1 << a.page_log2) - 1)) * dst_ts : t * dst_ts);
-      *(raw*)d = y1;
-      *(raw*)(d + HALF) = y2;
+      if constexpr (PAST) {
+        __builtin_nontemporal_store(y1, (raw*)d);
+        __builtin_nontemporal_store(y2, (raw*)(d + HALF));
+      } else {
+        *(raw*)d = y1;
+        *(raw*)(d + HALF) = y2;
+      }
     }
     if (tn >= a.T) return;
     t = tn;
@@ -199,12 +204,17 @@ static int launch_head_rows(RowsArgs& a, int dtype, int HD, hipStream_t st) {
   // 256 CUs x 32 waves walk over the tokens
   const int most = cdiv(8192, a.n_pass);
   a.t_step = a.T < most ? a.T : most;
+  // rows that the 256 MB behind the L2s cannot hold for their reader are written past them (16383 tokens x 40 fp32 heads of
+  // 128, 0.7 GB moved: 129 us, 139 without; 512 x 46 x 16 bf16 heads of 96: 30.6 and 29.2, but then they are there to be read)
+  const bool past = (int64_t)a.T * a.h_end[2] * HD * (dtype == DARK_BF16 ? 2 : 4) > (int64_t)256 << 20;
   const dim3 grid((unsigned)cdiv(a.t_step * a.n_pass, 4)), block(256);
   const bool norm = a.w[0] || a.w[1];
-#define DARK_ROWS(T, HDv)                                                                           \
-  do {                                                                                              \
-    if (norm) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true>), grid, block, 0, st, a);          \
-    else hipLaunchKernelGGL((head_rows_kernel<T, HDv, false>), grid, block, 0, st, a);              \
+#define DARK_ROWS(T, HDv)                                                                                  \
+  do {                                                                                                     \
+    if (norm && past) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true, true>), grid, block, 0, st, a);   \
+    else if (norm) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true, false>), grid, block, 0, st, a);     \
+    else if (past) hipLaunchKernelGGL((head_rows_kernel<T, HDv, false, true>), grid, block, 0, st, a);     \
+    else hipLaunchKernelGGL((head_rows_kernel<T, HDv, false, false>), grid, block, 0, st, a);              \
   } while (0)
   if (dtype == DARK_BF16) {
     if (HD == 64) DARK_ROWS(bf16_t, 64); else if (HD == 96) DARK_ROWS(bf16_t, 96); else DARK_ROWS(bf16_t, 128);

@@ -99,6 +99,36 @@ def test_qk_norm_rope_strides():
         assert torch.equal(y, a)
 
 
+@pytest.mark.parametrize("dtype,T,H,Hk,D", [(torch.bfloat16, 150001, 4, 3, 128), (torch.float32, 180000, 5, 1, 64), (torch.bfloat16, 470000, 2, 1, 96)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_more_rows_than_the_caches_hold(dtype, T, H, Hk, D, norm):
+    """Over 256 MB of rows, normed, rotated and stored; a sample of them checked."""
+    assert T * (H + 2 * Hk) * D * dtype.itemsize > 256 << 20
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, H + 2 * Hk, D, generator=g).to(dtype)
+    w = 1 + 0.2 * torch.randn(D, generator=g)
+    cos, sin = tables(1000, D)
+    pos = torch.randint(0, 1000, (T,), generator=g, dtype=torch.int32)
+    at = torch.cat([torch.tensor([0, T - 1]), torch.randint(0, T, (500,), generator=g)])
+    d = lambda t: t.to(DEV)
+    args = (d(w), d(w)) if norm else (None, None)
+    xd = d(x)
+    ref = {r: O.norm_rope(x[at, h], w if norm else None, cos, sin, pos[at], 1e-6) for r, h in (("q", slice(0, H)), ("k", slice(H, H + Hk)))}
+    if T * (H + Hk) * D * dtype.itemsize > 256 << 20:
+        q, k = kv_cache.qk_norm_rope(xd[:, :H], xd[:, H:H + Hk], *args, d(cos), d(sin), d(pos), eps=1e-6)
+        check_rows(q[d(at)], *ref["q"], dtype)
+        check_rows(k[d(at)], *ref["k"], dtype)
+    n_pages = -(-T // 64)
+    kc = torch.zeros(n_pages, 64, Hk, D, dtype=dtype, device=DEV)
+    vc = torch.zeros_like(kc)
+    slots = torch.randperm(n_pages * 64, generator=g)[:T]
+    q = kv_cache.append_kv(xd[:, H:H + Hk], xd[:, H + Hk:], kc, vc, d(slots), d(cos), d(sin), d(pos), q=xd[:, :H], q_weight=args[0],
+                           k_weight=args[1], eps=1e-6)
+    check_rows(q[d(at)], *ref["q"], dtype)
+    check_rows(kc.view(-1, Hk, D)[d(slots[at])], *ref["k"], dtype)
+    assert torch.equal(vc.view(-1, Hk, D)[d(slots)], xd[:, H + Hk:])
+
+
 # --------------------------------------------------------------------------- append
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T,H,Hk,D,page", [(1, 8, 8, 96, 16), (53, 12, 12, 64, 1), (200, 32, 8, 128, 64), (7, 3, 1, 96, 4096)])
@@ -270,6 +300,20 @@ def test_long_key_axis(dtype, q_lens, kv_lens, H, Hk, D, page, causal):
     check_attention(out, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=causal), max(kv_lens), D, dtype, lse)
     for _ in range(3):
         assert torch.equal(run_paged(p, causal=causal), out)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,H,Hk,D,page", [([1, 1, 4], [3001, 1, 700], 8, 2, 128, 64), ([1, 0, 2], [5000, 3, 0], 8, 4, 96, 16),
+                                                       ([1, 3], [2111, 65], 4, 4, 64, 16)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_tables_wider_than_the_caches_hold(q_lens, kv_lens, H, Hk, D, page, causal):
+    """Tables with room for over 256 MB of keys (their rows are then read past the caches), of which the sequences have a few."""
+    p = paged(q_lens, kv_lens, H, Hk, D, page, torch.bfloat16, seed=6)
+    p["max_kv"] = 140000
+    assert len(q_lens) * 140000 * Hk * D * 4 > 256 << 20
+    p["table"] = torch.cat([p["table"], torch.full((len(q_lens), -(-140000 // page) - p["table"].shape[1]), -3, dtype=torch.int32)], 1)
+    out, lse = run_paged(p, causal=causal, return_lse=True)
+    check_attention(out, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=causal), max(kv_lens), D, torch.bfloat16, lse)
+    assert torch.equal(run_paged(p, causal=causal), out)
 
 
 def test_views_strides_and_scores_far_apart():

@@ -153,6 +153,15 @@ __device__ __attribute__((aligned(16))) const unsigned kZeroRow[128] = {};   // 
 
 constexpr int PT_KEYS = 32;   // keys of a streamed tile
 
+// A load from global memory.  Said so, because the choice between a row and kZeroRow leaves the compiler a pointer of no known
+// memory: it then loads with instructions that LDS may serve as well, and waits for those before it touches LDS
+// (1024 x 11 over 46: 29.4 us so, 27.2).
+template <bool NT = false, typename V>
+__device__ __forceinline__ V load_global(const V* p) {
+  typedef const __attribute__((address_space(1))) V global_v;
+  return NT ? __builtin_nontemporal_load((global_v*)p) : *(global_v*)p;
+}
+
 // ---- what a wave of the streaming kernels works on: 16 rows of one key head against a part of its sequence's keys
 struct Unit {
   int b, hk, split, t0, row0, rows, tok, hq;   // row0: first of the 16; tok, hq: this lane's row (lane & 15)
@@ -160,10 +169,10 @@ struct Unit {
   bool live;
 };
 __device__ __forceinline__ bool open_unit(const PagedArgs& a, int id, int li, Unit& u) {
-  int q = a.by_hk.divmod(id);
-  u.hk = id;                         // (the key heads of a token lie next to each other)
-  id = a.by_tiles.divmod(q);
-  const int tile = q;
+  int q = a.by_tiles.divmod(id);
+  const int tile = id;               // (the tiles of a key head read the same keys, ...
+  id = a.by_hk.divmod(q);
+  u.hk = q;                          // ... the key heads of a token lie next to each other)
   u.b = a.by_split.divmod(id);
   // each sequence begins its round of the XCDs with another part: the first parts, which short sequences have as well, would
   // all fall to the same XCDs (64 x 1 over up to 16384: 462 us without, 404 with)
@@ -320,7 +329,7 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
     for (int n = 0; n < NL; ++n) {
       const int col = (n % (NL / 2) * 64 + lane) % CH * 8;
       const bf16_t* p = off[n] < 0 ? (const bf16_t*)kZeroRow : base + off[n];   // a key that is left out is read as zeros
-      x[n] = NT ? __builtin_nontemporal_load((const bf16x8*)(p + col)) : *(const bf16x8*)(p + col);
+      x[n] = load_global<NT>((const bf16x8*)(p + col));
     }
   };
   auto to_lds = [&](const bf16x8 (&x)[NL]) {   // (row = key, padded by 16 bytes: no bank conflict in either direction)
@@ -458,6 +467,8 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
 // ---- fp32: the same stream for any number of rows, 16 a workgroup, on 16 x 16 x 4 fp32 matrix instructions; nothing passes
 // through LDS.  The output's columns are dealt to the second product's rows so that a lane reads a V row's 16 bytes at
 // 64 c + 4 (lane & 15) -- 16 lanes a whole row piece -- and its four (HD 96: the last two) floats go to four instructions.
+// 16 sequences of 9 to 128 new tokens over 31 to 512 keys, 12 heads of 64: 23.4 us, 29 TFLOP/s; the SIMDs that get the long
+// sequences' rows work twice as long as the average.  (Eight waves a problem: 28.5 us; one: 47.)
 template <int HD, int WPP, bool ODD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const PagedArgs a) {
   constexpr int NC = HD / 16, KEYS = 16, NV = (HD + 63) / 64;   // NV: pieces of a V row a lane reads
@@ -479,7 +490,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
   for (int i = 0; i < NC; ++i) qf[i] = *(const f32x4*)(qrow + 16 * i);
   const int32_t* tab = a.table + u.b * a.table_stride;
   const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
-  const float* kbase = (const float*)a.k + (int64_t)u.hk * a.head_stride + g * 4;
+  const float* kbase = (const float*)a.k + (int64_t)u.hk * a.head_stride;
   const float* vbase = (const float*)a.v + (int64_t)u.hk * a.head_stride;
   const int pmask = (1 << a.page_log2) - 1;
   int rp = -1, rm = 1;   // page and mask of key k0 + li as they stand in memory
@@ -488,26 +499,29 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
     rp = tab[key >> a.page_log2];
     if (km) rm = km[key];
   };
-  auto place = [&](int k0) { return k0 + li < k_end && rp < a.n_pages && rm != 0 ? rp : -1; };   // -1: left out
-  f32x4 kr[NC], v0[4], v1[4];
-  auto fetch_k = [&](int k0, int pg) {
-    const float* p = kbase + (int64_t)pg * a.page_stride + (int64_t)((k0 + li) & pmask) * a.slot_stride;
-    if (pg < 0) p = (const float*)kZeroRow + g * 4;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) kr[i] = *(const f32x4*)(p + i * 16);
+  // where key k0 + li lies, in elements from its head's first; -1: left out, read as zeros
+  auto place = [&](int k0) -> int64_t {
+    const bool on = k0 + li < k_end && rp >= 0 && rp < a.n_pages && rm != 0;
+    return on ? (int64_t)rp * a.page_stride + (int64_t)((k0 + li) & pmask) * a.slot_stride : -1;
   };
-  auto fetch_v = [&](int k0, int pg) {   // rows 4 g + r: the keys whose weights this lane group holds
+  f32x4 kr[NC], v0[4], v1[4];
+  auto fetch_k = [&](int64_t at) {
+    const float* p = (at < 0 ? (const float*)kZeroRow : kbase + at) + g * 4;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) kr[i] = load_global((const f32x4*)(p + i * 16));
+  };
+  auto fetch_v = [&](int64_t at) {   // rows 4 g + r: the keys whose weights this lane group holds
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int pv = __shfl(pg, 4 * g + r, 16);
-      const float* p = vbase + (int64_t)pv * a.page_stride + (int64_t)((k0 + 4 * g + r) & pmask) * a.slot_stride;
-      if (pv < 0) p = (const float*)kZeroRow;
-      v0[r] = *(const f32x4*)(p + li * 4);
+      const unsigned lo32 = (unsigned)__builtin_amdgcn_ds_bpermute((4 * g + r) * 4, (int)(uint32_t)at);
+      const int hi32 = __builtin_amdgcn_ds_bpermute((4 * g + r) * 4, (int)(at >> 32));
+      const float* p = hi32 < 0 ? (const float*)kZeroRow : vbase + ((int64_t)hi32 << 32 | lo32);
+      v0[r] = load_global((const f32x4*)(p + li * 4));
       if constexpr (E1 == 2) {
-        const f32x2 x = *(const f32x2*)(p + 64 + li * 2);
+        const f32x2 x = load_global((const f32x2*)(p + 64 + li * 2));
         v1[r] = (f32x4){x[0], x[1], 0.f, 0.f};
       } else if constexpr (NV == 2) {
-        v1[r] = *(const f32x4*)(p + 64 + li * 4);
+        v1[r] = load_global((const f32x4*)(p + 64 + li * 4));
       }
     }
   };
@@ -518,7 +532,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
   float m = -INFINITY, l = 0.f;
   // (one turn brings tile t + 1 in and works on tile t, as above)
   const int step = WPP * KEYS;
-  int k0 = k_begin + (WPP == 1 ? 0 : wave * KEYS) - step, pg = -1, pn;
+  int k0 = k_begin + (WPP == 1 ? 0 : wave * KEYS) - step;
+  int64_t pg = -1, pn;
   if (k0 + step < k_end) look(k0 + step);
   for (bool work = false; k0 < k_end; k0 += step, work = true) {
     if (k0 + step >= k_end && !work) break;
@@ -536,7 +551,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
         }
       S += S2;
     }
-    fetch_k(k0 + step, pn);
+    fetch_k(pn);
     if (work) {
       float mx = -INFINITY;
       const unsigned on = (unsigned)__ballot(pg >= 0) >> (4 * g);   // (lanes 0..15 hold the 16 keys)
@@ -590,7 +605,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
         for (int i = 0; i < NC; ++i)
           O[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(i < 4 ? v0[r][i & 3] : v1[r][i & 3], S[r], O[i], 0, 0, 0);
     }
-    fetch_v(k0 + step, pn);
+    fetch_v(pn);
     pg = pn;
   }
   l = quad_sum(l);
@@ -1078,13 +1093,17 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   a.by_hk = make_div(a.Hk); a.by_tiles = make_div(s.n_tiles); a.by_split = make_div(s.n_split); a.by_group = make_div(a.G);
   a.by_heads = make_div(a.H); a.by_rows = make_div((int)(s.n_split > 1 ? (int64_t)p->max_q * a.H : 1));
   DARK_CHECK_ARG(s.n_split == 1 || (int64_t)p->n_seqs * p->max_q * p->n_heads < (1ll << 31), "%s: too many rows", who);
-  // units that share memory on one XCD, where there are enough such groups for all eight
+  // Units that share memory on one XCD: all heads and row tiles of a part, or else the row tiles of a key head -- where there
+  // are enough such groups to even out what they hold, or eight heads that hold the same (16 sequences of up to 512 keys,
+  // 12 heads, fp32: 27.4 us, 30.4 with the sequences dealt out whole).
   int blocks = s.few == 1 ? (int)((wgs + 3) / 4) : (int)wgs;
   a.n_inner = 1;
-  for (int inner : {s.few ? p->kv.n_kv_heads * s.n_tiles : s.n_tiles, s.few ? p->kv.n_kv_heads : 1}) {
-    if (s.few == 1) inner /= 4;   // (four units a workgroup)
+  for (const bool all : {true, false}) {
+    int inner = (all ? p->kv.n_kv_heads : 1) * s.n_tiles;
+    if (all && !s.few) continue;    // (its units are ordered by heads first)
+    if (s.few == 1) inner /= 4;     // (four units a workgroup)
     const int groups = inner > 1 ? cdiv(blocks, inner) : 0;
-    if (groups >= 64 || (groups > 0 && groups % 8 == 0)) {
+    if (groups >= 64 || (groups > 0 && !all && p->kv.n_kv_heads % 8 == 0)) {
       a.n_inner = inner;
       blocks = cdiv(groups, 8) * 8 * inner;
       break;

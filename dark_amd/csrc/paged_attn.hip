@@ -264,7 +264,7 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit& u, bo
 // successor is on its way into the registers t is done with, the pages of the one behind it are looked up -- and waits for
 // nobody.  K and V rows are read whole (16 lanes a row of 256 bytes) and turned into operands by way of LDS of the wave's
 // own: read from memory as the first product wants them, 64 bytes of each of 16 rows an instruction, every line is asked for
-// twice (64 x 1 over up to 16384: 518 us so, 440 whole, 402 = 6.1 TB/s whole and past the caches, see NT; a plain stream of
+// twice (64 x 1 over up to 16384: 518 us so, 435 whole, 399 = 6.2 TB/s whole and past the caches, see NT; a plain stream of
 // such rows reads 6.0 and 6.8 TB/s).  Two waves a SIMD: 502 us with three, 522 with one.
 // WPP waves share one problem (tiles dealt out in turn, joined in LDS at the end); WPP = 1: four problems a workgroup.
 template <int HD, int WPP, bool ODD, bool NT>
@@ -997,7 +997,13 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   const int64_t heads = (int64_t)p->kv.n_kv_heads * p->n_seqs;
   s.few = 0;
   if (p->kv.dtype == DARK_F32) s.few = p->max_kv <= 128 ? 1 : 4;
-  else if (rows <= 16) s.few = p->max_kv <= 128 ? 1 : (heads <= 64 && p->max_kv <= 1024) ? 8 : 4;
+  else if (rows <= 16) {
+    // Waves a problem: one where keys are few, eight where CUs are left over and the axis is short (16 x 1 over 900, 8 heads of
+    // 128: 14.6 us, 17.7 with four; over 1900: 29.3, 24.2 with four and a join; 12 heads of 64 over 1900: 15.2 and 24.0;
+    // 256 problems: 18.7 and 18.2)
+    const bool wide = heads <= 192 && p->max_kv <= (p->kv.head_dim == 64 ? 2048 : 1024);
+    s.few = p->max_kv <= 128 ? 1 : wide ? 8 : 4;
+  }
   const int tile_rows = s.few ? 16 : TT_ROWS;
   s.n_tiles = (int)((rows + tile_rows - 1) / tile_rows);
   if (s.n_tiles < 1) s.n_tiles = 1;
@@ -1005,11 +1011,12 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   // Parts of a key axis.  Few problems: 512 of them fill the card once (2 x 4 over 131072, 16 problems: 166 us; 172 with 1024
   // parts, 184 with 768, 183 with 2048).  Many, as with one token for each of many sequences: parts of 1024, because lengths
   // differ and the longest must not finish alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with
-  // 4096).  Never below 256 keys: a part's (O, m, l) is then 1/16 of the keys' bytes at most.
+  // 4096), of 512 where the card would be filled twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024).  Never
+  // below 256 keys: a part's (O, m, l) is then 1/16 of the keys' bytes at most.
   int64_t keys = p->max_kv;
   if (s.few == 0 || s.few == 4) {
     if (wgs < 256) keys = (p->max_kv * wgs + 511) / 512;
-    if (s.few && wgs >= 256 && keys > 1024) keys = 1024;
+    if (s.few && wgs >= 256 && keys > 1024) keys = wgs * ((keys + 1023) / 1024) <= (p->kv.head_dim == 64 ? 2048 : 1024) ? 512 : 1024;
     if (keys < 256) keys = 256;
   }
   s.split_keys = (int)((keys + 63) / 64 * 64);
@@ -1118,7 +1125,7 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
 #define DARK_PAGED_BF16(HDv)                                                                        \
   do {                                                                                              \
     if (s.few == 1) hipLaunchKernelGGL((paged_few_kernel<HDv, 1, ODD, false>), grid, block, 0, st, a);     \
-    else if (s.few == 4 && past) hipLaunchKernelGGL((paged_few_kernel<HDv, 4, ODD, true>), grid, block, 0, st, a); \
+    else if (s.few == 4 && past) hipLaunchKernelGGL((paged_few_kernel<HDv, 4, ODD, HDv % 64 == 0>), grid, block, 0, st, a); \
     else if (s.few == 4) hipLaunchKernelGGL((paged_few_kernel<HDv, 4, ODD, false>), grid, block, 0, st, a); \
     else if (s.few == 8) hipLaunchKernelGGL((paged_few_kernel<HDv, 8, ODD, false>), grid, block, 0, st, a); \
     else {                                                                                          \
@@ -1136,9 +1143,11 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
     DARK_JOIN(float, HDv);                                                                          \
   } while (0)
   const int HD = p->kv.head_dim;
-  // NT: keys that cannot stay in the 256 MB behind the L2s until somebody reads them again go past the caches (64 x 1 over up
-  // to 16384, 2.5 GB: 402 us, 440 without; 1024 x 11 over 46, 178 MB read again and again: 36.8 and 29.5 the other way)
-  const bool past = (int64_t)p->n_seqs * a.cap * p->kv.n_kv_heads * HD * es * 2 > (int64_t)256 << 20;
+  // NT: keys that, with four layers of them, cannot stay in the 256 MB behind the L2s until they are read again go past the caches (64 x 1 over up
+  // to 16384, 2.5 GB: 399 us, 435 without; head_dim 64: 207 and 234; 113 MB among other layers': 29.3 and 32.2, again and
+  // again: 27.0 and 26.0) -- if their rows are whole 128-byte lines: a line that two rows share is then read twice (head_dim 96:
+  // 365 and 331)
+  const bool past = HD % 64 == 0 && (int64_t)p->n_seqs * a.cap * p->kv.n_kv_heads * HD * es * 2 > (int64_t)64 << 20;
   // rows of one tile see different keys only where a token's own place bounds them and a tile holds several tokens
   if (p->causal && p->max_q > 1) {
     constexpr bool ODD = true;

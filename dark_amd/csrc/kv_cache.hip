@@ -51,11 +51,20 @@ template <> struct RowVec<float> {
   __device__ static __forceinline__ raw down(const float (&f)[4]) { return (raw){f[0], f[1], f[2], f[3]}; }
 };
 
+// 1 / sqrt(x), off by one unit in the last place (the instruction takes small denormals for zeros)
+__device__ __forceinline__ float rsqrt_of(float x) {
+  const bool tiny = x < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(tiny ? x * 0x1p100f : x) * (tiny ? 0x1p50f : 1.f);
+}
+
+// Every condition around a load is the same for the whole wave: lanes without a row of their own load the last one, a side
+// without weights the other's (a branch of its own around each had every load waited for: 512 x 46 40.8 us so, 36.5).
 template <typename T, int HD, bool NORM, bool PAST>
 __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
   constexpr int N = RowVec<T>::N, HALF = HD / 2, CH = HALF / N;         // CH lanes hold a row
   constexpr int LPR = CH <= 4 ? 4 : CH <= 8 ? 8 : 16, RPP = 64 / LPR;   // lanes a row is given, rows of one pass
   typedef typename RowVec<T>::raw raw;
+  typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));   // (weights may begin at any float)
   const int lane = threadIdx.x & 63;
   const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pass = unit % a.n_pass, step = a.t_step;
@@ -63,41 +72,42 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
   if (t >= step || t >= a.T) return;
   const int c = lane & (LPR - 1), r = pass * RPP + lane / LPR;
   const bool on = c < CH && r < a.h_end[2];
-  const int role = r < a.h_end[0] ? 0 : r < a.h_end[1] ? 1 : 2;
-  const int h = on ? r - (role == 0 ? 0 : role == 1 ? a.h_end[0] : a.h_end[1]) : 0, at = on ? c * N : 0;
-  const T* src = (const T*)(role == 0 ? a.src[0] : role == 1 ? a.src[1] : a.src[2]) +
-                 h * (role == 0 ? a.src_hs[0] : role == 1 ? a.src_hs[1] : a.src_hs[2]) + at;
+  const int rr = r < a.h_end[2] ? r : a.h_end[2] - 1, at = (c < CH ? c : 0) * N;
+  const int role = rr < a.h_end[0] ? 0 : rr < a.h_end[1] ? 1 : 2;
+  const int h = rr - (role == 0 ? 0 : role == 1 ? a.h_end[0] : a.h_end[1]);
   const int64_t src_ts = role == 0 ? a.src_ts[0] : role == 1 ? a.src_ts[1] : a.src_ts[2];
-  T* dst = (T*)(role == 0 ? a.dst[0] : role == 1 ? a.dst[1] : a.dst[2]) +
-           h * (role == 0 ? a.dst_hs[0] : role == 1 ? a.dst_hs[1] : a.dst_hs[2]) + at;
+  const T* src = (const T*)(role == 0 ? a.src[0] : role == 1 ? a.src[1] : a.src[2]) +
+                 h * (role == 0 ? a.src_hs[0] : role == 1 ? a.src_hs[1] : a.src_hs[2]) + t * src_ts + at;
+  const bool paged = role > 0 && a.slots;
   const int64_t dst_ts = role == 0 ? a.dst_ts[0] : role == 1 ? a.dst_ts[1] : a.dst_ts[2];
-  const bool paged = role > 0 && a.slots, turned = role < 2 && a.cosT;
-  const float* wp = role == 0 ? a.w[0] : role == 1 ? a.w[1] : nullptr;
+  T* dst = (T*)(role == 0 ? a.dst[0] : role == 1 ? a.dst[1] : a.dst[2]) +
+           h * (role == 0 ? a.dst_hs[0] : role == 1 ? a.dst_hs[1] : a.dst_hs[2]) + (paged ? 0 : t * dst_ts) + at;
   float w[2 * N];
+  bool normed = false;
   if constexpr (NORM) {
+    normed = role == 0 ? a.w[0] != nullptr : role == 1 && a.w[1] != nullptr;
+    const float* wp = normed ? (role == 0 ? a.w[0] : a.w[1]) : (a.w[0] ? a.w[0] : a.w[1]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      w[i] = wp ? wp[at + i] : 1.f;
-      w[N + i] = wp ? wp[HALF + at + i] : 1.f;
+    for (int i = 0; i < N; i += 4) {
+      *(f32x4*)(w + i) = *(const f32x4_any*)(wp + at + i);
+      *(f32x4*)(w + N + i) = *(const f32x4_any*)(wp + HALF + at + i);
     }
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) w[i] = normed ? w[i] : 1.f;
   }
-  raw x1 = {}, x2 = {};
+  raw x1, x2;
   float cs[N], sn[N];
-  int p = 0, p_next = 0;
   int64_t slot = 0;
   auto position = [&](int tt) {
-    if (!turned || tt >= a.T) return 0;
+    if (!a.cosT || tt >= a.T) return 0;
     const int q = a.pos ? a.pos[tt] : tt % a.pos_period;
     return q < 0 ? 0 : (q >= a.max_pos ? a.max_pos - 1 : q);
   };
-  auto fetch = [&](int tt, int pp) {
-    if (on) {
-      const T* s = src + tt * src_ts;
-      x1 = *(const raw*)s;
-      x2 = *(const raw*)(s + HALF);
-    }
-    if (paged) slot = a.slots[tt];
-    if (turned) {
+  auto fetch = [&](int tt, int pp) {   // (src is at token tt)
+    x1 = *(const raw*)src;
+    x2 = *(const raw*)(src + HALF);
+    if (a.slots) slot = a.slots[tt];
+    if (a.cosT) {
       const float* cp = a.cosT + (int64_t)pp * HALF + at;
       const float* sp = a.sinT + (int64_t)pp * HALF + at;
 #pragma unroll
@@ -109,9 +119,8 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
   };
 #pragma unroll
   for (int i = 0; i < N; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
-  p = position(t);
-  p_next = position(t + step);
-  fetch(t, p);
+  fetch(t, position(t));
+  int p_next = position(t + step);
   while (true) {
     // this token's rows and rotation, then its successor's take their place
     raw y1 = x1, y2 = x2;
@@ -121,6 +130,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
     const int64_t to = slot;
     const int tn = t + step;
     if (tn < a.T) {
+      src += step * src_ts;
       fetch(tn, p_next);
       p_next = position(tn + step);
     }
@@ -131,10 +141,10 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) sum += f1[i] * f1[i] + f2[i] * f2[i];
-      if (!on) sum = 0.f;   // (lanes without a chunk of the row)
+      if (CH < LPR && c >= CH) sum = 0.f;   // (lanes without a chunk of the row)
 #pragma unroll
       for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-      const float inv = wp ? 1.0f / sqrtf(sum / (float)HD + a.eps) : 1.f;
+      const float inv = normed ? rsqrt_of(sum * (1.f / HD) + a.eps) : 1.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         f1[i] *= inv * w[i];
@@ -152,7 +162,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
     }
     const bool kept = !paged || (to >= 0 && to < a.n_slots);
     if (on && kept) {
-      T* d = dst + (paged ? (to >> a.page_log2) * a.page_stride + (to & (((int64_t)1 << a.page_log2) - 1)) * dst_ts : t * dst_ts);
+      T* d = dst + (paged ? (to >> a.page_log2) * a.page_stride + (to & (((int64_t)1 << a.page_log2) - 1)) * dst_ts : 0);
       if constexpr (PAST) {
         __builtin_nontemporal_store(y1, (raw*)d);
         __builtin_nontemporal_store(y2, (raw*)(d + HALF));
@@ -162,6 +172,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
       }
     }
     if (tn >= a.T) return;
+    if (!paged) dst += step * dst_ts;
     t = tn;
   }
 }
@@ -201,14 +212,19 @@ static int launch_head_rows(RowsArgs& a, int dtype, int HD, hipStream_t st) {
   DARK_TRY(check_stream_device(st));
   const int ch = HD / 2 / (dtype == DARK_BF16 ? 8 : 4), rpp = 64 / (ch <= 4 ? 4 : ch <= 8 ? 8 : 16);
   a.n_pass = cdiv(a.h_end[2], rpp);
-  // 256 CUs x 32 waves walk over the tokens
-  const int most = cdiv(8192, a.n_pass);
-  a.t_step = a.T < most ? a.T : most;
+  // Tokens a wave walks over: some 32768 waves in all, so that the card sweeps over the tokens in order (8 x up to 4096, 48 heads:
+  // 117 us; 120 with 16384 waves, 134 with 8192, 157 with 4096), but two at least where there are enough and weights to fetch
+  // first (512 x 46: 36.9 us, 39.6 with one or two)
+  const bool norm = a.w[0] || a.w[1];
+  const int64_t units = (int64_t)a.T * a.n_pass;
+  int64_t walk = norm && units >= 16384 ? 2 : 1;
+  if (walk < (units + 16384) / 32768) walk = (units + 16384) / 32768;
+  a.t_step = (int)((a.T + walk - 1) / walk);
   // rows that the 256 MB behind the L2s cannot hold for their reader are written past them (16383 tokens x 40 fp32 heads of
-  // 128, 0.7 GB moved: 129 us, 139 without; 512 x 46 x 16 bf16 heads of 96: 30.6 and 29.2, but then they are there to be read)
+  // 128, 0.7 GB moved: 129 us, 139 without; 512 x 46 x 16 bf16 heads of 96, 72 MB: 38.7 and 40.5, but then they are there to
+  // be read)
   const bool past = (int64_t)a.T * a.h_end[2] * HD * (dtype == DARK_BF16 ? 2 : 4) > (int64_t)256 << 20;
   const dim3 grid((unsigned)cdiv(a.t_step * a.n_pass, 4)), block(256);
-  const bool norm = a.w[0] || a.w[1];
 #define DARK_ROWS(T, HDv)                                                                                  \
   do {                                                                                                     \
     if (norm && past) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true, true>), grid, block, 0, st, a);   \

@@ -52,7 +52,7 @@ struct PagedArgs {
   int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride, page_stride, slot_stride, head_stride;
   int32_t T, H, Hk, G, B, width, n_pages, page_log2, unit, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
   Div by_hk, by_tiles, by_split, by_group, by_inner, by_heads, by_rows;   // by_rows: max_q * n_heads
-  float scale_log2;            // scale * log2(e)
+  float scale_log2, q_factor;  // scale * log2(e); row tiles: its absolute value (1 for a scale of 0), what q is multiplied by
 };
 
 // Workgroups are handed to the eight XCDs, each with an L2 of its own, in turn.  `n_inner` units that follow each other and
@@ -715,6 +715,13 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   bf16x8 qb[HD / 16];
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) qb[i] = *(const bf16x8*)(qrow + i * 16 + h * 8);
+  // below, a larger product is a larger score: a scale that is not positive goes over to the queries (-1 and 0 times a bf16 are exact)
+  if (a.q_factor != 1.f) {
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qb[i][e] = (bf16_t)((float)qb[i][e] * a.q_factor);
+  }
 
   const int32_t* tab = a.table + b * a.table_stride;
   const uint8_t* km = a.kmask ? a.kmask + b * a.mask_stride : nullptr;
@@ -1093,6 +1100,11 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   const int64_t cap = (int64_t)p->table_width * p->kv.page_size;
   a.cap = (int)(cap < p->max_kv ? cap : p->max_kv);
   a.scale_log2 = p->scale * 1.44269504088896340736f;
+  a.q_factor = 1.f;
+  if (!s.few && !(a.scale_log2 > 0.f)) {
+    a.q_factor = a.scale_log2 < 0.f ? -1.f : 0.f;
+    a.scale_log2 = a.scale_log2 < 0.f ? -a.scale_log2 : 1.f;
+  }
   const int64_t wgs = (int64_t)s.n_tiles * p->kv.n_kv_heads * p->n_seqs * s.n_split;
   DARK_CHECK_ARG(wgs < (1ll << 30), "%s: %lld workgroups", who, (long long)wgs);
   a.n_units = (int)wgs;

@@ -91,7 +91,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``block_table[b]`` (int32, an entry outside the cache leaves its keys out).  Left out are keys whose ``key_mask[b, j]``
     (uint8 or bool) is 0 and, with ``causal``, keys behind the token's own place ``q_index[t]`` (int32; default: the
     sequence's last places).  A token with no key left gets zeros (lse -inf).  ``max_q`` / ``max_kv``: the most new tokens /
-    keys of a sequence.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out``, or ``(out, lse [T, n_heads] fp32)``."""
+    keys of a sequence.  Tokens that belong to no sequence are not written.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out``, or ``(out, lse [T, n_heads] fp32)``."""
     return (_bind or _ops()).paged_attention(_stream(q), q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_kv, q_index,
                                             key_mask, causal, scale, out, return_lse)
 
@@ -142,9 +142,11 @@ class PagedKVCache:
 
     def slots(self, block_table: torch.Tensor, seq: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
         """Slot (int64) of token ``index[t]`` of sequence ``seq[t]``; -1 where the table names no page for it."""
-        at = torch.div(index, self.page_size, rounding_mode="floor").long()
-        inside = (at >= 0) & (at < block_table.shape[1])
-        page = block_table[seq.long(), at.clamp(0, block_table.shape[1] - 1)].long()
+        if block_table.numel() == 0:
+            return torch.full(index.shape, -1, dtype=torch.int64, device=index.device)
+        at, b = torch.div(index, self.page_size, rounding_mode="floor").long(), seq.long()
+        inside = (at >= 0) & (at < block_table.shape[1]) & (b >= 0) & (b < block_table.shape[0])
+        page = block_table[b.clamp(0, block_table.shape[0] - 1), at.clamp(0, block_table.shape[1] - 1)].long()
         return torch.where(inside & (page >= 0) & (page < self.n_pages), page * self.page_size + index % self.page_size, -1)
 
     def _fields(self):

@@ -316,6 +316,19 @@ def test_tables_wider_than_the_caches_hold(q_lens, kv_lens, H, Hk, D, page, caus
     assert torch.equal(run_paged(p, causal=causal), out)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("q_lens,kv_lens,H,Hk,D", [([150, 9], [200, 41], 4, 2, 96), ([3, 1], [70, 400], 8, 2, 128)])
+def test_scales_that_are_not_positive(dtype, scale, q_lens, kv_lens, H, Hk, D):
+    """The smallest product becomes the largest score; all keys that are seen count alike.  Left-out keys stay out."""
+    p = paged(q_lens, kv_lens, H, Hk, D, 16, dtype, seed=3)
+    mask = torch.rand(2, 400, generator=torch.Generator().manual_seed(1)) > 0.3
+    for causal in (False, True):
+        kw = dict(scale=scale, key_mask=mask, causal=causal)
+        out, lse = run_paged(p, return_lse=True, **kw)
+        check_attention(out, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], **kw), max(kv_lens), D, dtype, lse)
+
+
 def test_views_strides_and_scores_far_apart():
     """q and out as views of larger tensors; scores so far apart that one key takes the whole row."""
     p = paged([9, 2], [100, 50], 8, 8, 96, 16, torch.float32, seed=8)

@@ -68,7 +68,8 @@ def test_kv_append_refuses(kw, msg):
 @pytest.mark.parametrize("kw,msg", [(dict(n_heads=9), "multiple"), (dict(kv=_kv(head_dim=32)), "head_dim"), (dict(q=None), "null pointer"),
                                     (dict(block_table=None), "null pointer"), (dict(max_kv=-1), "negative"), (dict(scale=math.inf), "scale"),
                                     (dict(o_ts=4), "16 bytes"), (dict(table_stride=1), "table_stride"), (dict(table_width=1 << 28), "2^30"),
-                                    (dict(max_kv=100000), "workspace")])
+                                    (dict(max_kv=100000), "workspace"),
+                                    (dict(max_q=64, kv=_kv(page_stride=8 * ((1 << 27) + 1), n_pages=64)), "spans more")])
 def test_paged_attention_refuses(kw, msg):
     f = dict(kv=_kv(), q=4096, out=8192, block_table=4096, cu_q=4096, kv_len=4096, q_ts=768, q_hs=96, o_ts=768, o_hs=96,
              table_stride=4, n_tokens=3, n_heads=8, n_seqs=2, table_width=4, max_q=2, max_kv=64, scale=0.1)
@@ -142,6 +143,8 @@ def test_pages_and_slots():
     table = torch.tensor([[5, -1], [2, 9]], dtype=torch.int32)
     seq, index = torch.tensor([0, 0, 0, 1, 1, 1, 1]), torch.tensor([0, 15, 16, 3, 17, 32, -1], dtype=torch.int32)
     assert c.slots(table, seq, index).tolist() == [80, 95, -1, 35, -1, -1, -1]
+    assert c.slots(table, torch.tensor([2, -1, 1]), torch.tensor([0, 0, 0])).tolist() == [-1, -1, 32]    # no such sequence
+    assert c.slots(table[:, :0], seq, index).tolist() == [-1] * 7 and c.slots(table[:0], seq, index).tolist() == [-1] * 7
     with pytest.raises(ValueError, match="power of two"):
         kv_cache.PagedKVCache(1, 1, 24, 1, 64, torch.float32, "cpu")
 

@@ -142,6 +142,47 @@ def test_long_windows_in_chunks(dtype, causal):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_single_tokens(dtype):
+    """One step of single tokens captured once and replayed along two sequences (ids, places and lengths written into the
+    captured tensors), with eager steps on a cache of their own in between: the same bits."""
+    cfg = config()
+    m, _ = build(cfg, dtype)
+    g = torch.Generator().manual_seed(3)
+    lens, room = [40, 7], 64
+    caches = [m.make_cache(2 * room, page_size=16) for _ in range(2)]
+    tables = [torch.tensor([c.allocate(room) for _ in range(2)], dtype=torch.int32, device=DEV) for c in caches]
+    ids = torch.randint(7, 500, (2, room), generator=g).to(DEV)
+    seq, cu = torch.arange(2, device=DEV), i32(0, 1, 2)
+    for c, t in zip(caches, tables):
+        n = sum(lens)
+        index = torch.cat([torch.arange(x) for x in lens]).int().to(DEV)
+        m.forward_cached(c, torch.cat([ids[b, :x] for b, x in enumerate(lens)]), torch.repeat_interleave(seq, i32(*lens)), index, t,
+                         i32(0, lens[0], n), i32(*lens), max(lens), room, causal=True)
+    new, index, kv = ids[:, 0].clone(), i32(*lens), i32(*[x + 1 for x in lens])
+
+    def step(c, t):
+        return m.forward_cached(c, new, seq, index, t, cu, kv, 1, room, causal=True).logits
+
+    side = torch.cuda.Stream()      # a first step outside the capture, on places that the loop writes again
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(caches[0], tables[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[0], tables[0])
+    for i in range(6):
+        at = torch.tensor([x + i for x in lens])
+        new.copy_(ids.cpu()[torch.arange(2), at])
+        index.copy_(at.int())
+        kv.copy_(at.int() + 1)
+        graph.replay()
+        want = step(caches[1], tables[1])
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_some_positions_against_a_stale_cache(dtype):
     """kv_cache.WindowCache: a whole forward, then one for the masked positions and their left neighbours after tokens were
     committed; the other positions keep the first forward's keys and values."""

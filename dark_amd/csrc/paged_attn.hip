@@ -168,9 +168,10 @@ struct Unit {
   int seen, lo, n_parts, k_begin, k_end;       // keys the row may look at; the fewest any row may; > 1: the axis is split
   bool live;
 };
-__device__ __forceinline__ bool open_unit(const PagedArgs& a, int id, int li, Unit& u) {
+// which it is (arithmetic alone), ...
+__device__ __forceinline__ void place_unit(const PagedArgs& a, int id, Unit& u) {
   int q = a.by_tiles.divmod(id);
-  const int tile = id;               // (the tiles of a key head read the same keys, ...
+  u.row0 = id * 16;                  // (the tiles of a key head read the same keys, ...
   id = a.by_hk.divmod(q);
   u.hk = q;                          // ... the key heads of a token lie next to each other)
   u.b = a.by_split.divmod(id);
@@ -179,13 +180,16 @@ __device__ __forceinline__ bool open_unit(const PagedArgs& a, int id, int li, Un
   int shift = (int)(((uint32_t)u.b * 0x9E3779B1u) >> 16);
   a.by_split.divmod(shift);
   u.split = id + shift - (id + shift >= a.n_split ? a.n_split : 0);
+  u.k_begin = u.split * a.split_keys;
+}
+// ... and what it holds
+__device__ __forceinline__ bool open_unit(const PagedArgs& a, int li, Unit& u) {
   int t0 = a.cu_q[u.b], t1 = a.cu_q[u.b + 1];
   const int len = seq_len(a, u.b);
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
   t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
   u.t0 = t0;
   u.rows = (t1 - t0) * a.G;
-  u.row0 = tile * 16;
   if (u.row0 >= u.rows) return false;
   const int row = u.row0 + li;
   u.live = row < u.rows;
@@ -216,7 +220,6 @@ __device__ __forceinline__ bool open_unit(const PagedArgs& a, int id, int li, Un
     }
   }
   u.n_parts = len <= a.split_keys ? 1 : 2;   // (one, or more)
-  u.k_begin = u.split * a.split_keys;
   if (u.split > 0 && u.k_begin >= len) return false;
   u.k_end = min(hi, u.split == a.n_split - 1 ? hi : u.k_begin + a.split_keys);
   return true;
@@ -279,30 +282,33 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
   if (WPP == 1) id = id * NW + wave;
   if (id < 0 || id >= a.n_units) return;
   Unit u;
-  if (!open_unit(a, id, li, u)) return;
-  const int k_begin = u.k_begin, k_end = u.k_end, seen = u.seen, lo = u.lo;
+  place_unit(a, id, u);
+  const int32_t* tab = a.table + u.b * a.table_stride;
+  const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
+  // pages and masks of this lane's two keys of a tile as they stand in memory: looked at two tiles ahead and made sense of
+  // one tile ahead, so that nothing waits for them -- the first even before the sequence's length is known, within the table
+  int rp[2] = {-1, -1}, rm[2] = {1, 1};
+  auto look = [&](int k0) {
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      const int key = min(k0 + jt * 16 + li, a.cap - 1);
+      rp[jt] = tab[key >> a.page_log2];
+      if (km) rm[jt] = km[key];
+    }
+  };
+  const int first = u.k_begin + (WPP == 1 ? 0 : wave * PT_KEYS);
+  if (a.cap > 0) look(first);
+  if (!open_unit(a, li, u)) return;
+  const int k_end = u.k_end, seen = u.seen, lo = u.lo;
 
   const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)u.tok * a.q_ts + u.hq * a.q_hs;
   bf16x8 qb[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) qb[i] = *(const bf16x8*)(qrow + i * 32 + g * 8);
 
-  const int32_t* tab = a.table + u.b * a.table_stride;
-  const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
   const bf16_t* kbase = (const bf16_t*)a.k + (int64_t)u.hk * a.head_stride;
   const bf16_t* vbase = (const bf16_t*)a.v + (int64_t)u.hk * a.head_stride;
   const int pmask = (1 << a.page_log2) - 1;
-  // pages and masks of this lane's two keys of a tile as they stand in memory: looked at two tiles ahead and made sense of
-  // one tile ahead, so that nothing waits for them
-  int rp[2] = {-1, -1}, rm[2] = {1, 1};
-  auto look = [&](int k0) {
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt) {
-      const int key = min(k0 + jt * 16 + li, k_end - 1);
-      rp[jt] = tab[key >> a.page_log2];
-      if (km) rm[jt] = km[key];
-    }
-  };
   // page of a key, -1 where it is left out
   auto place = [&](int k0, int (&pg)[2]) {
 #pragma unroll
@@ -348,11 +354,10 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
   // One turn of the loop brings tile t + 1 in and works on tile t; the first only brings (the code of both is there once:
   // short kernels are fetched as they run).
   const int step = WPP * PT_KEYS;
-  int k0 = k_begin + (WPP == 1 ? 0 : wave * PT_KEYS) - step;
+  int k0 = first - step;
   int pg[2] = {-1, -1}, pn[2];
   bf16x8 kr[NL], vr[NL];
   int64_t off[NL];
-  if (k0 + step < k_end) look(k0 + step);
   for (bool work = false; k0 < k_end; k0 += step, work = true) {
     if (k0 + step >= k_end && !work) break;
     place(k0 + step, pn);
@@ -481,24 +486,27 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
   if (WPP == 1) id = id * 4 + wave;
   if (id < 0 || id >= a.n_units) return;
   Unit u;
-  if (!open_unit(a, id, li, u)) return;
-  const int k_begin = u.k_begin, k_end = u.k_end, seen = u.seen, lo = u.lo;
+  place_unit(a, id, u);
+  const int32_t* tab = a.table + u.b * a.table_stride;
+  const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
+  int rp = -1, rm = 1;   // page and mask of key k0 + li as they stand in memory
+  auto look = [&](int k0) {
+    const int key = min(k0 + li, a.cap - 1);
+    rp = tab[key >> a.page_log2];
+    if (km) rm = km[key];
+  };
+  const int first = u.k_begin + (WPP == 1 ? 0 : wave * KEYS);
+  if (a.cap > 0) look(first);
+  if (!open_unit(a, li, u)) return;
+  const int k_end = u.k_end, seen = u.seen, lo = u.lo;
 
   const float* qrow = (const float*)a.q + (int64_t)u.tok * a.q_ts + u.hq * a.q_hs + g * 4;
   f32x4 qf[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) qf[i] = *(const f32x4*)(qrow + 16 * i);
-  const int32_t* tab = a.table + u.b * a.table_stride;
-  const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
   const float* kbase = (const float*)a.k + (int64_t)u.hk * a.head_stride;
   const float* vbase = (const float*)a.v + (int64_t)u.hk * a.head_stride;
   const int pmask = (1 << a.page_log2) - 1;
-  int rp = -1, rm = 1;   // page and mask of key k0 + li as they stand in memory
-  auto look = [&](int k0) {
-    const int key = min(k0 + li, k_end - 1);
-    rp = tab[key >> a.page_log2];
-    if (km) rm = km[key];
-  };
   // where key k0 + li lies, in elements from its head's first; -1: left out, read as zeros
   auto place = [&](int k0) -> int64_t {
     const bool on = k0 + li < k_end && rp >= 0 && rp < a.n_pages && rm != 0;
@@ -532,9 +540,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
   float m = -INFINITY, l = 0.f;
   // (one turn brings tile t + 1 in and works on tile t, as above)
   const int step = WPP * KEYS;
-  int k0 = k_begin + (WPP == 1 ? 0 : wave * KEYS) - step;
+  int k0 = first - step;
   int64_t pg = -1, pn;
-  if (k0 + step < k_end) look(k0 + step);
   for (bool work = false; k0 < k_end; k0 += step, work = true) {
     if (k0 + step >= k_end && !work) break;
     pn = place(k0 + step);
@@ -993,7 +1000,7 @@ struct PagedPlan {
 
 // The row tiles' kernel hands a key's place from lane to lane as 32 bits: in units of the largest power of two that divides
 // the cache's strides (256 bytes for one head of 128 bf16, a cache of 1 TiB then).
-static int place_unit(const dark_paged_kv& kv) {
+static int place_step(const dark_paged_kv& kv) {
   const uint64_t strides = (uint64_t)kv.page_stride | (uint64_t)kv.slot_stride | 1ull << 20;
   return __builtin_ctzll(strides);
 }
@@ -1078,7 +1085,7 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   DARK_CHECK_ARG(p->table_stride >= p->table_width || p->n_seqs == 1, "%s: table_stride %lld < table_width %d", who, (long long)p->table_stride, p->table_width);
   hipStream_t st = (hipStream_t)stream;
   const PagedPlan s = plan_paged(p);
-  const int unit = place_unit(p->kv);
+  const int unit = place_step(p->kv);
   DARK_CHECK_ARG(s.few || (double)p->kv.page_stride * (p->kv.n_pages > 0 ? p->kv.n_pages - 1 : 0) +
                               (double)p->kv.slot_stride * (p->kv.page_size - 1) < 4294967295.0 * (double)(1ll << unit),
                  "%s: the cache spans more than 2^32 times the power of two in its strides (%lld elements)", who, 1ll << unit);

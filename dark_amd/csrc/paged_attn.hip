@@ -667,7 +667,7 @@ template <int HD> struct TileSwz {
 
 constexpr int TT_ROWS = 128, TT_KEYS = 64;
 
-template <int HD, bool ODD>
+template <int HD, bool ODD, bool NT>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   typedef TileSwz<HD> Z;
   typedef __attribute__((address_space(3))) void lds_void;
@@ -759,8 +759,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
       const char* kp = (on ? kbase + ((uint64_t)o << (a.unit + 1)) : zr) + Z::k_chunk(r, pos) * 16;
       const char* vp = (on ? vbase + ((uint64_t)o << (a.unit + 1)) : zr) + Z::v_pos(r, pos) * 16;
       char* to = smem + buf * (2 * TILE) + (n * 4 + wave) * 1024;
-      __builtin_amdgcn_global_load_lds((gl_void*)kp, (lds_void*)to, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gl_void*)vp, (lds_void*)(to + TILE), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gl_void*)kp, (lds_void*)to, 16, 0, NT ? 2 : 0);   // (2: nt, past the caches)
+      __builtin_amdgcn_global_load_lds((gl_void*)vp, (lds_void*)(to + TILE), 16, 0, NT ? 2 : 0);
     }
   };
 
@@ -1011,7 +1011,8 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   const int64_t heads = (int64_t)p->kv.n_kv_heads * p->n_seqs;
   s.few = 0;
   if (p->kv.dtype == DARK_F32) s.few = p->max_kv <= 128 ? 1 : 4;
-  else if (rows <= 16) {
+  else if (rows <= 16 || (rows <= 48 && p->max_kv <= 128)) {   // (512 x 46 over 46, 8 heads of 96: 41.9 us, 45.6 by row tiles;
+                                                               // 64 x 8 over 2000, 32 rows: 160 and 98.5 the other way)
     // Waves a problem: one where keys are few, eight where CUs are left over and the axis is short (16 x 1 over 900, 8 heads of
     // 128: 14.6 us, 17.7 with four; over 1900: 29.3, 24.2 with four and a join; 12 heads of 64 over 1900: 15.2 and 24.0;
     // 256 problems: 18.7 and 18.2)
@@ -1149,9 +1150,14 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
     else if (s.few == 8) hipLaunchKernelGGL((paged_few_kernel<HDv, 8, ODD, false>), grid, block, 0, st, a); \
     else {                                                                                          \
       constexpr int lds = 4 * TT_KEYS * HDv * 2;                                                    \
-      static SmemOptIn optin;                                                                       \
-      DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv, ODD>, lds, st));                    \
-      hipLaunchKernelGGL((paged_tile_kernel<HDv, ODD>), grid, block, lds, st, a);                   \
+      static SmemOptIn optin, optin_nt;                                                             \
+      if (past && s.n_tiles == 1) {                                                                 \
+        DARK_TRY(optin_nt.ensure((const void*)paged_tile_kernel<HDv, ODD, HDv % 64 == 0>, lds, st)); \
+        hipLaunchKernelGGL((paged_tile_kernel<HDv, ODD, HDv % 64 == 0>), grid, block, lds, st, a);  \
+      } else {                                                                                      \
+        DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv, ODD, false>, lds, st));           \
+        hipLaunchKernelGGL((paged_tile_kernel<HDv, ODD, false>), grid, block, lds, st, a);          \
+      }                                                                                             \
     }                                                                                               \
     DARK_JOIN(bf16_t, HDv);                                                                         \
   } while (0)
@@ -1164,7 +1170,7 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   const int HD = p->kv.head_dim;
   // NT: keys that, with four layers of them, cannot stay in the 256 MB behind the L2s until they are read again go past the caches (64 x 1 over up
   // to 16384, 2.5 GB: 399 us, 435 without; head_dim 64: 207 and 234; 113 MB among other layers': 29.3 and 32.2, again and
-  // again: 27.0 and 26.0) -- if their rows are whole 128-byte lines: a line that two rows share is then read twice (head_dim 96:
+  // again: 27.0 and 26.0; 64 x 8 over 2000, one tile of rows: 88.5 us, 98.5 without) -- if their rows are whole 128-byte lines: a line that two rows share is then read twice (head_dim 96:
   // 365 and 331)
   const bool past = HD % 64 == 0 && (int64_t)p->n_seqs * a.cap * p->kv.n_kv_heads * HD * es * 2 > (int64_t)64 << 20;
   // rows of one tile see different keys only where a token's own place bounds them and a tile holds several tokens

@@ -213,6 +213,7 @@ SHAPES = [  # q_lens, kv_lens, H, Hk, D, page
     ([150], [400], 6, 3, 64, 1),                                  # pages of one slot
     ([3, 2], [40, 9], 28, 4, 128, 8),
     ([129, 257], [129, 700], 2, 2, 96, 16),
+    ([46, 30], [46, 100], 8, 8, 96, 16),                          # whole windows of a denoise step
 ]
 
 
@@ -303,7 +304,8 @@ def test_long_key_axis(dtype, q_lens, kv_lens, H, Hk, D, page, causal):
 
 
 @pytest.mark.parametrize("q_lens,kv_lens,H,Hk,D,page", [([1, 1, 4], [3001, 1, 700], 8, 2, 128, 64), ([1, 0, 2], [5000, 3, 0], 8, 4, 96, 16),
-                                                       ([1, 3], [2111, 65], 4, 4, 64, 16)])
+                                                       ([1, 3], [2111, 65], 4, 4, 64, 16), ([9, 31], [3000, 40], 8, 2, 128, 16),
+                                                       ([20, 1], [300, 2000], 4, 4, 64, 32)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_tables_wider_than_the_caches_hold(q_lens, kv_lens, H, Hk, D, page, causal):
     """Tables with room for over 256 MB of keys (their rows are then read past the caches), of which the sequences have a few."""

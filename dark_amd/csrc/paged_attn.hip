@@ -162,16 +162,17 @@ __device__ __forceinline__ V load_global(const V* p) {
   return NT ? __builtin_nontemporal_load((global_v*)p) : *(global_v*)p;
 }
 
-// ---- what a wave of the streaming kernels works on: 16 rows of one key head against a part of its sequence's keys
-struct Unit {
-  int b, hk, split, t0, row0, rows, tok, hq;   // row0: first of the 16; tok, hq: this lane's row (lane & 15)
-  int seen, lo, n_parts, k_begin, k_end;       // keys the row may look at; the fewest any row may; > 1: the axis is split
-  bool live;
+// ---- what a wave of the streaming kernels works on: RT times 16 rows of one key head against a part of its sequence's keys
+template <int RT> struct Unit {
+  int b, hk, split, t0, row0, rows, lo, n_parts, k_begin, k_end;   // row0: its first; lo: the fewest keys any row may look at
+  int tok[RT], hq[RT], seen[RT];                                   // this lane's rows (16 t + (lane & 15)); keys they may look at
+  bool live[RT];
 };
 // which it is (arithmetic alone), ...
-__device__ __forceinline__ void place_unit(const PagedArgs& a, int id, Unit& u) {
+template <int RT>
+__device__ __forceinline__ void place_unit(const PagedArgs& a, int id, Unit<RT>& u) {
   int q = a.by_tiles.divmod(id);
-  u.row0 = id * 16;                  // (the tiles of a key head read the same keys, ...
+  u.row0 = id * 16 * RT;             // (the tiles of a key head read the same keys, ...
   id = a.by_hk.divmod(q);
   u.hk = q;                          // ... the key heads of a token lie next to each other)
   u.b = a.by_split.divmod(id);
@@ -183,7 +184,8 @@ __device__ __forceinline__ void place_unit(const PagedArgs& a, int id, Unit& u) 
   u.k_begin = u.split * a.split_keys;
 }
 // ... and what it holds
-__device__ __forceinline__ bool open_unit(const PagedArgs& a, int li, Unit& u) {
+template <int RT>
+__device__ __forceinline__ bool open_unit(const PagedArgs& a, int li, Unit<RT>& u) {
   int t0 = a.cu_q[u.b], t1 = a.cu_q[u.b + 1];
   const int len = seq_len(a, u.b);
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
@@ -191,33 +193,41 @@ __device__ __forceinline__ bool open_unit(const PagedArgs& a, int li, Unit& u) {
   u.t0 = t0;
   u.rows = (t1 - t0) * a.G;
   if (u.row0 >= u.rows) return false;
-  const int row = u.row0 + li;
-  u.live = row < u.rows;
-  const int rr = u.live ? row : u.row0, ri = a.by_group.div(rr);
-  u.tok = t0 + ri;
-  u.hq = u.hk * a.G + rr - ri * a.G;
-  u.seen = u.live ? len : 0;
+  const int n = t1 - t0;
+  auto clip = [&](int64_t last) { return last + 1 < len ? (last + 1 < 0 ? 0 : (int)(last + 1)) : len; };
   int hi = len;
   u.lo = len;
-  if (a.causal) {
-    auto clip = [&](int64_t last) { return last + 1 < len ? (last + 1 < 0 ? 0 : (int)(last + 1)) : len; };
-    if (a.q_index) {
-      u.seen = u.live ? clip(a.q_index[u.tok]) : 0;
-      hi = u.seen;
-      u.lo = u.live ? u.seen : 0x7fffffff;
+  if (a.causal && !a.q_index) {   // the sequence's last places: rows see more and more
+    u.lo = clip((int64_t)len - n + a.by_group.div(u.row0));
+    hi = clip((int64_t)len - n + a.by_group.div(min(u.row0 + 16 * RT, u.rows) - 1));
+  } else if (a.causal) {
+    hi = 0;
+    u.lo = 0x7fffffff;
+  }
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) {
-        hi = max(hi, __shfl_xor(hi, o, 64));
-        u.lo = min(u.lo, __shfl_xor(u.lo, o, 64));
-      }
-      hi = __builtin_amdgcn_readfirstlane(hi);
-      u.lo = __builtin_amdgcn_readfirstlane(u.lo);
-    } else {   // the sequence's last places: rows see more and more
-      const int n = t1 - t0, last_row = min(u.row0 + 15, u.rows - 1);
-      if (u.live) u.seen = clip((int64_t)len - n + ri);
-      u.lo = clip((int64_t)len - n + a.by_group.div(u.row0));
-      hi = clip((int64_t)len - n + a.by_group.div(last_row));
+  for (int t = 0; t < RT; ++t) {
+    const int row = u.row0 + 16 * t + li;
+    u.live[t] = row < u.rows;
+    const int rr = u.live[t] ? row : u.row0, ri = a.by_group.div(rr);
+    u.tok[t] = t0 + ri;
+    u.hq[t] = u.hk * a.G + rr - ri * a.G;
+    u.seen[t] = u.live[t] ? len : 0;
+    if (a.causal && a.q_index) {
+      u.seen[t] = u.live[t] ? clip(a.q_index[u.tok[t]]) : 0;
+      hi = max(hi, u.seen[t]);
+      u.lo = min(u.lo, u.live[t] ? u.seen[t] : 0x7fffffff);
+    } else if (a.causal && u.live[t]) {
+      u.seen[t] = clip((int64_t)len - n + ri);
     }
+  }
+  if (a.causal && a.q_index) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      hi = max(hi, __shfl_xor(hi, o, 64));
+      u.lo = min(u.lo, __shfl_xor(u.lo, o, 64));
+    }
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    u.lo = __builtin_amdgcn_readfirstlane(u.lo);
   }
   u.n_parts = len <= a.split_keys ? 1 : 2;   // (one, or more)
   if (u.split > 0 && u.k_begin >= len) return false;
@@ -227,10 +237,10 @@ __device__ __forceinline__ bool open_unit(const PagedArgs& a, int li, Unit& u) {
 
 // ---- joins the WPP waves of a workgroup, whose (O [16][HD], m [16], l [16]) lie where `of(wave)` says: wave w of the first
 // four the rows 4 w .. 4 w + 3, a lane four columns of each 64
-template <typename T, int HD, int WPP, typename Of>
-__device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit& u, bool parts, int wave, int lane, Of of) {
+template <typename T, int HD, int WPP, int RT, typename Of>
+__device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit<RT>& u, int row0, bool parts, int wave, int lane, Of of) {
   const int li = lane & 15, r = wave * 4 + (lane >> 4);
-  if (wave >= 4 || u.row0 + r >= u.rows) return;
+  if (wave >= 4 || row0 + r >= u.rows) return;
   float mm = -INFINITY;
 #pragma unroll
   for (int w = 0; w < WPP; ++w) mm = fmaxf(mm, of(w)[16 * HD + r]);
@@ -246,7 +256,7 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit& u, bo
     for (int c = 0; c < (HD + 63) / 64; ++c)
       if (c * 64 + li * 4 < HD) acc[c] += *(const f32x4*)(o + r * HD + c * 64 + li * 4) * f;
   }
-  const int ti = a.by_group.div(u.row0 + r), tk = u.t0 + ti, h = u.hk * a.G + (u.row0 + r) - ti * a.G;
+  const int ti = a.by_group.div(row0 + r), tk = u.t0 + ti, h = u.hk * a.G + (row0 + r) - ti * a.G;
   const int64_t pa = ((int64_t)u.split * a.T + tk) * a.H + h;
   const float inv = parts ? 1.f : norm_of(ll);
 #pragma unroll
@@ -281,7 +291,7 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
   int id = unit_of_block(a);
   if (WPP == 1) id = id * NW + wave;
   if (id < 0 || id >= a.n_units) return;
-  Unit u;
+  Unit<1> u;
   place_unit(a, id, u);
   const int32_t* tab = a.table + u.b * a.table_stride;
   const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
@@ -299,9 +309,9 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
   const int first = u.k_begin + (WPP == 1 ? 0 : wave * PT_KEYS);
   if (a.cap > 0) look(first);
   if (!open_unit(a, li, u)) return;
-  const int k_end = u.k_end, seen = u.seen, lo = u.lo;
+  const int k_end = u.k_end, seen = u.seen[0], lo = u.lo;
 
-  const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)u.tok * a.q_ts + u.hq * a.q_hs;
+  const bf16_t* qrow = (const bf16_t*)a.q + (int64_t)u.tok[0] * a.q_ts + u.hq[0] * a.q_hs;
   bf16x8 qb[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) qb[i] = *(const bf16x8*)(qrow + i * 32 + g * 8);
@@ -456,8 +466,8 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
   l = quad_sum(l);
   const bool parts = u.n_parts > 1 && a.n_split > 1;
   if constexpr (WPP == 1) {
-    if (!u.live) return;
-    write_row<bf16_t, HD>(a, parts, ((int64_t)u.split * a.T + u.tok) * a.H + u.hq, u.tok, u.hq, g, O, m, l);
+    if (!u.live[0]) return;
+    write_row<bf16_t, HD>(a, parts, ((int64_t)u.split * a.T + u.tok[0]) * a.H + u.hq[0], u.tok[0], u.hq[0], g, O, m, l);
   } else {
     // O [16][HD] fp32, then m and l of the 16 rows, in the wave's own LDS
     float* mine = (float*)Vs;
@@ -465,27 +475,29 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
     for (int dt = 0; dt < HD / 16; ++dt) *(f32x4*)(mine + li * HD + dt * 16 + 4 * g) = O[dt];
     if (g == 0) { mine[16 * HD + li] = m; mine[16 * HD + 16 + li] = l; }
     __syncthreads();
-    join_waves<bf16_t, HD, WPP>(a, u, parts, wave, lane, [&](int w) { return (const float*)Vall[w]; });
+    join_waves<bf16_t, HD, WPP>(a, u, u.row0, parts, wave, lane, [&](int w) { return (const float*)Vall[w]; });
   }
 }
 
 // ---- fp32: the same stream for any number of rows, 16 a workgroup, on 16 x 16 x 4 fp32 matrix instructions; nothing passes
 // through LDS.  The output's columns are dealt to the second product's rows so that a lane reads a V row's 16 bytes at
 // 64 c + 4 (lane & 15) -- 16 lanes a whole row piece -- and its four (HD 96: the last two) floats go to four instructions.
-// 16 sequences of 9 to 128 new tokens over 31 to 512 keys, 12 heads of 64: 23.4 us, 29 TFLOP/s; the SIMDs that get the long
-// sequences' rows work twice as long as the average.  (Eight waves a problem: 28.5 us; one: 47.)
-template <int HD, int WPP, bool ODD>
+// 16 sequences of 9 to 128 new tokens over 31 to 512 keys, 12 heads of 64: 23.4 - 25 us, 29 TFLOP/s; the SIMDs that get the
+// long sequences' rows work twice as long as the average.  (Eight waves a problem: 28.5 us; one: 47.)  Long chunks (4 x 1024
+// over 9216, head_dim 128) 104 TFLOP/s of the 152 that a large fp32 product reaches: the softmax's vector instructions and the
+// matrix instructions of two or three waves overlap only in part.
+template <int HD, int WPP, int RT, bool ODD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const PagedArgs a) {
   constexpr int NC = HD / 16, KEYS = 16, NV = (HD + 63) / 64;   // NV: pieces of a V row a lane reads
   constexpr int E1 = HD == 96 ? 2 : 4;                                                      // floats of the second one
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  __shared__ __attribute__((aligned(16))) float Oall[WPP == 1 ? 1 : 4][WPP == 1 ? 4 : 16 * HD + 32];
+  __shared__ __attribute__((aligned(16))) float Oall[WPP == 1 ? 1 : 4][RT][WPP == 1 ? 4 : 16 * HD + 32];
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int id = unit_of_block(a);
   if (WPP == 1) id = id * 4 + wave;
   if (id < 0 || id >= a.n_units) return;
-  Unit u;
+  Unit<RT> u;
   place_unit(a, id, u);
   const int32_t* tab = a.table + u.b * a.table_stride;
   const uint8_t* km = a.kmask ? a.kmask + u.b * a.mask_stride : nullptr;
@@ -498,12 +510,15 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
   const int first = u.k_begin + (WPP == 1 ? 0 : wave * KEYS);
   if (a.cap > 0) look(first);
   if (!open_unit(a, li, u)) return;
-  const int k_end = u.k_end, seen = u.seen, lo = u.lo;
+  const int k_end = u.k_end, lo = u.lo;
 
-  const float* qrow = (const float*)a.q + (int64_t)u.tok * a.q_ts + u.hq * a.q_hs + g * 4;
-  f32x4 qf[NC];
+  f32x4 qf[RT][NC];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) qf[i] = *(const f32x4*)(qrow + 16 * i);
+  for (int t = 0; t < RT; ++t) {
+    const float* qrow = (const float*)a.q + (int64_t)u.tok[t] * a.q_ts + u.hq[t] * a.q_hs + g * 4;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) qf[t][i] = *(const f32x4*)(qrow + 16 * i);
+  }
   const float* kbase = (const float*)a.k + (int64_t)u.hk * a.head_stride;
   const float* vbase = (const float*)a.v + (int64_t)u.hk * a.head_stride;
   const int pmask = (1 << a.page_log2) - 1;
@@ -534,10 +549,14 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
     }
   };
 
-  f32x4 O[NC];   // [4 c + e]: column 64 c + 4 (4 g + r) + e (HD 96, c = 1: 64 + 2 (4 g + r) + e) in element r
+  f32x4 O[RT][NC];   // [4 c + e]: column 64 c + 4 (4 g + r) + e (HD 96, c = 1: 64 + 2 (4 g + r) + e) in element r
 #pragma unroll
-  for (int i = 0; i < NC; ++i) O[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int i = 0; i < NC; ++i) O[t][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m[RT], l[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) { m[t] = -INFINITY; l[t] = 0.f; }
   // (one turn brings tile t + 1 in and works on tile t, as above)
   const int step = WPP * KEYS;
   int k0 = first - step;
@@ -546,42 +565,50 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
     if (k0 + step >= k_end && !work) break;
     pn = place(k0 + step);
     if (k0 + 2 * step < k_end) look(k0 + 2 * step);
-    f32x4 S = {0.f, 0.f, 0.f, 0.f};
-    if (work) {
-      f32x4 S2 = {0.f, 0.f, 0.f, 0.f};
+    f32x4 S[RT];
+    if (work) {   // two sums a row tile: an instruction does not wait for the one before it
+      f32x4 S2[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) S[t] = S2[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          S = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][e], qf[i][e], S, 0, 0, 0);
-          S2 = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][e + 1], qf[i][e + 1], S2, 0, 0, 0);
-        }
-      S += S2;
+        for (int e = 0; e < 4; e += 2)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][e], qf[t][i][e], S[t], 0, 0, 0);
+            S2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[i][e + 1], qf[t][i][e + 1], S2[t], 0, 0, 0);
+          }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) S[t] += S2[t];
     }
     fetch_k(pn);
     if (work) {
-      float mx = -INFINITY;
       const unsigned on = (unsigned)__ballot(pg >= 0) >> (4 * g);   // (lanes 0..15 hold the 16 keys)
-      const int room = seen - (k0 + 4 * g);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        S[r] = ((on >> r) & 1) && r < room ? S[r] * a.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, S[r]);
-      }
-      mx = quad_max(mx);
-      if (__any(mx > m + kSlack)) {
-        const float mn = fmaxf(m, mx);
-        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-        m = mn;
-        l *= alpha;
+      for (int t = 0; t < RT; ++t) {
+        float mx = -INFINITY;
+        const int room = u.seen[t] - (k0 + 4 * g);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) O[i] *= alpha;
-      }
-      const float mz = m == -INFINITY ? 0.f : m;   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
+        for (int r = 0; r < 4; ++r) {
+          S[t][r] = ((on >> r) & 1) && r < room ? S[t][r] * a.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, S[t][r]);
+        }
+        mx = quad_max(mx);
+        if (__any(mx > m[t] + kSlack)) {
+          const float mn = fmaxf(m[t], mx);
+          const float alpha = __builtin_amdgcn_exp2f(m[t] - (mn == -INFINITY ? 0.f : mn));
+          m[t] = mn;
+          l[t] *= alpha;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        S[r] = __builtin_amdgcn_exp2f(S[r] - mz);
-        l += S[r];   // (this lane's keys only: the four lanes of a row are added up at the end)
+          for (int i = 0; i < NC; ++i) O[t][i] *= alpha;
+        }
+        const float mz = m[t] == -INFINITY ? 0.f : m[t];   // nothing seen yet: 2^(-inf - 0) = 0 everywhere
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          S[t][r] = __builtin_amdgcn_exp2f(S[t][r] - mz);
+          l[t] += S[t][r];   // (this lane's keys only: the four lanes of a row are added up at the end)
+        }
       }
       // ---- O^T += V^T P^T
       if (ODD && k0 + KEYS > lo && lo < k_end) {
@@ -593,16 +620,19 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
         if (__any(odd)) {
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
-            f32x4 code = {0.f, 0.f, 0.f, 0.f};
+            f32x4 code[RT] = {};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float c = odd_code(i < 4 ? v0[r][i & 3] : v1[r][i & 3]);
-              code = __builtin_amdgcn_mfma_f32_16x16x4f32(c, S[r] > 0.f ? 1.f : 0.f, code, 0, 0, 0);
+#pragma unroll
+              for (int t = 0; t < RT; ++t) code[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(c, S[t][r] > 0.f ? 1.f : 0.f, code[t], 0, 0, 0);
               if (i < 4) v0[r][i & 3] = c == 0.f ? v0[r][i & 3] : 0.f;
               else v1[r][i & 3] = c == 0.f ? v1[r][i & 3] : 0.f;
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) O[i][x] = odd_apply(O[i][x], code[x]);
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) O[t][i][x] = odd_apply(O[t][i][x], code[t][x]);
           }
         }
       }
@@ -610,37 +640,49 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          O[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(i < 4 ? v0[r][i & 3] : v1[r][i & 3], S[r], O[i], 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+            O[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(i < 4 ? v0[r][i & 3] : v1[r][i & 3], S[t][r], O[t][i], 0, 0, 0);
     }
     fetch_v(pn);
     pg = pn;
   }
-  l = quad_sum(l);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) l[t] = quad_sum(l[t]);
   const bool parts = u.n_parts > 1 && a.n_split > 1;
   // four (two) neighbouring columns of this lane's row for each r
-  auto emit = [&](float* row, float inv) {
+  auto emit = [&](float* row, const f32x4 (&o)[NC], float inv) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      *(f32x4*)(row + 4 * (4 * g + r)) = (f32x4){O[0][r], O[1][r], O[2][r], O[3][r]} * inv;
-      if constexpr (E1 == 2) *(f32x2*)(row + 64 + 2 * (4 * g + r)) = (f32x2){O[4][r], O[5][r]} * inv;
-      else if constexpr (NV == 2) *(f32x4*)(row + 64 + 4 * (4 * g + r)) = (f32x4){O[NC - 4][r], O[NC - 3][r], O[NC - 2][r], O[NC - 1][r]} * inv;
+      *(f32x4*)(row + 4 * (4 * g + r)) = (f32x4){o[0][r], o[1][r], o[2][r], o[3][r]} * inv;
+      if constexpr (E1 == 2) *(f32x2*)(row + 64 + 2 * (4 * g + r)) = (f32x2){o[4][r], o[5][r]} * inv;
+      else if constexpr (NV == 2) *(f32x4*)(row + 64 + 4 * (4 * g + r)) = (f32x4){o[NC - 4][r], o[NC - 3][r], o[NC - 2][r], o[NC - 1][r]} * inv;
     }
   };
   if constexpr (WPP == 1) {
-    if (!u.live) return;
-    const int64_t at = ((int64_t)u.split * a.T + u.tok) * a.H + u.hq;
-    if (parts) {
-      emit(a.part_o + at * HD, 1.f);
-      if (g == 0) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = l; }
-    } else {
-      emit((float*)a.out + (int64_t)u.tok * a.o_ts + u.hq * a.o_hs, norm_of(l));
-      if (a.lse && g == 0) a.lse[(int64_t)u.tok * a.H + u.hq] = lse_of(m, l);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (!u.live[t]) continue;
+      const int64_t at = ((int64_t)u.split * a.T + u.tok[t]) * a.H + u.hq[t];
+      if (parts) {
+        emit(a.part_o + at * HD, O[t], 1.f);
+        if (g == 0) { a.part_ml[at * 2] = m[t]; a.part_ml[at * 2 + 1] = l[t]; }
+      } else {
+        emit((float*)a.out + (int64_t)u.tok[t] * a.o_ts + u.hq[t] * a.o_hs, O[t], norm_of(l[t]));
+        if (a.lse && g == 0) a.lse[(int64_t)u.tok[t] * a.H + u.hq[t]] = lse_of(m[t], l[t]);
+      }
     }
   } else {
-    emit(Oall[wave] + li * HD, 1.f);
-    if (g == 0) { Oall[wave][16 * HD + li] = m; Oall[wave][16 * HD + 16 + li] = l; }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      float* mine = Oall[wave][t];
+      emit(mine + li * HD, O[t], 1.f);
+      if (g == 0) { mine[16 * HD + li] = m[t]; mine[16 * HD + 16 + li] = l[t]; }
+    }
     __syncthreads();
-    join_waves<float, HD, WPP>(a, u, parts, wave, lane, [&](int w) { return (const float*)Oall[w]; });
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      join_waves<float, HD, WPP>(a, u, u.row0 + 16 * t, parts, wave, lane, [&](int w) { return (const float*)Oall[w][t]; });
   }
 }
 
@@ -993,7 +1035,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
 }
 
 struct PagedPlan {
-  int few;               // waves a problem in paged_few_kernel, 0 = tiles of rows
+  int few, rt;           // waves a problem in the streaming kernels (0: tiles of rows) and their 16-row tiles
   int n_tiles, n_split, split_keys;
   int64_t ws_o, ws_ml;   // bytes
 };
@@ -1010,7 +1052,13 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   const int64_t rows = (int64_t)p->max_q * (p->n_heads / p->kv.n_kv_heads);
   const int64_t heads = (int64_t)p->kv.n_kv_heads * p->n_seqs;
   s.few = 0;
-  if (p->kv.dtype == DARK_F32) s.few = p->max_kv <= 128 ? 1 : 4;
+  s.rt = 1;
+  if (p->kv.dtype == DARK_F32) {
+    s.few = p->max_kv <= 128 ? 1 : 4;
+    // 32 rows a wave where they are there and dims enough to be worth it (4 x 512 over 2048, 8 key heads of 128: 652 us, 840 with
+    // 16; of 96, 8 x 512 over 2048: 275 and 310; 12 heads of 64, 64 x 40 over 440: 77 and 62)
+    if (rows > 16 && s.few == 4 && p->kv.head_dim > 64) s.rt = 2;
+  }
   else if (rows <= 16 || (rows <= 48 && p->max_kv <= 128)) {   // (512 x 46 over 46, 8 heads of 96: 41.9 us, 45.6 by row tiles;
                                                                // 64 x 8 over 2000, 32 rows: 160 and 98.5 the other way)
     // Waves a problem: one where keys are few, eight where CUs are left over and the axis is short (16 x 1 over 900, 8 heads of
@@ -1019,7 +1067,7 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
     const bool wide = heads <= 192 && p->max_kv <= (p->kv.head_dim == 64 ? 2048 : 1024);
     s.few = p->max_kv <= 128 ? 1 : wide ? 8 : 4;
   }
-  const int tile_rows = s.few ? 16 : TT_ROWS;
+  const int tile_rows = s.few ? 16 * s.rt : TT_ROWS;
   s.n_tiles = (int)((rows + tile_rows - 1) / tile_rows);
   if (s.n_tiles < 1) s.n_tiles = 1;
   const int64_t wgs = (int64_t)s.n_tiles * heads;
@@ -1163,8 +1211,10 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   } while (0)
 #define DARK_PAGED_F32(HDv)                                                                         \
   do {                                                                                              \
-    if (s.few == 1) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1, ODD>), grid, block, 0, st, a);     \
-    else hipLaunchKernelGGL((paged_f32_kernel<HDv, 4, ODD>), grid, block, 0, st, a);                \
+    if (s.few == 1 && s.rt == 2) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1, 2, ODD>), grid, block, 0, st, a); \
+    else if (s.few == 1) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1, 1, ODD>), grid, block, 0, st, a); \
+    else if (s.rt == 2) hipLaunchKernelGGL((paged_f32_kernel<HDv, 4, 2, ODD>), grid, block, 0, st, a); \
+    else hipLaunchKernelGGL((paged_f32_kernel<HDv, 4, 1, ODD>), grid, block, 0, st, a);             \
     DARK_JOIN(float, HDv);                                                                          \
   } while (0)
   const int HD = p->kv.head_dim;

@@ -370,7 +370,9 @@ int dark_prof_read(double* total_ms, double* total_flops, int* launches);
  * One layer's cache: `n_pages` pages of `page_size` slots (a power of two); element (page, slot, head, i) of k and of v
  * lies at page * page_stride + slot * slot_stride + head * head_stride + i (strides in elements, the same for k and v; all
  * strides multiples of 16 bytes, k and v 16-byte aligned).  Token j of a sequence lies in slot j % page_size of the page
- * that entry j / page_size of the sequence's block table names.  Types: DARK_F32, DARK_BF16; head_dim 64, 96 or 128. */
+ * that entry j / page_size of the sequence's block table names.  Types: DARK_F32, DARK_BF16; head_dim 64, 96 or 128.
+ * dark_paged_attention in bf16 refuses chunks of more than 16 rows of a key head over a cache that spans more than 2^32
+ * times the largest power of two (at most 2^20) that divides both strides (512 GiB and more for heads of 64 elements). */
 typedef struct dark_paged_kv {
   void* k;
   void* v;

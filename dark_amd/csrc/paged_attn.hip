@@ -253,8 +253,10 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit<RT>& u
     const float f = __builtin_amdgcn_exp2f(o[16 * HD + r] - mz);
     ll += o[16 * HD + 16 + r] * f;
 #pragma unroll
-    for (int c = 0; c < (HD + 63) / 64; ++c)
-      if (c * 64 + li * 4 < HD) acc[c] += *(const f32x4*)(o + r * HD + c * 64 + li * 4) * f;
+    for (int c = 0; c < (HD + 63) / 64; ++c) {
+      const int col = c * 64 + li * 4;
+      acc[c] += *(const f32x4*)(o + r * HD + (col < HD ? col : 0)) * f;   // (read anyway: a branch a wave would wait for each in turn)
+    }
   }
   const int ti = a.by_group.div(row0 + r), tk = u.t0 + ti, h = u.hk * a.G + (row0 + r) - ti * a.G;
   const int64_t pa = ((int64_t)u.split * a.T + tk) * a.H + h;

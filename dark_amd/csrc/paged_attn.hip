@@ -1074,15 +1074,20 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   if (s.n_tiles < 1) s.n_tiles = 1;
   const int64_t wgs = (int64_t)s.n_tiles * heads;
   // Parts of a key axis.  Few problems: 512 of them fill the card once (2 x 4 over 131072, 16 problems: 166 us; 172 with 1024
-  // parts, 184 with 768, 183 with 2048).  Many, as with one token for each of many sequences: parts of 1024, because lengths
-  // differ and the longest must not finish alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with
-  // 4096), of 512 where the card would be filled twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024).  Never
-  // below 256 keys: a part's (O, m, l) is then 1/16 of the keys' bytes at most.
+  // parts, 184 with 768, 183 with 2048), 1024 where a key head has several row tiles, of which shorter sequences lack some (6 x
+  // up to 366 over up to 38700, 8 key heads: 244 us, 339 with 512; 8 x 64 over 8064, one tile: 84 and 78 the other way).  Many,
+  // as with one token for each of many sequences: parts of 1024 keys, because lengths differ and the longest must not finish
+  // alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with 4096), of 512 where the card would be filled
+  // twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024).  Never below 256 keys (a part's (O, m, l) is then 1/16 of
+  // the keys' bytes at most), none where there are no more than 512 (5 x 279 over 284: 14.5 us, 20.9 in two parts).
   int64_t keys = p->max_kv;
-  if (s.few == 0 || s.few == 4) {
-    if (wgs < 256) keys = (p->max_kv * wgs + 511) / 512;
+  if ((s.few == 0 || s.few == 4) && p->max_kv > 512) {
+    if (wgs < 256) {
+      int64_t n = ((s.n_tiles > 1 ? 1024 : 512) + wgs / 2) / wgs;
+      if (n > (p->max_kv + 255) / 256) n = (p->max_kv + 255) / 256;
+      keys = (p->max_kv + n - 1) / n;
+    }
     if (s.few && wgs >= 256 && keys > 1024) keys = wgs * ((keys + 1023) / 1024) <= (p->kv.head_dim == 64 ? 2048 : 1024) ? 512 : 1024;
-    if (keys < 256) keys = 256;
   }
   s.split_keys = (int)((keys + 63) / 64 * 64);
   if (s.split_keys < 64) s.split_keys = 64;

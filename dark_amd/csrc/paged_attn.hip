@@ -1074,17 +1074,21 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   if (s.n_tiles < 1) s.n_tiles = 1;
   const int64_t wgs = (int64_t)s.n_tiles * heads;
   // Parts of a key axis.  Few problems: 512 of them fill the card once (2 x 4 over 131072, 16 problems: 166 us; 172 with 1024
-  // parts, 184 with 768, 183 with 2048), 1024 where a key head has several row tiles, of which shorter sequences lack some (6 x
-  // up to 366 over up to 38700, 8 key heads: 244 us, 339 with 512; 8 x 64 over 8064, one tile: 84 and 78 the other way).  Many,
+  // parts, 184 with 768, 183 with 2048), 1024 where key heads have several row tiles, of which shorter sequences lack some (6 x
+  // up to 366 over up to 38700, 8 key heads: 239 us, 339 with 512; 8 x 64 over 8064, one tile: 84 and 78 the other way).  Many,
   // as with one token for each of many sequences: parts of 1024 keys, because lengths differ and the longest must not finish
   // alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with 4096), of 512 where the card would be filled
   // twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024).  Never below 256 keys (a part's (O, m, l) is then 1/16 of
-  // the keys' bytes at most), none where there are no more than 512 (5 x 279 over 284: 14.5 us, 20.9 in two parts).
+  // the keys' bytes at most), nor below 1024 for the many rows of one sequence, all there (1 x 643 over 645, 32 heads of 64: 17.9
+  // us, 30 in three parts; 1 x 1024 over 8024: 57.8 and 68.7; but 4 x up to 199 over up to 1559: 31.6, 22.9 with parts of 256);
+  // none where there are no more than 512 (5 x 279 over 284: 14.5 us, 20.9 in two parts).
   int64_t keys = p->max_kv;
   if ((s.few == 0 || s.few == 4) && p->max_kv > 512) {
     if (wgs < 256) {
-      int64_t n = ((s.n_tiles > 1 ? 1024 : 512) + wgs / 2) / wgs;
-      if (n > (p->max_kv + 255) / 256) n = (p->max_kv + 255) / 256;
+      const bool tiles = s.n_tiles > 1, ragged = p->n_seqs > 1;
+      int64_t n = ((tiles && ragged ? 1024 : 512) + wgs / 2) / wgs;
+      const int64_t most = (p->max_kv + (tiles && !ragged ? 1023 : 255)) / (tiles && !ragged ? 1024 : 256);
+      if (n > most) n = most;
       keys = (p->max_kv + n - 1) / n;
     }
     if (s.few && wgs >= 256 && keys > 1024) keys = wgs * ((keys + 1023) / 1024) <= (p->kv.head_dim == 64 ? 2048 : 1024) ? 512 : 1024;

@@ -1056,10 +1056,15 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   s.few = 0;
   s.rt = 1;
   if (p->kv.dtype == DARK_F32) {
-    s.few = p->max_kv <= 128 ? 1 : 4;
+    // A wave a problem where keys are few, or problems many: four waves of a workgroup then read the same keys, and nothing is
+    // joined (634 x up to 42 over up to 247, 4 key heads of 128: 403 us, 511 with four waves a problem; 116 x up to 349 over up to
+    // 353: 536 and 725; 21 x up to 346 over up to 531, 7308 problems: 162 and 131 the other way).
     // 32 rows a wave where they are there and dims enough to be worth it (4 x 512 over 2048, 8 key heads of 128: 652 us, 840 with
-    // 16; of 96, 8 x 512 over 2048: 275 and 310; 12 heads of 64, 64 x 40 over 440: 77 and 62)
-    if (rows > 16 && s.few == 4 && p->kv.head_dim > 64) s.rt = 2;
+    // 16; of 96, 8 x 512 over 2048: 275 and 310; 12 heads of 64, 64 x 40 over 440: 77 and 62).
+    const int64_t problems = heads * ((rows + 15) / 16);
+    const bool many = problems >= 8192 && p->max_kv <= 2048 && p->kv.head_dim > 64 && rows > 16;
+    s.few = p->max_kv <= 128 || (p->max_kv <= 256 && problems >= 1024) || many ? 1 : 4;
+    if (rows > 16 && p->kv.head_dim > 64 && (s.few == 4 || (many && p->max_kv > 256))) s.rt = 2;
   }
   else if (rows <= 16 || (rows <= 48 && p->max_kv <= 128)) {   // (512 x 46 over 46, 8 heads of 96: 41.9 us, 45.6 by row tiles;
                                                                // 64 x 8 over 2000, 32 rows: 160 and 98.5 the other way)
@@ -1075,7 +1080,9 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   const int64_t wgs = (int64_t)s.n_tiles * heads;
   // Parts of a key axis.  Few problems: 512 of them fill the card once (2 x 4 over 131072, 16 problems: 166 us; 172 with 1024
   // parts, 184 with 768, 183 with 2048), 1024 where key heads have several row tiles, of which shorter sequences lack some (6 x
-  // up to 366 over up to 38700, 8 key heads: 239 us, 339 with 512; 8 x 64 over 8064, one tile: 84 and 78 the other way).  Many,
+  // up to 366 over up to 38700, 8 key heads: 239 us, 339 with 512; 4 x up to 334 over up to 12305, 32 heads of 64: 177, 287 whole,
+  // 168 and 164 with 2048 and 4096, but 8 x up to 512 over up to 4512 168, 228 and 250; 8 x 64 over 8064, one tile: 84 and 78 the
+  // other way).  Many,
   // as with one token for each of many sequences: parts of 1024 keys, because lengths differ and the longest must not finish
   // alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with 4096), of 512 where the card would be filled
   // twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024).  Never below 256 keys (a part's (O, m, l) is then 1/16 of
@@ -1084,10 +1091,10 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   // none where there are no more than 512 (5 x 279 over 284: 14.5 us, 20.9 in two parts).
   int64_t keys = p->max_kv;
   if ((s.few == 0 || s.few == 4) && p->max_kv > 512) {
-    if (wgs < 256) {
-      const bool tiles = s.n_tiles > 1, ragged = p->n_seqs > 1;
+    const bool tiles = s.n_tiles > 1, ragged = p->n_seqs > 1;
+    if (wgs < (s.few == 0 && tiles && ragged ? 1024 : 256)) {
       int64_t n = ((tiles && ragged ? 1024 : 512) + wgs / 2) / wgs;
-      const int64_t most = (p->max_kv + (tiles && !ragged ? 1023 : 255)) / (tiles && !ragged ? 1024 : 256);
+      const int64_t least = s.few == 0 && tiles && (!ragged || wgs >= 256) ? 1024 : 256, most = (p->max_kv + least - 1) / least;
       if (n > most) n = most;
       keys = (p->max_kv + n - 1) / n;
     }

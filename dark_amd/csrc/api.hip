@@ -30,6 +30,11 @@ static int check_model(const dark_model_desc* m) {
   DARK_CHECK_ARG(m->n_layers >= 0 && (m->n_layers == 0 || m->layers), "layers missing");
   DARK_CHECK_ARG(m->embed && m->final_norm && m->lm_head && m->rope_cos && m->rope_sin, "null weight pointer");
   DARK_CHECK_ARG(m->max_pos >= 1, "max_pos=%d", m->max_pos);
+  for (int l = 0; l < m->n_layers; ++l) {
+    const dark_layer_weights& L = m->layers[l];
+    DARK_CHECK_ARG((L.q_norm == nullptr) == (L.k_norm == nullptr) && (!L.q_norm || (m->ident_cos && m->ident_sin)),
+                   "layer %d: q_norm, k_norm and the identity rotation go together", l);
+  }
   DARK_CHECK_ARG(m->resid_dtype == DARK_F32 || (m->resid_dtype == DARK_BF16 && m->dtype == DARK_BF16),
                  "resid_dtype %d with model dtype %d (fp32 always, bf16 for bf16 models)", m->resid_dtype, m->dtype);
   return DARK_OK;
@@ -79,7 +84,6 @@ static int resid_gemm_norm(const dark_model_desc* m, const void* A, const void* 
 // per-head norms + rotation of the q and k columns of a [M, 3d] projection, in place (pos == null: row index mod N)
 static int norm_heads(const dark_model_desc* m, const dark_layer_weights& L, void* qkv, const int32_t* pos, int M, int N,
                       hipStream_t st) {
-  DARK_CHECK_ARG(L.k_norm && m->ident_cos && m->ident_sin, "q_norm without k_norm or the identity rotation");
   const int64_t es = (int64_t)esize(m->dtype), d = m->d;
   dark_qk_norm_rope_args a = {};
   a.q = a.q_out = qkv;

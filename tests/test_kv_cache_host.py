@@ -83,6 +83,24 @@ def test_null_arguments():
     assert _hip.load().dark_paged_attention_workspace_bytes(None) == 0
 
 
+def test_head_norms_go_together():
+    """A layer with one of the two norms is refused by both forwards before anything is launched."""
+    lib = _hip.load()
+    w = (_hip.LayerWeights * 1)()
+    for name, _ in _hip.LayerWeights._fields_:
+        setattr(w[0], name, 4096)
+    desc = _hip.ModelDesc(dtype=1, vocab=512, vocab_pad=512, d=192, ff=384, n_layers=1, n_heads=2, head_dim=96, max_pos=64, rms_eps=1e-6,
+                          resid_dtype=1, embed=4096, final_norm=4096, lm_head=4096, rope_cos=4096, rope_sin=4096,
+                          layers=C.cast(w, C.POINTER(_hip.LayerWeights)))
+    cached = _hip.CachedTokens(ids=4096, pos=4096, slots=4096)
+    cached.attn.n_tokens = 1
+    for q, k, ident in ((4096, None, 4096), (None, 4096, 4096), (4096, 4096, None)):
+        w[0].q_norm, w[0].k_norm, desc.ident_cos, desc.ident_sin = q, k, ident, ident
+        for rc in (lib.dark_forward_hidden(C.byref(desc), 4096, None, None, 1, 46, 4096, 1 << 40, 4096, None),
+                   lib.dark_forward_cached(C.byref(desc), C.byref(cached), 4096, 1 << 40, 4096, None)):
+            assert rc == _hip.DARK_ERR_ARG and b"go together" in lib.dark_hip_last_error()
+
+
 def test_workspace_bytes():
     """A function of the sizes alone: none for a short axis, parts of (O, m, l) for few rows over a long one."""
     lib = _hip.load()

@@ -311,6 +311,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.kv_len = (const int32_t*)c.vec(a[6], "kv_len", at::kInt, B);
     p.q_index = (const int32_t*)c.vec(a[9], "q_index", at::kInt, T);
     const at::Tensor out = c.out(given(a[13], "out"), "out", q0);
+    need(out.numel() == 0 || out.data_ptr() != q.data_ptr(), "out must not overlap q");
     at::Tensor lse;
     const int want = PyObject_IsTrue(a[14]), causal = PyObject_IsTrue(a[11]);
     if (want < 0 || causal < 0) throw Refusal(nullptr, "");

@@ -91,7 +91,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``block_table[b]`` (int32, an entry outside the cache leaves its keys out).  Left out are keys whose ``key_mask[b, j]``
     (uint8 or bool) is 0 and, with ``causal``, keys behind the token's own place ``q_index[t]`` (int32; default: the
     sequence's last places).  A token with no key left gets zeros (lse -inf).  ``max_q`` / ``max_kv``: the most new tokens /
-    keys of a sequence.  Tokens that belong to no sequence are not written.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out``, or ``(out, lse [T, n_heads] fp32)``."""
+    keys of a sequence.  Tokens that belong to no sequence are not written; ``out`` must not overlap ``q``.  ``scale`` defaults to
+    ``head_dim ** -0.5``.  Returns ``out``, or ``(out, lse [T, n_heads] fp32)``."""
     return (_bind or _ops()).paged_attention(_stream(q), q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_kv, q_index,
                                             key_mask, causal, scale, out, return_lse)
 

@@ -467,6 +467,24 @@ def test_nothing_to_do():
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 40, 200])
+@pytest.mark.parametrize("causal", [False, True])
+def test_sequences_without_keys(dtype, n, causal):
+    """No table, no room, no keys, keys of another sequence only: zeros, and the other sequence as if it were alone."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    p = paged([n, 3], [0, 700], 4, 2, 96, 16, dtype, seed=4)
+    q, k, v = (p[x].to(DEV) for x in "qkv")
+    cu = p["cu"].to(DEV)
+    for table, kv, room in ((torch.zeros(2, 0, dtype=torch.int32), i32(9, 9), 9), (p["table"], i32(0, 700), 0), (p["table"], i32(0, 0), 5000),
+                            (p["table"], i32(-5, -1), 700)):
+        out, lse = kv_cache.paged_attention(q, k, v, table.to(DEV), cu, kv, n, room, causal=causal, return_lse=True)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    got = run_paged(p, causal=causal)
+    assert bool((got[:n] == 0).all())
+    check_attention(got, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=causal), 700, 96, dtype)
+
+
 def test_refused_operands():
     """What a call cannot be given: said by name before anything is enqueued."""
     z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device=DEV)
@@ -513,7 +531,7 @@ def test_refused_operands():
     for kw, msg in ((dict(q=z(2, 6, 96)), "q is"), (dict(cu=i32(0, 1, 2)), "cu_q must be"), (dict(kv=i32(5).long()), "kv_len is torch.int64"),
                     (dict(table=z(1, 3)), "block_table is torch.float32"), (dict(key_mask=z(1, 4, dtype=torch.uint8)), "key_mask is"),
                     (dict(key_mask=z(1, 5)), "uint8 or bool"), (dict(mk=-1), "max_kv=-1"), (dict(q_index=i32(0)), "q_index must be"),
-                    (dict(out=z(2, 8, 96).bfloat16()), "out is torch.bfloat16")):
+                    (dict(out=z(2, 8, 96).bfloat16()), "out is torch.bfloat16"), (dict(out=q), "overlap")):
         with pytest.raises(ValueError, match=msg):
             att(**kw)
     with pytest.raises(_hip.DarkHipError, match="scale"):

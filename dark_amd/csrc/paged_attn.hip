@@ -896,12 +896,15 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
       if (on != ~0ull || (PART && k0 + TT_KEYS > wlo)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const unsigned w = (unsigned)(on >> (32 * t)) >> (4 * h);
-          const int room = seen - (k0 + 32 * t + 4 * h);
+          unsigned out = ~((unsigned)(on >> (32 * t)) >> (4 * h));   // keys left out, by the numbers of this lane's
+          if (PART) {
+            const int room = seen - (k0 + 32 * t + 4 * h);
+            out |= room <= 0 ? ~0u : room >= 32 ? 0u : ~0u << room;
+          }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = (i & 3) + 8 * (i >> 2);
-            if (!((w >> j) & 1) || j >= room) S[t][i] = -INFINITY;
+          for (int i = 0; i < 16; ++i) {   // (the bit over the whole word, then one word or the other: 1 x 725 over 939, masked, 34.9 -> 31.5 us)
+            const unsigned bits = (unsigned)((int)(out << (31 - ((i & 3) + 8 * (i >> 2)))) >> 31);
+            S[t][i] = __uint_as_float((bits & 0xff800000u) | (~bits & __float_as_uint(S[t][i])));   // (-inf, or as it is)
           }
         }
       }

@@ -50,7 +50,7 @@ struct PagedArgs {
   const uint8_t* kmask;
   float *part_o, *part_ml;     // [n_split][T][H][HD], [n_split][T][H][2]; null when n_split == 1
   int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride, page_stride, slot_stride, head_stride;
-  int32_t T, H, Hk, G, B, width, n_pages, page_log2, unit, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
+  int32_t T, H, Hk, G, B, width, n_pages, page_log2, unit, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner, by_length;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
   Div by_hk, by_tiles, by_split, by_group, by_inner, by_heads, by_rows;   // by_rows: max_q * n_heads
   float scale_log2, q_factor;  // scale * log2(e); row tiles: its absolute value (1 for a scale of 0), what q is multiplied by
 };
@@ -715,6 +715,19 @@ template <int HD> struct TileSwz {
 
 constexpr int TT_ROWS = 128, TT_KEYS = 64;
 
+// The sequence with the n-th most keys (of 64 at most, a lane each): the longest begin first and the shortest
+// fill up what is left (24 x up to 200 over up to 6200: 190 us, 235 in the batch's order; 12 x up to 400 over up to
+// 10400, 240 and 292; ordered by rows times keys 238 and 282: a workgroup has 128 rows whatever the sequence has).
+__device__ __forceinline__ int nth_longest(const PagedArgs& a, int n, int lane) {
+  const int len = lane < a.B ? seq_len(a, lane) : -1;
+  int ahead = 0;   // longer sequences, or as long ones before it
+  for (int i = 0; i < a.B; ++i) {
+    const int other = __builtin_amdgcn_readlane(len, i);
+    ahead += other > len || (other == len && i < lane) ? 1 : 0;
+  }
+  return __builtin_ctzll(__ballot(lane < a.B && ahead == n));   // (exactly one is the n-th)
+}
+
 template <int HD, bool ODD, bool NT>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   typedef TileSwz<HD> Z;
@@ -733,7 +746,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   const int tile = a.n_tiles - 1 - id;                // (the tiles of a key head read the same keys; the last see most and come
                                                       // first: 2 chunks of 4096 tokens, causal, 343 -> 302 us)
   id = a.by_split.divmod(rest);
-  const int split = rest, b = a.by_hk.divmod(id), hk = id;
+  const int split = rest;
+  int b = a.by_hk.divmod(id);
+  const int hk = id;
+  if (a.by_length) b = nth_longest(a, b, lane);
   // the page and the mask of key k0 + lane as they stand in memory (made sense of one tile later, so that nothing waits here;
   // the first even before the sequence's length is known, within the table) ...
   const int32_t* tab = a.table + b * a.table_stride;
@@ -1191,6 +1207,9 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   DARK_CHECK_ARG(wgs < (1ll << 30), "%s: %lld workgroups", who, (long long)wgs);
   a.n_units = (int)wgs;
   a.max_q = p->max_q;
+  // (not for short ones, which wait for the ranking: 60 x up to 200 over up to 700 83 us, 97 with it; nor for few, split evenly)
+  a.by_length = s.few == 0 && p->n_seqs > 1 && p->n_seqs <= 64 && p->max_kv >= 1024 && (s.n_split == 1 || wgs >= 512 * (int64_t)s.n_split);
+
   a.by_hk = make_div(a.Hk); a.by_tiles = make_div(s.n_tiles); a.by_split = make_div(s.n_split); a.by_group = make_div(a.G);
   a.by_heads = make_div(a.H); a.by_rows = make_div((int)(s.n_split > 1 ? (int64_t)p->max_q * a.H : 1));
   DARK_CHECK_ARG(s.n_split == 1 || (int64_t)p->n_seqs * p->max_q * p->n_heads < (1ll << 31), "%s: too many rows", who);

@@ -331,6 +331,21 @@ def test_scales_that_are_not_positive(dtype, scale, q_lens, kv_lens, H, Hk, D):
         check_attention(out, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], **kw), max(kv_lens), D, dtype, lse)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("n,max_q", [(24, 1000), (64, 400), (65, 400), (2, 9000)])
+def test_chunks_of_sequences_of_very_different_lengths(n, max_q, causal):
+    """The longest sequence's rows begin first wherever it stands; equal lengths, empty sequences, more room than any has."""
+    kv_lens = [(37 * i) % 90 for i in range(n)]
+    kv_lens[n // 2], kv_lens[-1], kv_lens[0] = 1100, 1100, 0
+    q_lens = [min(k, (5 * i) % 7) for i, k in enumerate(kv_lens)]
+    q_lens[n // 2] = 70
+    p = paged(q_lens, kv_lens, 16, 8, 64, 32, torch.bfloat16, seed=12, lead=1)
+    p["max_q"], p["max_kv"] = max_q, 1200
+    out, lse = run_paged(p, causal=causal, return_lse=True)
+    check_attention(out, O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=causal), 1100, 64, torch.bfloat16, lse)
+    assert torch.equal(run_paged(p, causal=causal)[1:], out[1:])
+
+
 def test_views_strides_and_scores_far_apart():
     """q and out as views of larger tensors; scores so far apart that one key takes the whole row."""
     p = paged([9, 2], [100, 50], 8, 8, 96, 16, torch.float32, seed=8)

@@ -1106,7 +1106,8 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   // parts, 184 with 768, 183 with 2048), 1024 where key heads have several row tiles, of which shorter sequences lack some (6 x
   // up to 366 over up to 38700, 8 key heads: 239 us, 339 with 512; 4 x up to 334 over up to 12305, 32 heads of 64: 177, 287 whole,
   // 168 and 164 with 2048 and 4096, but 8 x up to 512 over up to 4512 168, 228 and 250; 8 x 64 over 8064, one tile: 84 and 78 the
-  // other way).  Many,
+  // other way), and of 2048 keys at most where those are longer, as far as 4096 parts go (18 x up to 200 over up to 36946: 161 us,
+  // 294 without; 11 x up to 142 over up to 25082 210 and 303; but 2 x up to 300 over up to 60300 718 and 691).  Many,
   // as with one token for each of many sequences: parts of 1024 keys, because lengths differ and the longest must not finish
   // alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with 4096), of 512 where the card would be filled
   // twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024).  Never below 256 keys (a part's (O, m, l) is then 1/16 of
@@ -1118,6 +1119,10 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
     const bool tiles = s.n_tiles > 1, ragged = p->n_seqs > 1;
     if (wgs < (s.few == 0 && tiles && ragged ? 1024 : 256)) {
       int64_t n = ((tiles && ragged ? 1024 : 512) + wgs / 2) / wgs;
+      if (s.few == 0 && tiles && ragged) {
+        const int64_t even = (p->max_kv + 2047) / 2048, room = 4096 / wgs;
+        if (n < even) n = even < room ? even : (n < room ? room : n);
+      }
       const int64_t least = s.few == 0 && tiles && (!ragged || wgs >= 256) ? 1024 : 256, most = (p->max_kv + least - 1) / least;
       if (n > most) n = most;
       keys = (p->max_kv + n - 1) / n;

@@ -1,5 +1,5 @@
-"""float64 CPU restatement of the paged cache's operators (dark_amd/kv_cache.py), written from their definitions; a
-checker for the tests only.  The attention also returns the bound its caller derives tolerances from."""
+"""float64 CPU restatement of the paged cache's operators (dark_amd/kv_cache.py), written from their definitions, for
+the tests only.  The attention also returns the bound its caller derives tolerances from."""
 import math
 
 import torch

@@ -1,5 +1,5 @@
 """The paged cache's operators without a GPU: what their entry points refuse (C and Python), the packed argument
-structs, and the float64 checker of the GPU tests against a dense attention."""
+structs, and the float64 oracle of the GPU tests against a dense attention."""
 import ctypes as C
 import math
 
@@ -123,7 +123,7 @@ def test_cpu_tensors_are_refused():
                                  torch.tensor([5], dtype=torch.int32), 1, 5)
 
 
-def test_checker_against_dense_attention():
+def test_oracle_against_dense_attention():
     g = torch.Generator().manual_seed(1)
     B, n, H, Hk, D, page = 2, 21, 4, 2, 64, 8
     q, k, v = (torch.randn(B, n, h, D, generator=g, dtype=torch.float64) for h in (H, Hk, Hk))

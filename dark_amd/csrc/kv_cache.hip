@@ -6,7 +6,10 @@
 // c of them with the 16 bytes at chunk c of the row's first half and of its second half -- the two elements of every rotated
 // pair in one lane -- so the 64 / LPR rows of a pass need no exchange but the norm's sum (log2(LPR) xor-shuffles).  A wave
 // keeps its pass (which heads, hence its pointers, strides and weights) and walks over the tokens, the next one's rows,
-// rotation and, one further, position on their way while it computes.
+// rotation and, one further, position on their way while it computes.  Read and written, each time other inputs: 16383 tokens
+// x 40 fp32 heads of 128 in 120.5 us (5.6 TB/s), 512 x 46 x 16 bf16 heads of 96 in 36 us (4.0; a copy of as much takes 28.7),
+// 1024 x 11 x 24 such heads into their pages in 22 us (4.7), 8 x up to 4096 x 48 bf16 heads of 128 with norms in 118 us (5.5);
+// one token in 2.4 us.  Rows two tokens ahead instead of one: 39.7 us for 38.5, registers cost a wave.
 #include "common.h"
 
 namespace dark {

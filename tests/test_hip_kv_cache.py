@@ -383,6 +383,12 @@ def test_offsets_past_32_bits():
     smallv = torch.stack([qkv[:64, 2 * Hk:], torch.cat([qkv[64:, 2 * Hk:], torch.zeros(28, Hk, D).bfloat16()])])
     ref = O.attention(qkv[:, :Hk], small, smallv, torch.tensor([[0, 1]]), [0, T], [T], causal=True)
     check_attention(out, ref, T, D, torch.bfloat16)
+    last = tuple(r[-1:] for r in ref)      # a single token's stream of the same keys, with room for more as well
+    for room in (T, 2000, 200000):
+        wide = torch.cat([pages, torch.full((1, -(-room // page) - 2 if room > T else 0), -1, dtype=torch.int32)], 1).to(DEV)
+        one = kv_cache.paged_attention(x[T - 1:, :Hk], kc, vc, wide, torch.tensor([0, 1], dtype=torch.int32, device=DEV),
+                                       torch.tensor([T], dtype=torch.int32, device=DEV), 1, room, causal=True)
+        check_attention(one, last, T, D, torch.bfloat16)
 
 
 # --------------------------------------------------------------------------- together

@@ -62,7 +62,8 @@ __device__ __forceinline__ float rsqrt_of(float x) {
 
 // Every condition around a load is the same for the whole wave: lanes without a row of their own load the last one, a side
 // without weights the other's (a branch of its own around each had every load waited for: 512 x 46 40.8 us so, 36.5).
-template <typename T, int HD, bool NORM, bool PAST>
+// ROPE = there are tables; asked at run time, the two ways of a row had its loads waited for (1024 x 11: 27.3 us so, 21.7).
+template <typename T, int HD, bool NORM, bool ROPE, bool PAST>
 __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
   constexpr int N = RowVec<T>::N, HALF = HD / 2, CH = HALF / N;         // CH lanes hold a row
   constexpr int LPR = CH <= 4 ? 4 : CH <= 8 ? 8 : 16, RPP = 64 / LPR;   // lanes a row is given, rows of one pass
@@ -99,10 +100,10 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
     for (int i = 0; i < 2 * N; ++i) w[i] = normed ? w[i] : 1.f;
   }
   raw x1, x2;
-  float cs[N], sn[N];
+  float cs[N] = {}, sn[N] = {};
   int64_t slot = 0;
   auto position = [&](int tt) {
-    if (!a.cosT || tt >= a.T) return 0;
+    if (!ROPE || tt >= a.T) return 0;
     const int q = a.pos ? a.pos[tt] : tt % a.pos_period;
     return q < 0 ? 0 : (q >= a.max_pos ? a.max_pos - 1 : q);
   };
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
     x1 = *(const raw*)src;
     x2 = *(const raw*)(src + HALF);
     if (a.slots) slot = a.slots[tt];
-    if (a.cosT) {
+    if constexpr (ROPE) {
       const float* cp = a.cosT + (int64_t)pp * HALF + at;
       const float* sp = a.sinT + (int64_t)pp * HALF + at;
 #pragma unroll
@@ -120,8 +121,6 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
       }
     }
   };
-#pragma unroll
-  for (int i = 0; i < N; ++i) { cs[i] = 1.f; sn[i] = 0.f; }
   fetch(t, position(t));
   int p_next = position(t + step);
   while (true) {
@@ -154,12 +153,13 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const RowsArgs a) {
         f2[i] *= inv * w[N + i];
       }
     }
+    // (without tables no turn by an angle of 0: an infinity times its sine would make the other half's element a NaN)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      o1[i] = f1[i] * cc[i] - f2[i] * ss[i];
-      o2[i] = f2[i] * cc[i] + f1[i] * ss[i];
+      o1[i] = ROPE ? f1[i] * cc[i] - f2[i] * ss[i] : f1[i];
+      o2[i] = ROPE ? f2[i] * cc[i] + f1[i] * ss[i] : f2[i];
     }
-    if (role < 2) {   // (values are carried as they are)
+    if (role < 2 && (ROPE || normed)) {   // (values, and rows with neither norm nor rotation, are carried as they are)
       y1 = RowVec<T>::down(o1);
       y2 = RowVec<T>::down(o2);
     }
@@ -228,12 +228,16 @@ static int launch_head_rows(RowsArgs& a, int dtype, int HD, hipStream_t st) {
   // be read)
   const bool past = (int64_t)a.T * a.h_end[2] * HD * (dtype == DARK_BF16 ? 2 : 4) > (int64_t)256 << 20;
   const dim3 grid((unsigned)cdiv(a.t_step * a.n_pass, 4)), block(256);
-#define DARK_ROWS(T, HDv)                                                                                  \
-  do {                                                                                                     \
-    if (norm && past) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true, true>), grid, block, 0, st, a);   \
-    else if (norm) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true, false>), grid, block, 0, st, a);     \
-    else if (past) hipLaunchKernelGGL((head_rows_kernel<T, HDv, false, true>), grid, block, 0, st, a);     \
-    else hipLaunchKernelGGL((head_rows_kernel<T, HDv, false, false>), grid, block, 0, st, a);              \
+#define DARK_ROWS_AT(T, HDv, ROPE)                                                                               \
+  do {                                                                                                           \
+    if (norm && past) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true, ROPE, true>), grid, block, 0, st, a);   \
+    else if (norm) hipLaunchKernelGGL((head_rows_kernel<T, HDv, true, ROPE, false>), grid, block, 0, st, a);     \
+    else if (past) hipLaunchKernelGGL((head_rows_kernel<T, HDv, false, ROPE, true>), grid, block, 0, st, a);     \
+    else hipLaunchKernelGGL((head_rows_kernel<T, HDv, false, ROPE, false>), grid, block, 0, st, a);              \
+  } while (0)
+#define DARK_ROWS(T, HDv)                                                                    \
+  do {                                                                                       \
+    if (a.cosT) DARK_ROWS_AT(T, HDv, true); else DARK_ROWS_AT(T, HDv, false);                \
   } while (0)
   if (dtype == DARK_BF16) {
     if (HD == 64) DARK_ROWS(bf16_t, 64); else if (HD == 96) DARK_ROWS(bf16_t, 96); else DARK_ROWS(bf16_t, 128);
@@ -241,6 +245,7 @@ static int launch_head_rows(RowsArgs& a, int dtype, int HD, hipStream_t st) {
     if (HD == 64) DARK_ROWS(float, 64); else if (HD == 96) DARK_ROWS(float, 96); else DARK_ROWS(float, 128);
   }
 #undef DARK_ROWS
+#undef DARK_ROWS_AT
   DARK_CHECK_LAUNCH();
   return DARK_OK;
 }

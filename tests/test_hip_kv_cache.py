@@ -169,6 +169,39 @@ def test_append_kv(dtype, T, H, Hk, D, page, norm, heads_first):
     assert torch.equal(view(k2).cpu(), O.append(view(kc), qkv[:, H:H + Hk], slots))
 
 
+def bits(t):
+    return t.contiguous().view(torch.int16 if t.dtype == torch.bfloat16 else torch.int32).cpu()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,H,Hk,D", [(5, 8, 2, 96), (40, 3, 3, 64), (3, 32, 8, 128)])
+def test_rows_without_a_rotation(dtype, T, H, Hk, D):
+    """No tables: infinities, NaN and zeros of either sign stay in their own elements.  Without a norm too the rows are
+    carried bit for bit; a norm on one side leaves the other side's so."""
+    g = torch.Generator().manual_seed(D)
+    x = torch.randn(T, H + 2 * Hk, D, generator=g).to(dtype)
+    h = D // 2
+    for r in (0, H):                                          # a query's and a key's head
+        x[0, r, 3], x[0, r, h + 7] = math.inf, -math.inf      # one half each
+        x[1, r, h + 1], x[1, r, 5] = math.nan, -0.0
+        x[2, r] = -0.0
+        x[2, r, :4] = 2.0 ** -130                             # denormal
+    xd, w = x.to(DEV), 1 + 0.2 * torch.randn(D, generator=g)
+    q, k = kv_cache.qk_norm_rope(xd[:, :H], xd[:, H:H + Hk], None, None, None, None, None)
+    assert torch.equal(bits(q), bits(x[:, :H])) and torch.equal(bits(k), bits(x[:, H:H + Hk]))
+    q, k = kv_cache.qk_norm_rope(xd[:, :H], xd[:, H:H + Hk], w.to(DEV), None, None, None, None)
+    assert torch.equal(bits(k), bits(x[:, H:H + Hk]))
+    check_rows(q[2:], *O.norm_rope(x[2:, :H], w, None, None, None, 1e-6), dtype)
+    n = q[1, 0].cpu()                                         # (a NaN under the root reaches its own row only)
+    assert bool(n.isnan().all()) and not bool(q[1, 1:].isnan().any())
+    kc, vc = (torch.zeros(2, 64, Hk, D, dtype=dtype, device=DEV) for _ in range(2))
+    slots = torch.randperm(128, generator=g)[:T].to(DEV)
+    q = kv_cache.append_kv(xd[:, H:H + Hk], xd[:, H + Hk:], kc, vc, slots, q=xd[:, :H])
+    assert torch.equal(bits(q), bits(x[:, :H]))
+    assert torch.equal(bits(kc.view(128, Hk, D)[slots]), bits(x[:, H:H + Hk]))
+    assert torch.equal(bits(vc.view(128, Hk, D)[slots]), bits(x[:, H + Hk:]))
+
+
 # --------------------------------------------------------------------------- attention
 def paged(q_lens, kv_lens, H, Hk, D, page, dtype, seed=0, spare=3, lead=0, tail=0, heads_first=False, fill=math.nan):
     """A batch over shuffled pages; every slot no sequence uses holds `fill`."""

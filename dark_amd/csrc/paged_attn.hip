@@ -50,7 +50,7 @@ struct PagedArgs {
   const uint8_t* kmask;
   float *part_o, *part_ml;     // [n_split][T][H][HD], [n_split][T][H][2]; null when n_split == 1
   int64_t q_ts, q_hs, o_ts, o_hs, table_stride, mask_stride, page_stride, slot_stride, head_stride;
-  int32_t T, H, Hk, G, B, width, n_pages, page_log2, unit, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner, by_length;   // n_units: problems of the launch: sequences x key heads x row tiles x parts
+  int32_t T, H, Hk, G, B, width, n_pages, page_log2, unit, causal, n_split, split_keys, n_tiles, cap, max_q, n_units, n_inner, by_length, block0;   // block0: workgroups (join: rows) of the call before this launch's; n_units: problems of the launch: sequences x key heads x row tiles x parts
   Div by_hk, by_tiles, by_split, by_group, by_inner, by_heads, by_rows;   // by_rows: max_q * n_heads
   float scale_log2, q_factor;  // scale * log2(e); row tiles: its absolute value (1 for a scale of 0), what q is multiplied by
 };
@@ -58,10 +58,11 @@ struct PagedArgs {
 // Workgroups are handed to the eight XCDs, each with an L2 of its own, in turn.  `n_inner` units that follow each other and
 // read the same memory (row tiles of a key head; key heads of one token row) go to one XCD: unit number of this workgroup.
 __device__ __forceinline__ int unit_of_block(const PagedArgs& a) {
-  if (a.n_inner <= 1) return blockIdx.x;
-  int k = blockIdx.x >> 3;
+  const int block = a.block0 + blockIdx.x;
+  if (a.n_inner <= 1) return block;
+  int k = block >> 3;
   const int group = a.by_inner.divmod(k);
-  return (group * 8 + (blockIdx.x & 7)) * a.n_inner + k;
+  return (group * 8 + (block & 7)) * a.n_inner + k;
 }
 
 // keys of a sequence: what it says, within the table and the caller's bound (hence within the mask's rows)
@@ -1013,7 +1014,7 @@ template <typename T, int HD, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   __shared__ float so[4][HD], sl[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int h = WPR == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+  int h = a.block0 + (WPR == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave);
   const int b = a.by_rows.divmod(h);
   if (b >= a.B) return;
   const int i = a.by_heads.divmod(h);
@@ -1059,6 +1060,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   }
   if (a.lse && lane == 0) a.lse[row] = lse_of(m, l);
 }
+
+// Workgroups of one launch at most, a multiple of the XCDs; a call of more takes several.  (A launch of 2^32 threads or more is
+// not refused: it runs the rest of a division by 2^32.)
+constexpr int MAX_BLOCKS = 1 << 22;
 
 struct PagedPlan {
   int few, rt;           // waves a problem in the streaming kernels (0: tiles of rows) and their 16-row tiles
@@ -1217,7 +1222,8 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
 
   a.by_hk = make_div(a.Hk); a.by_tiles = make_div(s.n_tiles); a.by_split = make_div(s.n_split); a.by_group = make_div(a.G);
   a.by_heads = make_div(a.H); a.by_rows = make_div((int)(s.n_split > 1 ? (int64_t)p->max_q * a.H : 1));
-  DARK_CHECK_ARG(s.n_split == 1 || (int64_t)p->n_seqs * p->max_q * p->n_heads < (1ll << 31), "%s: too many rows", who);
+  const int64_t jrows = s.n_split > 1 ? (int64_t)p->n_seqs * p->max_q * p->n_heads : 0;   // (padded: a sequence's last may not be there)
+  DARK_CHECK_ARG(jrows < (1ll << 31) - MAX_BLOCKS * 4, "%s: too many rows", who);
   // Units that share memory on one XCD: all heads and row tiles of a part, or else the row tiles of a key head -- where there
   // are enough such groups to even out what they hold, or eight heads that hold the same (16 sequences of up to 512 keys,
   // 12 heads, fp32: 27.4 us, 30.4 with the sequences dealt out whole).
@@ -1235,37 +1241,46 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
     }
   }
   a.by_inner = make_div(a.n_inner);
-  const dim3 grid((unsigned)blocks), block(s.few == 8 ? 512 : 256), jblock(256);
-  const unsigned jrows = (unsigned)((int64_t)p->n_seqs * p->max_q * p->n_heads);
-#define DARK_JOIN(T, HDv)                                                                           \
-  if (s.n_split > 8) hipLaunchKernelGGL((paged_join_kernel<T, HDv, 4>), dim3(jrows), jblock, 0, st, a);  \
-  else if (s.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<T, HDv, 1>), dim3((jrows + 3) / 4), jblock, 0, st, a)
-#define DARK_PAGED_BF16(HDv)                                                                        \
-  do {                                                                                              \
-    if (s.few == 1) hipLaunchKernelGGL((paged_few_kernel<HDv, 1, ODD, false>), grid, block, 0, st, a);     \
-    else if (s.few == 4 && past) hipLaunchKernelGGL((paged_few_kernel<HDv, 4, ODD, HDv % 64 == 0>), grid, block, 0, st, a); \
-    else if (s.few == 4) hipLaunchKernelGGL((paged_few_kernel<HDv, 4, ODD, false>), grid, block, 0, st, a); \
-    else if (s.few == 8) hipLaunchKernelGGL((paged_few_kernel<HDv, 8, ODD, false>), grid, block, 0, st, a); \
-    else {                                                                                          \
-      constexpr int lds = 4 * TT_KEYS * HDv * 2;                                                    \
-      static SmemOptIn optin, optin_nt;                                                             \
-      if (past && s.n_tiles == 1) {                                                                 \
-        DARK_TRY(optin_nt.ensure((const void*)paged_tile_kernel<HDv, ODD, HDv % 64 == 0>, lds, st)); \
-        hipLaunchKernelGGL((paged_tile_kernel<HDv, ODD, HDv % 64 == 0>), grid, block, lds, st, a);  \
-      } else {                                                                                      \
-        DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv, ODD, false>, lds, st));           \
-        hipLaunchKernelGGL((paged_tile_kernel<HDv, ODD, false>), grid, block, lds, st, a);          \
-      }                                                                                             \
-    }                                                                                               \
-    DARK_JOIN(bf16_t, HDv);                                                                         \
+  auto launch = [&](auto kernel, int lds) {
+    for (a.block0 = 0; a.block0 < blocks; a.block0 += MAX_BLOCKS)
+      hipLaunchKernelGGL(kernel, dim3(blocks - a.block0 < MAX_BLOCKS ? blocks - a.block0 : MAX_BLOCKS), dim3(s.few == 8 ? 512 : 256), lds, st, a);
+  };
+  auto join = [&](auto kernel, int per) {   // `per` rows a workgroup
+    for (int64_t row = 0; row < jrows; row += (int64_t)MAX_BLOCKS * per) {
+      const int64_t n = (jrows - row + per - 1) / per;
+      a.block0 = (int)row;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(n < MAX_BLOCKS ? n : MAX_BLOCKS)), dim3(256), 0, st, a);
+    }
+  };
+#define DARK_JOIN(T, HDv)                                                 \
+  if (s.n_split > 8) join(paged_join_kernel<T, HDv, 4>, 1);               \
+  else if (s.n_split > 1) join(paged_join_kernel<T, HDv, 1>, 4)
+#define DARK_PAGED_BF16(HDv)                                                                                        \
+  do {                                                                                                              \
+    if (s.few == 1) launch(paged_few_kernel<HDv, 1, ODD, false>, 0);                                                \
+    else if (s.few == 4 && past) launch(paged_few_kernel<HDv, 4, ODD, HDv % 64 == 0>, 0);                           \
+    else if (s.few == 4) launch(paged_few_kernel<HDv, 4, ODD, false>, 0);                                           \
+    else if (s.few == 8) launch(paged_few_kernel<HDv, 8, ODD, false>, 0);                                           \
+    else {                                                                                                          \
+      constexpr int lds = 4 * TT_KEYS * HDv * 2;                                                                    \
+      static SmemOptIn optin, optin_nt;                                                                             \
+      if (past && s.n_tiles == 1) {                                                                                 \
+        DARK_TRY(optin_nt.ensure((const void*)paged_tile_kernel<HDv, ODD, HDv % 64 == 0>, lds, st));                \
+        launch(paged_tile_kernel<HDv, ODD, HDv % 64 == 0>, lds);                                                    \
+      } else {                                                                                                      \
+        DARK_TRY(optin.ensure((const void*)paged_tile_kernel<HDv, ODD, false>, lds, st));                           \
+        launch(paged_tile_kernel<HDv, ODD, false>, lds);                                                            \
+      }                                                                                                             \
+    }                                                                                                               \
+    DARK_JOIN(bf16_t, HDv);                                                                                         \
   } while (0)
-#define DARK_PAGED_F32(HDv)                                                                         \
-  do {                                                                                              \
-    if (s.few == 1 && s.rt == 2) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1, 2, ODD>), grid, block, 0, st, a); \
-    else if (s.few == 1) hipLaunchKernelGGL((paged_f32_kernel<HDv, 1, 1, ODD>), grid, block, 0, st, a); \
-    else if (s.rt == 2) hipLaunchKernelGGL((paged_f32_kernel<HDv, 4, 2, ODD>), grid, block, 0, st, a); \
-    else hipLaunchKernelGGL((paged_f32_kernel<HDv, 4, 1, ODD>), grid, block, 0, st, a);             \
-    DARK_JOIN(float, HDv);                                                                          \
+#define DARK_PAGED_F32(HDv)                                                             \
+  do {                                                                                  \
+    if (s.few == 1 && s.rt == 2) launch(paged_f32_kernel<HDv, 1, 2, ODD>, 0);           \
+    else if (s.few == 1) launch(paged_f32_kernel<HDv, 1, 1, ODD>, 0);                   \
+    else if (s.rt == 2) launch(paged_f32_kernel<HDv, 4, 2, ODD>, 0);                    \
+    else launch(paged_f32_kernel<HDv, 4, 1, ODD>, 0);                                   \
+    DARK_JOIN(float, HDv);                                                              \
   } while (0)
   const int HD = p->kv.head_dim;
   // NT: keys that, with four layers of them, cannot stay in the 256 MB behind the L2s until they are read again go past the caches (64 x 1 over up

@@ -379,6 +379,34 @@ def test_chunks_of_sequences_of_very_different_lengths(n, max_q, causal):
     assert torch.equal(run_paged(p, causal=causal)[1:], out[1:])
 
 
+@pytest.mark.parametrize("dtype,n,max_q,max_kv,H,Hk,D,page", [
+    (torch.bfloat16, (1 << 21) + 77, 1, 100, 8, 8, 64, 128),       # a wave a problem
+    (torch.bfloat16, (1 << 17) + 5, 4, 9000, 32, 8, 64, 4096),     # parts of the keys, and 2^24 rows to join one by one
+    (torch.bfloat16, (1 << 17) + 5, 4, 1500, 32, 8, 96, 512),      # ... four by four
+    (torch.bfloat16, (1 << 17) + 5, 600, 700, 8, 8, 96, 256),      # row tiles
+    (torch.float32, (1 << 17) + 5, 600, 1000, 8, 8, 64, 256),      # 2^32 threads and more
+    (torch.float32, (1 << 17) + 5, 600, 1000, 8, 8, 128, 256),
+])
+def test_more_workgroups_than_a_launch_holds(dtype, n, max_q, max_kv, H, Hk, D, page):
+    """Room for so many sequences that one call takes several launches; a few of them have tokens, the first and last too."""
+    assert n * Hk * max(1, max_q * (H // Hk) // 128) >= 1 << 20
+    q_lens = [min(max_q, x) for x in (1, 3, 130, 2, 1)]
+    kv_lens = [min(max_kv, x) for x in (max_kv, 40, 1030, 77, max_kv - 3)]
+    p = paged(q_lens, kv_lens, H, Hk, D, page, dtype, seed=3, tail=2)
+    ref = O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], causal=True)
+    at = torch.tensor([0, 1, n // 2 + 3, n - 2, n - 1])
+    new = torch.zeros(n, dtype=torch.int32)
+    new[at] = torch.tensor(q_lens, dtype=torch.int32)
+    kv = torch.zeros(n, dtype=torch.int32)
+    kv[at] = p["kv"]
+    table = torch.full((n, p["table"].shape[1]), -1, dtype=torch.int32)
+    table[at] = p["table"]
+    p.update(table=table, kv=kv, cu=torch.cat([torch.zeros(1, dtype=torch.int32), new.cumsum(0).int()]), max_q=max_q, max_kv=max_kv)
+    out, lse = run_paged(p, causal=True, out=torch.full(p["q"].shape, 5.0, dtype=dtype, device=DEV), return_lse=True)
+    check_attention(out, ref, max_kv, D, dtype, lse)
+    assert bool((out[-2:] == 5).all())
+
+
 def test_views_strides_and_scores_far_apart():
     """q and out as views of larger tensors; scores so far apart that one key takes the whole row."""
     p = paged([9, 2], [100, 50], 8, 8, 96, 16, torch.float32, seed=8)

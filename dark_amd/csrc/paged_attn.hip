@@ -1112,11 +1112,13 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   // up to 366 over up to 38700, 8 key heads: 239 us, 339 with 512; 4 x up to 334 over up to 12305, 32 heads of 64: 177, 287 whole,
   // 168 and 164 with 2048 and 4096, but 8 x up to 512 over up to 4512 168, 228 and 250; 8 x 64 over 8064, one tile: 84 and 78 the
   // other way), and of 2048 keys at most where those are longer, as far as 4096 parts go (18 x up to 200 over up to 36946: 161 us,
-  // 294 without; 11 x up to 142 over up to 25082 210 and 303; but 2 x up to 300 over up to 60300 718 and 691).  Many,
-  // as with one token for each of many sequences: parts of 1024 keys, because lengths differ and the longest must not finish
+  // 294 without; 11 x up to 142 over up to 25082 210 and 303; but 2 x up to 300 over up to 60300 718 and 691).  Many
+  // with one row tile a key head, as with one token for each of many sequences: parts of 1024 keys, because lengths differ and the longest must not finish
   // alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with 4096), of 512 where the card would be filled
-  // twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024).  Never below 256 keys (a part's (O, m, l) is then 1/16 of
-  // the keys' bytes at most), nor below 1024 for the many rows of one sequence, all there (1 x 643 over 645, 32 heads of 64: 17.9
+  // twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024); many row tiles in fp32 as far as 4096 parts go, or else
+  // what is joined grows with tokens times keys (4 x 1024 over 9216, 8 key heads of 128: 4.93 ms whole, 5.75 in 9 parts; 1 x
+  // 1500 over 20000, 8 heads of 96: 1.20 and 0.96 in 10).  Never below 256 keys (a part's (O, m, l) is then 1/16 of the keys'
+  // bytes at most for 16 rows, 1/2 for the 128 of a row tile), nor below 1024 for the many rows of one sequence, all there (1 x 643 over 645, 32 heads of 64: 17.9
   // us, 30 in three parts; 1 x 1024 over 8024: 57.8 and 68.7; but 4 x up to 199 over up to 1559: 31.6, 22.9 with parts of 256);
   // none where there are no more than 512 (5 x 279 over 284: 14.5 us, 20.9 in two parts).
   int64_t keys = p->max_kv;
@@ -1132,7 +1134,19 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
       if (n > most) n = most;
       keys = (p->max_kv + n - 1) / n;
     }
-    if (s.few && wgs >= 256 && keys > 1024) keys = wgs * ((keys + 1023) / 1024) <= (p->kv.head_dim == 64 ? 2048 : 1024) ? 512 : 1024;
+    if (s.few && wgs >= 256 && keys > 1024) {
+      if (s.n_tiles == 1) {
+        keys = wgs * ((keys + 1023) / 1024) <= (p->kv.head_dim == 64 ? 2048 : 1024) ? 512 : 1024;
+      } else {
+        int64_t n = (keys + 1023) / 1024;
+        if (n > 4096 / wgs) n = 4096 / wgs;
+        if (n > 1) keys = (keys + n - 1) / n;
+      }
+    }
+    // no more than 1 GiB of parts (a token has room in every part, however short its own axis; 1024 single tokens, one of them
+    // over 131072 keys, 8 key heads of 128: 977 us in 62 parts, 1772 in 128, 2 GiB)
+    const int64_t part = (int64_t)p->n_tokens * p->n_heads * (p->kv.head_dim * 4 + 8), room = ((int64_t)1 << 30) / (part > 0 ? part : 1);
+    if ((p->max_kv + keys - 1) / keys > room) keys = room > 1 ? (p->max_kv + room - 1) / room : p->max_kv;
   }
   s.split_keys = (int)((keys + 63) / 64 * 64);
   if (s.split_keys < 64) s.split_keys = 64;

@@ -436,8 +436,8 @@ int dark_kv_append(const dark_kv_append_args* a, void* stream);
  *   max_q, max_kv: no sequence has more new tokens / more keys (tokens of a sequence beyond max_q may be left as they
  *     were, keys beyond max_kv are left out)
  *   lse [n_tokens, n_heads] fp32 or NULL: log(sum_j exp(score))
- * workspace: dark_paged_attention_workspace_bytes(a) bytes, 16-byte aligned (0: none needed); calls that overlap must not
- * share it. */
+ * workspace: dark_paged_attention_workspace_bytes(a) bytes, 16-byte aligned (0: none needed; about 1 GiB at most); calls
+ * that overlap must not share it. */
 typedef struct dark_paged_attention_args {
   dark_paged_kv kv;
   const void* q;

@@ -111,6 +111,26 @@ def test_workspace_bytes():
     assert n > 0 and n >= 2 * 3 * 8 * (96 + 2) * 4
 
 
+@pytest.mark.parametrize("dtype", [_hip.DARK_F32, _hip.DARK_BF16])
+def test_workspace_does_not_grow_with_tokens_times_keys(dtype):
+    """Long chunks fill the card by themselves: their keys are not cut (or into a bounded number of parts), and many single
+    tokens beside one long sequence stay within 1 GiB."""
+    lib = _hip.load()
+
+    def need(seqs, new, keys, tokens=None, heads=32, kv_heads=8, dim=128):
+        kv = _kv(dtype=dtype, n_kv_heads=kv_heads, head_dim=dim, slot_stride=dim, head_stride=16 * dim, page_stride=16 * kv_heads * dim)
+        a = _hip.PagedAttentionArgs(kv=kv, n_tokens=tokens or seqs * new, n_heads=heads, n_seqs=seqs, table_width=-(-keys // 16),
+                                    max_q=new, max_kv=keys, scale=0.1)
+        return lib.dark_paged_attention_workspace_bytes(C.byref(a))
+
+    for seqs, new, keys in ((1, 16384, 16384), (1, 32768, 32768), (8, 4096, 65536), (1, 131072, 131072), (4, 1024, 9216)):
+        assert need(seqs, new, keys) == 0, (seqs, new, keys)
+    for seqs, new, keys, tokens in ((128, 4096, 16384, 4096 + 127), (64, 40, 131072, 2560), (2, 300, 60300, 600), (1, 100, 1 << 20, 100),
+                                    (1024, 1, 131072, 1024), (4096, 1, 1 << 20, 4096), (1 << 16, 4, 1 << 18, 1 << 18)):
+        for heads, kv_heads, dim in ((32, 8, 128), (12, 12, 64), (8, 8, 96)):
+            assert need(seqs, new, keys, tokens, heads, kv_heads, dim) <= (1 << 30) + 512, (seqs, new, keys, heads)
+
+
 def test_cpu_tensors_are_refused():
     q = torch.zeros(1, 8, 96)
     cache = torch.zeros(2, 16, 8, 96)

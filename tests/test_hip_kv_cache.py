@@ -129,6 +129,27 @@ def test_more_rows_than_the_caches_hold(dtype, T, H, Hk, D, norm):
     assert torch.equal(vc.view(-1, Hk, D)[d(slots)], xd[:, H + Hk:])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("norm,rope", [(True, True), (False, True), (True, False), (False, False)])
+def test_more_rows_than_the_caches_hold_of_each_kind(dtype, D, norm, rope):
+    """Over 256 MB of rows of each type and width, with and without norm and rotation; a sample of them checked."""
+    T, H, Hk = (257 << 20) // (3 * D * dtype.itemsize) + 5, 2, 1
+    g = torch.Generator(device=DEV).manual_seed(D)
+    x = torch.randn(T, H + Hk, D, generator=g, device=DEV).to(dtype)
+    w = 1 + 0.2 * torch.randn(D, generator=g, device=DEV) if norm else None
+    cos, sin = tables(1000, D) if rope else (None, None)
+    pos = torch.randint(0, 1000, (T,), generator=g, device=DEV, dtype=torch.int32) if rope else None
+    d = lambda t: None if t is None else t.to(DEV)
+    q, k = kv_cache.qk_norm_rope(x[:, :H], x[:, H:], w, w, d(cos), d(sin), pos, eps=1e-6)
+    if not norm and not rope:
+        assert torch.equal(q, x[:, :H]) and torch.equal(k, x[:, H:])
+    at = torch.cat([torch.tensor([0, T - 1]), torch.randint(0, T, (300,), generator=torch.Generator().manual_seed(1))])
+    c = lambda t: None if t is None else t.cpu()
+    for got, src in ((q, x[:, :H]), (k, x[:, H:])):
+        check_rows(got[d(at)], *O.norm_rope(src[d(at)].cpu(), c(w), cos, sin, pos[d(at)].cpu() if rope else None, 1e-6), dtype)
+
+
 # --------------------------------------------------------------------------- append
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T,H,Hk,D,page", [(1, 8, 8, 96, 16), (53, 12, 12, 64, 1), (200, 32, 8, 128, 64), (7, 3, 1, 96, 4096)])
@@ -405,6 +426,52 @@ def test_more_workgroups_than_a_launch_holds(dtype, n, max_q, max_kv, H, Hk, D, 
     out, lse = run_paged(p, causal=True, out=torch.full(p["q"].shape, 5.0, dtype=dtype, device=DEV), return_lse=True)
     check_attention(out, ref, max_kv, D, dtype, lse)
     assert bool((out[-2:] == 5).all())
+
+
+F32, BF16 = torch.float32, torch.bfloat16
+PLANS = [  # dtype, sequences, new tokens, keys, room for (new tokens, keys), H, Hk, D
+    (F32, 9, 40, 1100, (2000, 1200), 8, 8, 128),         # 8192 problems and more: a wave each, 32 rows
+    (F32, 9, 23, 700, (1000, 900), 16, 4, 96),
+    (F32, 10, 20, 200, (160, 256), 12, 12, 64),          # ... of few keys: 16 rows
+    (F32, 10, 20, 200, (160, 250), 4, 4, 128),
+    (F32, 3, 40, 500, (40, 500), 8, 8, 64),              # four waves a problem, a key head's tiles on one XCD
+    (F32, 70, 20, 290, (20, 300), 4, 2, 96),             # all of a sequence's
+    (F32, 70, 3, 100, (9, 128), 12, 12, 64),             # four problems a workgroup, a sequence's on one XCD
+    (F32, 8, 100, 2900, (100, 3000), 8, 8, 64),          # many row tiles whose keys are cut
+    (F32, 16, 40, 2500, (80, 2600), 16, 8, 128),
+    (F32, 40, 1, 2900, (1, 3000), 32, 8, 128),           # single tokens in parts of 512 keys
+    (BF16, 40, 1, 2900, (1, 3000), 32, 8, 128),
+    (F32, 70, 1, 2900, (1, 3000), 8, 8, 96),             # ... of 1024
+    (BF16, 70, 1, 2900, (1, 3000), 8, 8, 96),
+    (BF16, 70, 2, 2900, (2, 3000), 24, 8, 64),
+    (F32, 70, 1, 9900, (1, 10000), 12, 12, 64),          # more than eight parts
+    (BF16, 70, 1, 9900, (1, 10000), 32, 8, 128),
+    (BF16, 130, 11, 46, (11, 46), 8, 8, 96),             # a denoise step between two whole ones
+    (BF16, 130, 46, 46, (46, 46), 2, 2, 96),             # a whole one
+    (BF16, 66, 3, 120, (3, 128), 32, 8, 128),
+    (BF16, 70, 3, 200, (3, 250), 12, 12, 64),            # four waves a problem, keys that stay in the caches
+    (BF16, 40, 200, 1500, (200, 1500), 4, 4, 64),        # row tiles in parts
+]
+
+
+@pytest.mark.parametrize("plan", range(len(PLANS)))
+@pytest.mark.parametrize("causal", [False, True])
+def test_large_batches(plan, causal):
+    """The divisions of work that many sequences, or room for long ones, bring: most sequences short, one whole, some without
+    tokens or keys.  Causal calls are masked as well."""
+    dtype, n, new, keys, room, H, Hk, D = PLANS[plan]
+    kv_lens = [(23 * i) % min(60, keys) for i in range(n)]
+    kv_lens[n // 3], kv_lens[-1], kv_lens[1] = keys, keys // 2, min(keys, 1 + keys * 2 // 3)
+    q_lens = [1 if new == 1 else min(kv_lens[i], (5 * i) % min(new + 1, 8)) for i in range(n)]
+    q_lens[n // 3], q_lens[-1] = new, min(new, 5)
+    p = paged(q_lens, kv_lens, H, Hk, D, 32, dtype, seed=plan, lead=1, tail=1)
+    p["max_q"], p["max_kv"] = room
+    mask = torch.rand(n, room[1], generator=torch.Generator().manual_seed(plan)) > 0.2 if causal else None
+    kw = dict(causal=causal, key_mask=mask)
+    out, lse = run_paged(p, out=torch.full(p["q"].shape, 5.0, dtype=dtype, device=DEV), return_lse=True, **kw)
+    check_attention(out[1:-1], tuple(x[1:-1] for x in O.attention(p["q"], p["k"], p["v"], p["table"], p["cu"], p["kv"], **kw)), keys, D, dtype, lse[1:-1])
+    assert bool((out[:1] == 5).all()) and bool((out[-1:] == 5).all())
+    assert torch.equal(run_paged(p, **kw)[1:-1], out[1:-1])
 
 
 def test_views_strides_and_scores_far_apart():

@@ -1290,10 +1290,12 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   } while (0)
 #define DARK_PAGED_F32(HDv)                                                             \
   do {                                                                                  \
-    if (s.few == 1 && s.rt == 2) launch(paged_f32_kernel<HDv, 1, 2, ODD>, 0);           \
-    else if (s.few == 1) launch(paged_f32_kernel<HDv, 1, 1, ODD>, 0);                   \
-    else if (s.rt == 2) launch(paged_f32_kernel<HDv, 4, 2, ODD>, 0);                    \
-    else launch(paged_f32_kernel<HDv, 4, 1, ODD>, 0);                                   \
+    if (s.rt == 1 && s.few == 1) launch(paged_f32_kernel<HDv, 1, 1, ODD>, 0);           \
+    else if (s.rt == 1) launch(paged_f32_kernel<HDv, 4, 1, ODD>, 0);                    \
+    else if constexpr (HDv > 64) {   /* (32 rows a wave, see plan_paged) */             \
+      if (s.few == 1) launch(paged_f32_kernel<HDv, 1, 2, ODD>, 0);                      \
+      else launch(paged_f32_kernel<HDv, 4, 2, ODD>, 0);                                 \
+    }                                                                                   \
     DARK_JOIN(float, HDv);                                                              \
   } while (0)
   const int HD = p->kv.head_dim;

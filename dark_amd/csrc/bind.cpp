@@ -371,4 +371,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__bind(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__bind(void) {
+  PyObject* m = PyModule_Create(&module);
+  // (the argument structs this file was compiled with: whoever binds the library compares)
+  if (m && PyModule_AddIntConstant(m, "ABI_VERSION", DARK_HIP_ABI_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -32,6 +32,9 @@ def _ops():
         except ImportError as e:
             raise ImportError(f"dark_amd/_bind.so cannot be loaded ({e}): build it with `make -C dark_amd/csrc`") from e
         lib = _hip.load()
+        if getattr(mod, "ABI_VERSION", None) != _hip.ABI_VERSION:
+            raise ImportError(f"dark_amd/_bind.so was built for ABI version {getattr(mod, 'ABI_VERSION', None)}, the library has "
+                              f"{_hip.ABI_VERSION}: build it anew with `make -C dark_amd/csrc`")
         mod.init(_hip.DarkHipError, *(C.cast(getattr(lib, n), C.c_void_p).value for n in (
             "dark_qk_norm_rope", "dark_kv_append", "dark_paged_attention", "dark_paged_attention_workspace_bytes",
             "dark_hip_last_error")))

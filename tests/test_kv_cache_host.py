@@ -215,3 +215,17 @@ def test_window_cache_schedule(monkeypatch):
     wc.forward(st, x, 6)
     assert seen[5:] == [40, 40]
     assert kv_cache.WindowCache(model, 2, 20, None, None, 1).forward(st, x, 6) is None and seen[-1] == 40
+
+
+def test_a_binding_of_another_version_is_refused(monkeypatch):
+    import sys
+    from types import SimpleNamespace
+
+    import dark_amd
+    assert kv_cache._ops().ABI_VERSION == _hip.ABI_VERSION
+    for stale in (SimpleNamespace(ABI_VERSION=_hip.ABI_VERSION - 1), SimpleNamespace()):
+        monkeypatch.setattr(kv_cache, "_bind", None)
+        monkeypatch.setattr(dark_amd, "_bind", stale, raising=False)
+        monkeypatch.setitem(sys.modules, "dark_amd._bind", stale)
+        with pytest.raises(ImportError, match="ABI version"):
+            kv_cache._ops()

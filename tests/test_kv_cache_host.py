@@ -229,3 +229,16 @@ def test_a_binding_of_another_version_is_refused(monkeypatch):
         monkeypatch.setitem(sys.modules, "dark_amd._bind", stale)
         with pytest.raises(ImportError, match="ABI version"):
             kv_cache._ops()
+
+
+@pytest.mark.parametrize("goal", ["all", "probes"])
+def test_changed_flags_reach_every_object(goal):
+    """A changed Makefile compiles everything anew: a library of objects with other flags would pass for a built one."""
+    import glob
+    import os
+    import subprocess
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dark_amd", "csrc")
+    plan = subprocess.run(["make", "-C", src, "-n", "-W", "Makefile", goal], check=True, capture_output=True, text=True).stdout
+    for f in glob.glob(os.path.join(src, "*.hip")):
+        assert f"-c {os.path.basename(f)} " in plan, f
+    assert goal != "all" or "bind.cpp -o ../_bind.so" in plan

@@ -137,12 +137,12 @@ class PagedKVCache:
         return out
 
     def free(self, pages) -> None:
-        held = set(self._free)
+        """Gives pages back; ValueError (nothing given back) if one of them is not held or named twice."""
+        pages, gone = [int(p) for p in pages], set(self._free)
         for p in pages:
-            p = int(p)
-            _need(0 <= p < self.n_pages and p not in held, f"page {p} is not held")
-            held.add(p)
-            self._free.append(p)
+            _need(0 <= p < self.n_pages and p not in gone, f"page {p} is not held")
+            gone.add(p)
+        self._free.extend(pages)
 
     def slots(self, block_table: torch.Tensor, seq: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
         """Slot (int64) of token ``index[t]`` of sequence ``seq[t]``; -1 where the table names no page for it."""

@@ -242,3 +242,15 @@ def test_changed_flags_reach_every_object(goal):
     for f in glob.glob(os.path.join(src, "*.hip")):
         assert f"-c {os.path.basename(f)} " in plan, f
     assert goal != "all" or "bind.cpp -o ../_bind.so" in plan
+
+
+def test_pages_are_freed_all_or_none():
+    c = kv_cache.PagedKVCache(1, 6, 16, 1, 64, torch.float32, "cpu")
+    a = c.allocate(64)
+    for bad in ([a[0], a[1], 99], [a[0], a[0]], [a[2], -1], [a[0], 5 - a[0] if 5 - a[0] not in a else 6]):
+        with pytest.raises(ValueError, match="not held"):
+            c.free(bad)
+        with pytest.raises(MemoryError):
+            c.allocate(48)                     # two pages are free, as before
+    c.free(torch.tensor(a))
+    assert sorted(c.allocate(96)) == list(range(6))

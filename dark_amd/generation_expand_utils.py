@@ -148,6 +148,8 @@ class DreamGenerationMixin(_fixed.DreamGenerationMixin):
 
     def _generate_rows(self, rows: List[torch.Tensor], generation_config, single: bool, **kwargs):
         kwargs.pop("tokenizer", None)                                                            # :301
+        if kwargs.pop("cache_interval", 0):
+            raise NotImplementedError("cache_interval serves windows of a fixed length (diffusion_generate_length)")
         noise_fn = kwargs.pop("_noise_fn", None)   # parity tests: (row, step, M_row, V) -> Exp(1) draws
         rank_noise_fn = kwargs.pop("_rank_noise_fn", None)   # parity tests: (row, step, M_row) -> multinomial's draws
         trace = kwargs.pop("_trace", None)         # parity tests: dict receiving per-step M / conf / x0 / rows

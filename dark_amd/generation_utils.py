@@ -228,6 +228,8 @@ class DreamGenerationMixin:
         interval = kwargs.pop("cache_interval", 0) or 0
         if int(interval) != interval or interval < 0:
             raise ValueError(f"cache_interval={interval!r}: a whole number of forwards, 0 = no cache")
+        if interval and not hasattr(self, "forward_cached"):
+            raise NotImplementedError(f"cache_interval: {type(self).__name__} has no cached forward")
         ctx = _LoopCtx(skip_noop=bool(kwargs.pop("skip_noop_steps", True)), cache_interval=int(interval),
                        lazy_noise=bool(kwargs.pop("lazy_noise", True)),
                        noise_fn=kwargs.pop("_noise_fn", None), rand_fn=kwargs.pop("_rand_fn", None),

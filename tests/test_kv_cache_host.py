@@ -254,3 +254,20 @@ def test_pages_are_freed_all_or_none():
             c.allocate(48)                     # two pages are free, as before
     c.free(torch.tensor(a))
     assert sorted(c.allocate(96)) == list(range(6))
+
+
+def test_a_cache_interval_that_is_not_served_is_refused():
+    """The variable-length loop and the GPT-2 backbone say so instead of running without a cache."""
+    from dark_amd import DreamConfig, DreamModel, synth
+    from dark_amd.custom_gpt import DiffusionModel, GPT2DiffusionConfig
+    dream = DreamModel(DreamConfig(vocab_size=512, hidden_size=192, intermediate_size=384, num_hidden_layers=1, num_attention_heads=2,
+                                   num_key_value_heads=2, max_position_embeddings=64, mask_token_id=synth.MASK, pad_token_id=synth.END))
+    gpt2 = DiffusionModel(GPT2DiffusionConfig(vocab_size=512, n_positions=64, n_embd=128, n_layer=1, n_head=2, mask_token_id=synth.MASK))
+    ids = torch.full((1, 8), synth.MASK)
+    for call in (dream.diffusion_generate, gpt2.diffusion_generate, gpt2.diffusion_generate_length):
+        with pytest.raises(NotImplementedError, match="cache_interval"):
+            call(ids, max_length=16, steps=2, alg="entropy", cache_interval=2)
+        with pytest.raises(RuntimeError, match="HIP device"):          # none asked for: as without the argument
+            call(ids, max_length=16, steps=2, alg="entropy", cache_interval=0, expand_token_id=5, eos_token_id=2)
+    with pytest.raises(NotImplementedError, match="cache_interval"):
+        dream.diffusion_generate_batch([ids[0]], max_length=16, cache_interval=4)

@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -65,6 +66,7 @@ struct Call {
   at::ScalarType dt = at::kFloat;
   int64_t es = 4;
   bool grad = c10::GradMode::is_enabled();
+  bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
 
   void open(const at::Tensor& t) {
     if (!t.is_cuda()) throw Refusal(PyExc_RuntimeError, "dark_amd runs on a HIP device only");
@@ -81,6 +83,8 @@ struct Call {
     if (t.dim() != dim) refuse(std::string(name) + " has " + std::to_string(t.dim()) + " dimensions, expected " + std::to_string(dim));
     if (grad && t.requires_grad())
       throw Refusal(PyExc_RuntimeError, std::string(name) + " requires gradients: the cache's operators have no backward (use torch.no_grad())");
+    if (tangents && t._fw_grad(0).defined())
+      throw Refusal(PyExc_RuntimeError, std::string(name) + " carries a forward-mode tangent: the cache's operators have no derivative");
   }
 
   // 16-byte pointer and strides, contiguous last dimension (a dimension of one has no stride of its own)
@@ -97,6 +101,10 @@ struct Call {
     if (!fits(t)) refuse(std::string(name) + ": pointer and strides must be multiples of 16 bytes, the last dimension contiguous");
     for (int64_t i = 0; i + 1 < t.dim(); ++i)
       if (t.size(i) > 1 && t.stride(i) <= 0) refuse(std::string(name) + ": an expanded tensor cannot be written");
+  }
+  // what a call wrote into a tensor of the caller's: autograd refuses to go back through what it saved of it before
+  static void wrote(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   }
   static int64_t stride(const at::Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
 
@@ -218,6 +226,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st = PyLong_AsVoidPtr(a[0]);
     const c10::DeviceGuard guard(c.dev);
     done(f_norm_rope(&p, st));
+    if (a[9] != Py_None) c.wrote(qo);
+    if (a[10] != Py_None) c.wrote(ko);
     PyObject *x = a[9] == Py_None ? THPVariable_Wrap(qo) : (Py_INCREF(a[9]), a[9]);
     PyObject *y = a[10] == Py_None ? THPVariable_Wrap(ko) : (Py_INCREF(a[10]), a[10]);
     PyObject* r = PyTuple_Pack(2, x, y);
@@ -265,7 +275,12 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st = PyLong_AsVoidPtr(a[0]);
     const c10::DeviceGuard guard(c.dev);
     // (empty vectors have no pointer)
-    if (T > 0) done(f_append(&p, st));
+    if (T > 0) {
+      done(f_append(&p, st));
+      c.wrote(*given(a[3], "k_cache"));
+      c.wrote(*given(a[4], "v_cache"));
+      if (qo0) c.wrote(qo);
+    }
     if (!q0) Py_RETURN_NONE;
     if (a[10] != Py_None) return Py_INCREF(a[10]), a[10];
     return THPVariable_Wrap(qo);
@@ -332,7 +347,10 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.workspace = ws.data_ptr();
       p.workspace_bytes = (int64_t)bytes;
     }
-    if (T > 0) done(f_attend(&p, st));
+    if (T > 0) {
+      done(f_attend(&p, st));
+      if (a[13] != Py_None) c.wrote(out);
+    }
     PyObject* o = a[13] == Py_None ? THPVariable_Wrap(out) : (Py_INCREF(a[13]), a[13]);
     if (!want) return o;
     PyObject* l = THPVariable_Wrap(lse);

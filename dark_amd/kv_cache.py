@@ -7,7 +7,8 @@ the whole window in every denoise step.  With a cache a step recomputes only the
 A layer's cache is two tensors ``[n_pages, page_size, n_kv_heads, head_dim]`` (any strides with a contiguous last
 dimension, the same for both); token ``j`` of a sequence lies in slot ``j % page_size`` of page
 ``block_table[b, j // page_size]``.  The functions enqueue on torch's current stream of the tensors' device, never
-synchronise, and have no backward: a tensor that asks for gradients is refused while gradients are enabled.
+synchronise, and have no derivatives: a tensor that asks for gradients is refused while gradients are enabled, one with a
+forward-mode tangent while those are.  What they write counts as written for autograd.
 """
 from __future__ import annotations
 
@@ -211,6 +212,9 @@ def forward_cached(model, cache: PagedKVCache, input_ids: torch.Tensor, seq: tor
         need = lib.dark_forward_cached_workspace_bytes(pk.ref, tokens)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _hip.check(lib.dark_forward_cached(pk.ref, tokens, ws.data_ptr(), need, hidden.data_ptr(), _hip.stream_ptr(dev)))
+    for t in (cache._k, cache._v, hidden):     # (autograd refuses to go back through what it saved of them before)
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
     return hidden
 
 

@@ -287,3 +287,31 @@ def test_refusals():
         m.forward_cached(kv_cache.PagedKVCache(2, 4, 16, 2, 64, torch.float32, DEV), *args, 1)
     with pytest.raises(ValueError, match="dtype"):
         m.forward_cached(kv_cache.PagedKVCache(2, 4, 16, 2, 96, torch.bfloat16, DEV), *args, 1)
+
+
+def test_autograd_knows_of_a_cached_forward():
+    cfg = config(max_position_embeddings=64)
+    m, _ = build(cfg, torch.float32)
+    cache = m.make_cache(16)
+    z = torch.zeros(1, dtype=torch.int64, device=DEV)
+    w = torch.ones_like(cache.k(0), requires_grad=True)
+    cache._k.zero_()
+    y = (w * cache.k(0)).sum()
+    m.forward_cached(cache, z, z, z.int(), torch.zeros(1, 1, dtype=torch.int32, device=DEV), i32(0, 1), i32(1), 1, 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_the_expanding_model_in_windows_of_a_fixed_length():
+    """DreamModel.diffusion_generate_length with a cache is DreamModel_length.diffusion_generate with one."""
+    from dark_amd import DreamModel
+    cfg = config(max_position_embeddings=64)
+    m, _ = build(cfg, torch.float32)
+    d = DreamModel(cfg)
+    d.load_state_dict(m.state_dict(), strict=True)
+    d = d.to(DEV)
+    ids = synth.make_inputs(4, "abd", nentity=300, nrelation=111, seed=4)
+    want, _ = _generate(m, ids, 9, cache_interval=3)
+    d.diffusion_generate = d.diffusion_generate_length
+    got, _ = _generate(d, ids, 9, cache_interval=3)
+    assert torch.equal(got, want)

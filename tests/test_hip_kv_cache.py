@@ -685,3 +685,41 @@ def test_refused_operands():
             att(**kw)
     with pytest.raises(_hip.DarkHipError, match="scale"):
         att(scale=math.nan)
+
+
+def test_autograd_knows_of_the_calls():
+    """Operands with a forward-mode tangent are refused as those that ask for gradients are; what a call writes counts as
+    written, so that a backward pass which saved it before fails instead of using the new values."""
+    import torch.autograd.forward_ad as fw
+    z = lambda *s: torch.randn(s, device=DEV)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    q, k, slots = z(2, 8, 96), z(2, 4, 96), torch.arange(2, device=DEV)
+    kc, vc, table, cu, kv = z(1, 16, 4, 96), z(1, 16, 4, 96), i32(0).view(1, 1), i32(0, 2), i32(2)
+    calls = {"q": [lambda x: kv_cache.qk_norm_rope(x, k, None, None, None, None, None),
+                   lambda x: kv_cache.append_kv(k, k, kc, vc, slots, q=x),
+                   lambda x: kv_cache.paged_attention(x, kc, vc, table, cu, kv, 2, 2)],
+             "k_cache": [lambda x: kv_cache.append_kv(k, k, x, vc, slots), lambda x: kv_cache.paged_attention(q, x, vc, table, cu, kv, 2, 2)]}
+    with fw.dual_level():
+        for name, fs in calls.items():
+            x = {"q": q, "k_cache": kc}[name]
+            for f in fs:
+                with pytest.raises(RuntimeError, match=f"{name} carries a forward-mode tangent"):
+                    f(fw.make_dual(x, torch.ones_like(x)))
+                f(x)
+    for out, f in ((q.clone(), lambda o: kv_cache.qk_norm_rope(q, k, None, None, None, None, None, q_out=o)),
+                   (k.clone(), lambda o: kv_cache.qk_norm_rope(q, k, None, None, None, None, None, k_out=o)),
+                   (kc.clone(), lambda o: kv_cache.append_kv(k, k, o, vc, slots)), (vc.clone(), lambda o: kv_cache.append_kv(k, k, kc, o, slots)),
+                   (q.clone(), lambda o: kv_cache.append_kv(k, k, kc, vc, slots, q=q, q_out=o)),
+                   (q.clone(), lambda o: kv_cache.paged_attention(q, kc, vc, table, cu, kv, 2, 2, out=o))):
+        w = torch.ones_like(out, requires_grad=True)
+        y = (w * out).sum()                                   # saves `out` for w's gradient
+        f(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    before = q._version, k._version                           # inputs are not written
+    kv_cache.paged_attention(q, kc, vc, table, cu, kv, 2, 2)
+    kv_cache.append_kv(k, k, kc, vc, slots, q=q)
+    assert (q._version, k._version) == before
+    with torch.inference_mode():
+        o = torch.empty_like(q)
+        assert kv_cache.paged_attention(q, kc, vc, table, cu, kv, 2, 2, out=o) is o

@@ -39,6 +39,16 @@ template <> struct AttnVec<bf16_t> {
   }
 };
 
+// The rotation of one pair (element e of a 16-byte piece).  Which products are fused into a multiply-add is written out element
+// by element: loops are compared with recorded ones token for token, and left to the compiler that choice goes with its flags.
+template <bool F32, bool HOIST>
+__device__ __forceinline__ void rotate(int e, float x1, float x2, float c, float s, float& o1, float& o2) {
+#pragma clang fp contract(off)
+  const bool fuse1 = F32 ? e < 2 : HOIST ? e != 1 : e < 6, fuse2 = F32 ? e < 2 : HOIST ? e == 0 : e < 6;
+  o1 = fuse1 ? __builtin_fmaf(x1, c, -(x2 * s)) : x1 * c - x2 * s;
+  o2 = fuse2 ? __builtin_fmaf(x2, c, x1 * s) : x2 * c + x1 * s;
+}
+
 template <typename T, int HD, int NT, int NW, bool HOIST = false>
 __global__ __launch_bounds__(NW * 64) void attn_kernel(const T* __restrict__ qkv, const float* __restrict__ cosT,
                                                    const float* __restrict__ sinT,
@@ -114,8 +124,9 @@ __global__ __launch_bounds__(NW * 64) void attn_kernel(const T* __restrict__ qkv
       const float ss[8] = {sn[u][0].x, sn[u][0].y, sn[u][0].z, sn[u][0].w, sn[u][1].x, sn[u][1].y, sn[u][1].z, sn[u][1].w};
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        o1[e] = t < N ? x1[e] * cc[e] - x2[e] * ss[e] : 0.f;
-        o2[e] = t < N ? x2[e] * cc[e] + x1[e] * ss[e] : 0.f;
+        rotate<false, true>(e, x1[e], x2[e], cc[e], ss[e], o1[e], o2[e]);
+        o1[e] = t < N ? o1[e] : 0.f;
+        o2[e] = t < N ? o2[e] : 0.f;
       }
       T* dst = (which ? Ks : Qs) + t * LD + c * VEC;
       *(raw_t*)dst = AttnVec<T>::pack(o1);
@@ -151,11 +162,7 @@ __global__ __launch_bounds__(NW * 64) void attn_kernel(const T* __restrict__ qkv
       const float* cp = cosT + (int64_t)p * HALF + c * VEC;
       const float* sp = sinT + (int64_t)p * HALF + c * VEC;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float cs = cp[e], sn = sp[e];
-        o1[e] = x1[e] * cs - x2[e] * sn;
-        o2[e] = x2[e] * cs + x1[e] * sn;
-      }
+      for (int e = 0; e < VEC; ++e) rotate<kF32, false>(e, x1[e], x2[e], cp[e], sp[e], o1[e], o2[e]);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o1[e] = o2[e] = 0.f;

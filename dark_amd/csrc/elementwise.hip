@@ -20,6 +20,13 @@ __global__ __launch_bounds__(256) void embed_kernel(const int64_t* __restrict__ 
   for (int c = lane * 4; c < d; c += 256) store4<TH>(dst + c, load4<TW>(src + c));
 }
 
+// ss + the squares of four elements, each rounded before it is added: written out, because left to the compiler which products
+// are fused into multiply-adds goes with its flags, and fp32 loops are compared with recorded ones token for token
+__device__ __forceinline__ float add_squares(float ss, const float4 v) {
+#pragma clang fp contract(off)
+  return ss + (v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w);
+}
+
 // Embedding + the first layer's input RMSNorm in one pass (d <= 1024): the gathered row is already in registers, so
 // xn = weight * row / rms(row) costs no second read of the 4*d-byte fp32 row.  Arithmetic and summation order are
 // rmsnorm_kernel's.
@@ -45,7 +52,7 @@ __global__ __launch_bounds__(256) void embed_norm_kernel(const int64_t* __restri
   float ss = 0.f;
 #pragma unroll
   for (int p = 0; p < 4; ++p)
-    if (lane * 4 + p * 256 < d) ss += v[p].x * v[p].x + v[p].y * v[p].y + v[p].z * v[p].z + v[p].w * v[p].w;
+    if (lane * 4 + p * 256 < d) ss = add_squares(ss, v[p]);
   ss = wave_sum(ss);
   const float r = 1.0f / sqrtf(ss / (float)d + eps);
 #pragma unroll
@@ -132,7 +139,7 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const TH* __restrict__ x,
     float ss = 0.f;
 #pragma unroll
     for (int p = 0; p < 4; ++p)
-      if (lane * 4 + p * 256 < d) ss += v[p].x * v[p].x + v[p].y * v[p].y + v[p].z * v[p].z + v[p].w * v[p].w;
+      if (lane * 4 + p * 256 < d) ss = add_squares(ss, v[p]);
     ss = wave_sum(ss);
     const float r = 1.0f / sqrtf(ss / (float)d + eps);
 #pragma unroll
@@ -143,7 +150,7 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const TH* __restrict__ x,
   float ss = 0.f;
   for (int c = lane * 4; c < d; c += 256) {
     const float4 v = load4<TH>(xr + c);
-    ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+    ss = add_squares(ss, v);
   }
   ss = wave_sum(ss);
   const float r = 1.0f / sqrtf(ss / (float)d + eps);

@@ -271,3 +271,16 @@ def test_a_cache_interval_that_is_not_served_is_refused():
             call(ids, max_length=16, steps=2, alg="entropy", cache_interval=0, expand_token_id=5, eos_token_id=2)
     with pytest.raises(NotImplementedError, match="cache_interval"):
         dream.diffusion_generate_batch([ids[0]], max_length=16, cache_interval=4)
+
+
+def test_no_source_is_compiled_with_packed_fp32():
+    """hipcc makes v_pk_{add,mul,fma}_f32 of ordinary float code unless it is told not to, some forms of which have given wrong
+    results on this card: every compile line of the library says so."""
+    import os
+    import subprocess
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dark_amd", "csrc")
+    plan = subprocess.run(["make", "-C", src, "-n", "-W", "Makefile", "all", "probes"], check=True, capture_output=True, text=True).stdout
+    lines = [x for x in plan.splitlines() if ".hip -o" in x]
+    assert len(lines) >= 13
+    for x in lines:
+        assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in x, x

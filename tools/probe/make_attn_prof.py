@@ -34,7 +34,8 @@ rep('}  // namespace dark', '}  // namespace dark\nextern "C" int dark_dbg_attn_
 os.makedirs(os.path.join(CSRC, "build"), exist_ok=True)
 open(os.path.join(CSRC, "build", "attn_prof.hip"), "w").write(src)
 hipcc = "/opt/rocm/bin/hipcc"
-subprocess.check_call([hipcc, "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-I.", "-I../../include", "-c",
+subprocess.check_call([hipcc, "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Xclang", "-target-feature",
+                       "-Xclang", "-packed-fp32-ops", "-I.", "-I../../include", "-c",
                        "build/attn_prof.hip", "-o", "build/attn_prof.o"], cwd=CSRC)
 objs = [f"build/{n}.o" for n in ("api", "gemm", "elementwise", "sample", "expand", "grpo", "layout")] + ["build/attn_prof.o"]
 subprocess.check_call([hipcc, "-shared", "-fPIC", "--offload-arch=gfx950", *objs, "-o", "../libdark_hip_prof.so"], cwd=CSRC)

@@ -60,8 +60,10 @@ rep('}  // namespace dark\n', '}  // namespace dark\nextern "C" int dark_dbg_sam
 os.makedirs(os.path.join(CSRC, "build"), exist_ok=True)
 open(os.path.join(CSRC, "build", "sample_prof.hip"), "w").write(src)
 hipcc = "/opt/rocm/bin/hipcc"
-subprocess.check_call([hipcc, "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-I.", "-I../../include", "-c",
+subprocess.check_call([hipcc, "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Xclang", "-target-feature",
+                       "-Xclang", "-packed-fp32-ops", "-I.", "-I../../include", "-c",
                        "build/sample_prof.hip", "-o", "build/sample_prof.o"], cwd=CSRC)
-objs = [f"build/{n}.o" for n in ("api", "gemm", "gemm256", "gemm_rowpanel", "attn", "elementwise", "expand", "grpo", "layout", "gpt2")] + ["build/sample_prof.o"]
+objs = [f"build/{n}.o" for n in ("api", "gemm", "gemm256", "gemm_rowpanel", "attn", "elementwise", "expand", "grpo", "layout", "gpt2",
+                                  "kv_cache", "paged_attn")] + ["build/sample_prof.o"]
 subprocess.check_call([hipcc, "-shared", "-fPIC", "--offload-arch=gfx950", *objs, "-o", "../libdark_hip_prof.so"], cwd=CSRC)
 print("built dark_amd/libdark_hip_prof.so")

@@ -2,7 +2,7 @@
 // (two waves each, independent accumulators, operands with random mantissas), 16x16x32 against 32x32x16: same MACs per
 // second at the same clock, half the operand-register reads per MAC for the larger shape.  Prints the achieved rate;
 // run it beside `rocm-smi --showclocks --showpower` (tools/probe/mfma_clock_probe.sh).
-// Build: hipcc -O3 --offload-arch=gfx950 tools/probe/mfma_clock_probe.hip -o tools/probe/mfma_clock_probe
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/mfma_clock_probe.hip -o tools/probe/mfma_clock_probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

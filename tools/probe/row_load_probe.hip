@@ -1,6 +1,6 @@
 // Micro-benchmark behind the sampler's row-load phase: how fast can one workgroup per row
 // bring a [M, V] fp32 matrix through the CU, as a function of LDS footprint, persistence and prefetch.
-// Build: hipcc -O3 --offload-arch=gfx950 row_load_probe.hip -o row_load_probe ; run: ./row_load_probe [M] [V]
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops row_load_probe.hip -o row_load_probe ; run: ./row_load_probe [M] [V]
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -4,7 +4,7 @@
 // double-buffered in registers (the reads of K-tile t+1 and the DMA of K-tile t+NB are issued between the MFMAs of
 // K-tile t).  Purpose: measure what this structure costs per K-tile BEFORE it is built into the library, against the
 // two-waves-per-SIMD kernel that runs today (gemm_bf16_s256: 925 - 1030 ns per 320 x 256 x 32 K-tile).
-// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 w4_probe.hip -o w4_probe ; run: ./w4_probe [M] [N] [K]
+// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops w4_probe.hip -o w4_probe ; run: ./w4_probe [M] [N] [K]
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <cstdint>

@@ -1172,6 +1172,8 @@ static int check_paged_attention(const dark_paged_attention_args* p) {
   DARK_CHECK_ARG((int64_t)p->table_width * p->kv.page_size < (1ll << 30) && p->max_kv < (1 << 30), "%s: 2^30 keys a sequence or more", who);
   const int64_t G = p->n_heads / p->kv.n_kv_heads;
   DARK_CHECK_ARG(p->n_tokens * G < (1ll << 31) - 128 && p->max_q * G < (1ll << 31) - 128, "%s: 2^31 rows of a key head or more", who);
+  // (far beyond what a call is refused for; below, the plan's products of them stay within 64 bits)
+  DARK_CHECK_ARG((double)p->n_seqs * p->kv.n_kv_heads * ((double)p->max_q * G / 16 + 1) < 1e12, "%s: too many rows", who);
   DARK_CHECK_ARG(p->scale == p->scale && fabsf(p->scale) < INFINITY, "%s: scale is not finite", who);
   return DARK_OK;
 }

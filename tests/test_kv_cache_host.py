@@ -284,3 +284,20 @@ def test_no_source_is_compiled_with_packed_fp32():
     assert len(lines) >= 13
     for x in lines:
         assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in x, x
+
+
+@pytest.mark.parametrize("dtype", [_hip.DARK_F32, _hip.DARK_BF16])
+def test_sizes_beyond_any_call_are_refused(dtype):
+    """Products of the largest sizes that the fields hold: an error, no division by a product that wrapped round to 0."""
+    lib = _hip.load()
+    kv = _kv(dtype=dtype, n_kv_heads=4096, head_dim=64, slot_stride=64, head_stride=1024, page_stride=1024 * 4096)
+    a = _hip.PagedAttentionArgs(kv=kv, q=4096, out=8192, block_table=4096, cu_q=4096, kv_len=4096, o_ts=64 * 4096, q_ts=64 * 4096, q_hs=64,
+                                o_hs=64, n_tokens=1, n_heads=4096, n_seqs=1 << 30, table_width=64, table_stride=64, max_q=1 << 30, max_kv=1000,
+                                scale=0.1)
+    assert lib.dark_paged_attention_workspace_bytes(C.byref(a)) == 0
+    _refused("dark_paged_attention", a, "too many rows")
+    for big in (dict(max_q=1 << 30, n_seqs=1), dict(max_q=1, n_seqs=1 << 30), dict(max_q=1 << 20, n_seqs=1 << 20), dict(max_q=(1 << 31) - 200, n_seqs=(1 << 31) - 1)):
+        for k, v in big.items():
+            setattr(a, k, v)
+        lib.dark_paged_attention_workspace_bytes(C.byref(a))
+        assert lib.dark_paged_attention(C.byref(a), None) == _hip.DARK_ERR_ARG

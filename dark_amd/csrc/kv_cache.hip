@@ -295,6 +295,7 @@ int dark_kv_append(const dark_kv_append_args* p, void* stream) {
   if (p->n_tokens == 0) return DARK_OK;
   const int es = p->kv.dtype == DARK_BF16 ? 2 : 4;
   DARK_CHECK_ARG(p->k && p->v && p->slots, "%s: null pointer", who);
+  DARK_CHECK_ARG(p->kv.n_pages == 0 || p->kv.k != p->kv.v, "%s: k and v would go to the same memory", who);
   DARK_CHECK_ARG((p->q == nullptr) == (p->q_out == nullptr) && (p->n_heads == 0 || p->q), "%s: q and q_out go together", who);
   DARK_CHECK_ARG((p->rope_cos == nullptr) == (p->rope_sin == nullptr), "%s: rope_cos and rope_sin go together", who);
   DARK_CHECK_ARG(!p->rope_cos || (p->pos && p->max_pos >= 1), "%s: a rotation needs positions and a table", who);

@@ -77,6 +77,12 @@ def test_paged_attention_refuses(kw, msg):
     _refused("dark_paged_attention", _hip.PagedAttentionArgs(**f), msg)
 
 
+def test_keys_and_values_into_one_cache_are_refused():
+    """Two rows for every slot: whichever came last would stay."""
+    f = dict(kv=_kv(v=4096), k=4096, v=4096, slots=4096, k_ts=768, k_hs=96, v_ts=768, v_hs=96, n_tokens=3, max_pos=64, eps=1e-6)
+    _refused("dark_kv_append", _hip.KVAppendArgs(**f), "same memory")
+
+
 def test_null_arguments():
     for fn in ("dark_qk_norm_rope", "dark_kv_append", "dark_paged_attention"):
         _refused(fn, None, "null arguments")

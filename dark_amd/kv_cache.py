@@ -20,7 +20,6 @@ import torch
 from . import _hip
 
 _DTYPES = {torch.float32: _hip.DARK_F32, torch.bfloat16: _hip.DARK_BF16}
-_raw_stream = torch._C._cuda_getCurrentRawStream          # hipStream_t of torch's current stream on a device
 _bind = None
 
 
@@ -44,8 +43,9 @@ def _ops():
 
 
 def _stream(t: torch.Tensor) -> int:
+    """hipStream_t of torch's current stream on the tensor's device."""
     dev = t.get_device()
-    return _raw_stream(dev) if dev >= 0 else 0
+    return torch._C._cuda_getCurrentRawStream(dev) if dev >= 0 else 0
 
 
 def _need(cond: bool, msg: str) -> None:

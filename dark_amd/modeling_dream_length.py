@@ -112,7 +112,7 @@ class PackedWeights:
             lw.w_down = dev(_pad_rows(sd[p + "mlp.down_proj.weight"])).data_ptr()
             lw.ln1 = dev(sd[p + "input_layernorm.weight"], torch.float32).data_ptr()
             lw.ln2 = dev(sd[p + "post_attention_layernorm.weight"], torch.float32).data_ptr()
-            if cfg.qk_norm:
+            if getattr(cfg, "qk_norm", False):
                 lw.q_norm = dev(sd[a + "q_norm.weight"], torch.float32).data_ptr()
                 lw.k_norm = dev(sd[a + "k_norm.weight"], torch.float32).data_ptr()
         head = _pad_rows(sd["lm_head.weight"])
@@ -405,7 +405,7 @@ class _Base(nn.Module):
     def __init__(self, cfg: DreamConfig):
         super().__init__()
         self.embed_tokens = _Weight(cfg.vocab_size, cfg.hidden_size)
-        self.layers = nn.ModuleList([_Layer(cfg.hidden_size, cfg.intermediate_size, cfg.head_dim if cfg.qk_norm else 0)
+        self.layers = nn.ModuleList([_Layer(cfg.hidden_size, cfg.intermediate_size, cfg.head_dim if getattr(cfg, "qk_norm", False) else 0)
                                      for _ in range(cfg.num_hidden_layers)])
         self.norm = _Weight(cfg.hidden_size)
 

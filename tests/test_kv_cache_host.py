@@ -307,3 +307,21 @@ def test_sizes_beyond_any_call_are_refused(dtype):
             setattr(a, k, v)
         lib.dark_paged_attention_workspace_bytes(C.byref(a))
         assert lib.dark_paged_attention(C.byref(a), None) == _hip.DARK_ERR_ARG
+
+
+def test_what_knows_nothing_of_the_cache_still_works():
+    """The package imports beside a torch without a HIP runtime's bindings; a config object of the caller's own, without the
+    field of the per-head norms, makes a model."""
+    import os
+    import subprocess
+    import sys
+    from types import SimpleNamespace
+
+    from dark_amd import DreamConfig, DreamModel_length
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = "import torch; del torch._C._cuda_getCurrentRawStream; import dark_amd; dark_amd.DreamConfig()"
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root)
+    cfg = DreamConfig(vocab_size=512, hidden_size=192, intermediate_size=384, num_hidden_layers=1, num_attention_heads=2,
+                      num_key_value_heads=2, max_position_embeddings=64)
+    other = SimpleNamespace(**cfg.__dict__, head_dim=cfg.head_dim, to_dict=cfg.to_dict)
+    assert set(DreamModel_length(other).state_dict()) == set(DreamModel_length(cfg).state_dict())

@@ -83,7 +83,7 @@ struct Call {
     if (t.dim() != dim) refuse(std::string(name) + " has " + std::to_string(t.dim()) + " dimensions, expected " + std::to_string(dim));
     if (grad && t.requires_grad())
       throw Refusal(PyExc_RuntimeError, std::string(name) + " requires gradients: the cache's operators have no backward (use torch.no_grad())");
-    if (tangents && t._fw_grad(0).defined())
+    if (tangents && (type == at::kFloat || type == at::kBFloat16) && t._fw_grad(0).defined())   // (whole numbers have none)
       throw Refusal(PyExc_RuntimeError, std::string(name) + " carries a forward-mode tangent: the cache's operators have no derivative");
   }
 

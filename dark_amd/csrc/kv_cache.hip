@@ -7,8 +7,8 @@
 // pair in one lane -- so the 64 / LPR rows of a pass need no exchange but the norm's sum (log2(LPR) xor-shuffles).  A wave
 // keeps its pass (which heads, hence its pointers, strides and weights) and walks over the tokens, the next one's rows,
 // rotation and, one further, position on their way while it computes.  Read and written, each time other inputs: 16383 tokens
-// x 40 fp32 heads of 128 in 120.5 us (5.6 TB/s), 512 x 46 x 16 bf16 heads of 96 in 36 us (4.0; a copy of as much takes 28.7),
-// 1024 x 11 x 24 such heads into their pages in 22 us (4.7), 8 x up to 4096 x 48 bf16 heads of 128 with norms in 118 us (5.5);
+// x 40 fp32 heads of 128 in 121 us (5.6 TB/s), 512 x 46 x 16 bf16 heads of 96 in 34.7 us (4.2; a copy of as much takes 28.7),
+// 1024 x 11 x 24 such heads into their pages in 21.7 us (4.8), 8 x up to 4096 x 48 bf16 heads of 128 with norms in 115 us (5.7);
 // one token in 2.4 us.  Rows two tokens ahead instead of one: 39.7 us for 38.5, registers cost a wave.
 #include "common.h"
 
@@ -216,15 +216,15 @@ static int launch_head_rows(RowsArgs& a, int dtype, int HD, hipStream_t st) {
   const int ch = HD / 2 / (dtype == DARK_BF16 ? 8 : 4), rpp = 64 / (ch <= 4 ? 4 : ch <= 8 ? 8 : 16);
   a.n_pass = cdiv(a.h_end[2], rpp);
   // Tokens a wave walks over: some 32768 waves in all, so that the card sweeps over the tokens in order (8 x up to 4096, 48 heads:
-  // 117 us; 120 with 16384 waves, 134 with 8192, 157 with 4096), but two at least where there are enough and weights to fetch
-  // first (512 x 46: 36.9 us, 39.6 with one or two)
+  // 116 us; 119 with 16384 waves, 135 with 8192), but two at least where there are enough and weights to fetch first (512 x 46:
+  // 34.8 us, 39.8 with one, 36.1 with three)
   const bool norm = a.w[0] || a.w[1];
   const int64_t units = (int64_t)a.T * a.n_pass;
   int64_t walk = norm && units >= 16384 ? 2 : 1;
   if (walk < (units + 16384) / 32768) walk = (units + 16384) / 32768;
   a.t_step = (int)((a.T + walk - 1) / walk);
   // rows that the 256 MB behind the L2s cannot hold for their reader are written past them (16383 tokens x 40 fp32 heads of
-  // 128, 0.7 GB moved: 129 us, 139 without; 512 x 46 x 16 bf16 heads of 96, 72 MB: 38.7 and 40.5, but then they are there to
+  // 128, 0.7 GB moved: 120 us, 129 without; 512 x 46 x 16 bf16 heads of 96, 72 MB: 31.0 and 34.8, but then they are there to
   // be read)
   const bool past = (int64_t)a.T * a.h_end[2] * HD * (dtype == DARK_BF16 ? 2 : 4) > (int64_t)256 << 20;
   const dim3 grid((unsigned)cdiv(a.t_step * a.n_pass, 4)), block(256);

@@ -279,9 +279,9 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const Unit<RT>& u
 // keys that is read once.  Bound by HBM; what counts is bytes in flight, so every wave streams tiles of its own -- tile t's
 // successor is on its way into the registers t is done with, the pages of the one behind it are looked up -- and waits for
 // nobody.  K and V rows are read whole (16 lanes a row of 256 bytes) and turned into operands by way of LDS of the wave's
-// own: read from memory as the first product wants them, 64 bytes of each of 16 rows an instruction, every line is asked for
-// twice (64 x 1 over up to 16384: 518 us so, 435 whole, 399 = 6.2 TB/s whole and past the caches, see NT; a plain stream of
-// such rows reads 6.0 and 6.8 TB/s).  Two waves a SIMD: 502 us with three, 522 with one.
+// own: read from memory as the first product wants them, 64 bytes of each of 16 rows an instruction, they come slower (64 x 1
+// over up to 16384, 32 heads on 8 of 128: 518 us so, 439 whole, 401 = 6.1 TB/s whole and past the caches, see NT; a plain stream
+// of such rows reads 6.0 and 6.8 TB/s).  Two waves a SIMD: 502 us with three, 522 with one.
 // WPP waves share one problem (tiles dealt out in turn, joined in LDS at the end); WPP = 1: four problems a workgroup.
 template <int HD, int WPP, bool ODD, bool NT>
 __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_few_kernel(const PagedArgs a) {
@@ -485,10 +485,12 @@ __global__ __launch_bounds__(WPP == 8 ? 512 : 256, HD == 64 ? 3 : 2) void paged_
 // ---- fp32: the same stream for any number of rows, 16 a workgroup, on 16 x 16 x 4 fp32 matrix instructions; nothing passes
 // through LDS.  The output's columns are dealt to the second product's rows so that a lane reads a V row's 16 bytes at
 // 64 c + 4 (lane & 15) -- 16 lanes a whole row piece -- and its four (HD 96: the last two) floats go to four instructions.
-// 16 sequences of 9 to 128 new tokens over 31 to 512 keys, 12 heads of 64: 23.4 - 25 us, 29 TFLOP/s; the SIMDs that get the
+// 16 sequences of 9 to 128 new tokens over 31 to 512 keys, 12 heads of 64: 24 us, 29 TFLOP/s; the SIMDs that get the
 // long sequences' rows work twice as long as the average.  (Eight waves a problem: 28.5 us; one: 47.)  Long chunks (4 x 1024
-// over 9216, head_dim 128) 104 TFLOP/s of the 152 that a large fp32 product reaches: the softmax's vector instructions and the
-// matrix instructions of two or three waves overlap only in part.
+// over 9216, head_dim 128) 118 TFLOP/s of the 152 that a large fp32 product reaches: a read of K and V serves the wave's 32 rows
+// alone (16 for heads of 64), 16 flops a byte, so that 7.4 TB/s of them go into registers, beside the softmax's vector
+// instructions, which overlap with the matrix instructions of two or three waves only in part.  Single tokens over long
+// contexts are bound by HBM (64 x 1 over up to 16384, 32 heads on 8 of 128: 812 us, 6.1 TB/s, every byte fetched once).
 template <int HD, int WPP, int RT, bool ODD>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const PagedArgs a) {
   constexpr int NC = HD / 16, KEYS = 16, NV = (HD + 63) / 64;   // NV: pieces of a V row a lane reads
@@ -695,8 +697,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void paged_f32_kernel(const 
 // LDS rows are not padded (the direct writes are linear), their 16-byte chunks are permuted instead: by the row's number,
 // so that the 16 rows a K read touches at once, and the 4 rows of a transposed V read, lie in different banks.
 // Bound by matrix and vector instructions in turn: 32 and some 220 of them for 32 x 64 scores of head_dim 128, two waves a SIMD.
-// 4 x 1024 tokens over 9216, 8 key heads of 128, groups of 4: 640 us, 970 TFLOP/s (causal 617 us, 947); head_dim 96 375 us, 926;
-// 64 379 us, 815; over up to 17408, ragged, 523 us, 900.  The next tile's first product between this tile's exponentials (by
+// 4 x 1024 tokens over 9216, 8 key heads of 128, groups of 4: 668 us, 926 TFLOP/s (causal 626 us, 933); head_dim 96 527 us, 880;
+// 64 388 us, 797; over up to 17408, ragged, 525 us, 896.  The next tile's first product between this tile's exponentials (by
 // scheduling groups, by source order): 841 and 920 TFLOP/s, the other wave of the SIMD fills those gaps already.
 template <int HD> struct TileSwz {
   static constexpr int CH = HD / 8;   // chunks of a row
@@ -717,8 +719,8 @@ template <int HD> struct TileSwz {
 constexpr int TT_ROWS = 128, TT_KEYS = 64;
 
 // The sequence with the n-th most keys (of 64 at most, a lane each): the longest begin first and the shortest
-// fill up what is left (24 x up to 200 over up to 6200: 190 us, 235 in the batch's order; 12 x up to 400 over up to
-// 10400, 240 and 292; ordered by rows times keys 238 and 282: a workgroup has 128 rows whatever the sequence has).
+// fill up what is left (32 heads on 8 of 128: 24 x up to 200 over up to 6200 180 us, 238 in the batch's order; 12 x up to
+// 400 over up to 10400 302 and 365.  Not by rows times keys: a workgroup has 128 rows whatever the sequence has).
 __device__ __forceinline__ int nth_longest(const PagedArgs& a, int n, int lane) {
   const int len = lane < a.B ? seq_len(a, lane) : -1;
   int ahead = 0;   // longer sequences, or as long ones before it
@@ -745,7 +747,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedArgs a) {
   if (id < 0 || id >= a.n_units) return;
   int rest = a.by_tiles.divmod(id);
   const int tile = a.n_tiles - 1 - id;                // (the tiles of a key head read the same keys; the last see most and come
-                                                      // first: 2 chunks of 4096 tokens, causal, 343 -> 302 us)
+                                                      // first: 2 chunks of 4096 tokens, causal, 343 us otherwise, 312)
   id = a.by_split.divmod(rest);
   const int split = rest;
   int b = a.by_hk.divmod(id);
@@ -1086,20 +1088,20 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   s.rt = 1;
   if (p->kv.dtype == DARK_F32) {
     // A wave a problem where keys are few, or problems many: four waves of a workgroup then read the same keys, and nothing is
-    // joined (634 x up to 42 over up to 247, 4 key heads of 128: 403 us, 511 with four waves a problem; 116 x up to 349 over up to
-    // 353: 536 and 725; 21 x up to 346 over up to 531, 7308 problems: 162 and 131 the other way).
-    // 32 rows a wave where they are there and dims enough to be worth it (4 x 512 over 2048, 8 key heads of 128: 652 us, 840 with
-    // 16; of 96, 8 x 512 over 2048: 275 and 310; 12 heads of 64, 64 x 40 over 440: 77 and 62).
+    // joined (16 heads on 4 of 128: 634 x up to 42 over up to 247 303 us, 322 with four waves a problem; 116 x up to 349 over up to
+    // 353 322 and 436; 12 heads of 64, 21 x up to 346 over up to 531: 69 and 54 the other way).
+    // 32 rows a wave where they are there and dims enough to be worth it (4 x 512 over 2048, 32 heads on 8 of 128: 653 us, 811 with
+    // 16; 8 of 96, 8 x 512 over 2048: 289 and 358; 12 heads of 64, 64 x 40 over 440: 76 and 62 the other way).
     const int64_t problems = heads * ((rows + 15) / 16);
     const bool many = problems >= 8192 && p->max_kv <= 2048 && p->kv.head_dim > 64 && rows > 16;
     s.few = p->max_kv <= 128 || (p->max_kv <= 256 && problems >= 1024) || many ? 1 : 4;
     if (rows > 16 && p->kv.head_dim > 64 && (s.few == 4 || (many && p->max_kv > 256))) s.rt = 2;
   }
-  else if (rows <= 16 || (rows <= 48 && p->max_kv <= 128)) {   // (512 x 46 over 46, 8 heads of 96: 41.9 us, 45.6 by row tiles;
-                                                               // 64 x 8 over 2000, 32 rows: 160 and 98.5 the other way)
+  else if (rows <= 16 || (rows <= 48 && p->max_kv <= 128)) {   // (512 x 46 over 46, 8 heads of 96: 42.3 us, 44.6 by row tiles;
+                                                               // 64 x 8 over 2000, 32 rows: 160 and 88 the other way)
     // Waves a problem: one where keys are few, eight where CUs are left over and the axis is short (16 x 1 over 900, 8 heads of
-    // 128: 14.6 us, 17.7 with four; over 1900: 29.3, 24.2 with four and a join; 12 heads of 64 over 1900: 15.2 and 24.0;
-    // 256 problems: 18.7 and 18.2)
+    // 128: 20.1 us, 21.2 with four; over 1900: 32.4, 29.8 with four and a join; 12 heads of 64 over 1900: 22.2 and 25.8;
+    // 256 problems, 32 x 1 over 900: 27.4 and 23.5)
     const bool wide = heads <= 192 && p->max_kv <= (p->kv.head_dim == 64 ? 2048 : 1024);
     s.few = p->max_kv <= 128 ? 1 : wide ? 8 : 4;
   }
@@ -1107,20 +1109,22 @@ static PagedPlan plan_paged(const dark_paged_attention_args* p) {
   s.n_tiles = (int)((rows + tile_rows - 1) / tile_rows);
   if (s.n_tiles < 1) s.n_tiles = 1;
   const int64_t wgs = (int64_t)s.n_tiles * heads;
-  // Parts of a key axis.  Few problems: 512 of them fill the card once (2 x 4 over 131072, 16 problems: 166 us; 172 with 1024
-  // parts, 184 with 768, 183 with 2048), 1024 where key heads have several row tiles, of which shorter sequences lack some (6 x
-  // up to 366 over up to 38700, 8 key heads: 239 us, 339 with 512; 4 x up to 334 over up to 12305, 32 heads of 64: 177, 287 whole,
-  // 168 and 164 with 2048 and 4096, but 8 x up to 512 over up to 4512 168, 228 and 250; 8 x 64 over 8064, one tile: 84 and 78 the
-  // other way), and of 2048 keys at most where those are longer, as far as 4096 parts go (18 x up to 200 over up to 36946: 161 us,
-  // 294 without; 11 x up to 142 over up to 25082 210 and 303; but 2 x up to 300 over up to 60300 718 and 691).  Many
-  // with one row tile a key head, as with one token for each of many sequences: parts of 1024 keys, because lengths differ and the longest must not finish
-  // alone (64 x 1 over 16384: 404 us; 425 with parts of 512, 404 with 2048, 417 with 4096), of 512 where the card would be filled
-  // twice at most (32 x 1 over 1900: 31.2 us, 35.7 with parts of 1024); many row tiles in fp32 as far as 4096 parts go, or else
-  // what is joined grows with tokens times keys (4 x 1024 over 9216, 8 key heads of 128: 4.93 ms whole, 5.75 in 9 parts; 1 x
-  // 1500 over 20000, 8 heads of 96: 1.20 and 0.96 in 10).  Never below 256 keys (a part's (O, m, l) is then 1/16 of the keys'
-  // bytes at most for 16 rows, 1/2 for the 128 of a row tile), nor below 1024 for the many rows of one sequence, all there (1 x 643 over 645, 32 heads of 64: 17.9
-  // us, 30 in three parts; 1 x 1024 over 8024: 57.8 and 68.7; but 4 x up to 199 over up to 1559: 31.6, 22.9 with parts of 256);
-  // none where there are no more than 512 (5 x 279 over 284: 14.5 us, 20.9 in two parts).
+  // Parts of a key axis (8 key heads of 128 where nothing else is said; "up to": ragged).  Few problems: 512 of them fill the
+  // card once (2 x 4 over 131072, 16 problems: 180 us in 32 parts; 191 in 24, 185 in 48, 189 in 64), 1024 where key heads have
+  // several row tiles, of which shorter sequences lack some (8 x up to 512 over up to 4512: 105 us in 4 parts, 120 whole, 120 in 8;
+  // 8 x 64 over 8064, one tile: 71 and 59 the other way), and of 2048 keys at most where those are longer, as far as 4096 parts
+  // go (11 x up to 142 over up to 25082: 155 us, 185 without, 612 whole; 6 x up to 366 over up to 38700 307, 960 whole; 4 x up to 334
+  // over up to 12305, 32 heads of 64, 119, 139 without, 213 whole; but 18 x up to 200 over up to 36946 381 and 363, 2 x up to
+  // 300 over up to 60300 250 and 231).  Many with one row tile a key head, as with one token for each of many sequences: parts
+  // of 1024 keys, because lengths differ and the longest must not finish alone (64 x 1 over up to 16384: 403 us; 425 with parts
+  // of 512, 405 with 2048, 417 with 4096, 477 whole), of 512 where the card would be filled twice at most (32 x 1 over up to 4000:
+  // 56.6 us, 62.4 with parts of 1024, 59.6 whole; but equal lengths would rather stay whole: 32 x 1 over 1900 48.7 and 42.7); many
+  // row tiles in fp32 as far as 4096 parts go, or else what is joined grows with tokens times keys (4 x 1024 over 9216: 4.95 ms
+  // whole, 5.78 in 9 parts; 1 x 1500 over 20000, 8 heads of 96: 1.21 and 0.97 in 10).  Never below 256 keys (a part's (O, m, l) is
+  // then 1/16 of the keys' bytes at most for 16 rows, 1/2 for the 128 of a row tile), nor below 1024 for the many rows of one
+  // sequence, all there (1 x 643 over 645, 32 heads of 64: 16.9 us, 29.6 in three parts; 1 x 1024 over 8024: 61.8 and 73.1; but 4 x
+  // up to 199 over up to 1559: 27.0, 32.9 in two parts of 832); none where there are no more than 512 (5 x 279 over 284: 14.7
+  // us, 22.8 in two parts).
   int64_t keys = p->max_kv;
   if ((s.few == 0 || s.few == 4) && p->max_kv > 512) {
     const bool tiles = s.n_tiles > 1, ragged = p->n_seqs > 1;
@@ -1233,7 +1237,8 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   DARK_CHECK_ARG(wgs < (1ll << 30), "%s: %lld workgroups", who, (long long)wgs);
   a.n_units = (int)wgs;
   a.max_q = p->max_q;
-  // (not for short ones, which wait for the ranking: 60 x up to 200 over up to 700 83 us, 97 with it; nor for few, split evenly)
+  // (not for short ones, which wait for the ranking: 60 x up to 200 over up to 700 91 us, 106 with it; nor for few, split evenly;
+  // more than 64 sequences, a lane each, begin in the batch's order)
   a.by_length = s.few == 0 && p->n_seqs > 1 && p->n_seqs <= 64 && p->max_kv >= 1024 && (s.n_split == 1 || wgs >= 512 * (int64_t)s.n_split);
 
   a.by_hk = make_div(a.Hk); a.by_tiles = make_div(s.n_tiles); a.by_split = make_div(s.n_split); a.by_group = make_div(a.G);
@@ -1242,7 +1247,7 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
   DARK_CHECK_ARG(jrows < (1ll << 31) - MAX_BLOCKS * 4, "%s: too many rows", who);
   // Units that share memory on one XCD: all heads and row tiles of a part, or else the row tiles of a key head -- where there
   // are enough such groups to even out what they hold, or eight heads that hold the same (16 sequences of up to 512 keys,
-  // 12 heads, fp32: 27.4 us, 30.4 with the sequences dealt out whole).
+  // 12 heads, fp32: 26.3 us, 34.9 with the units dealt out one by one).
   int blocks = s.few == 1 ? (int)((wgs + 3) / 4) : (int)wgs;
   a.n_inner = 1;
   for (const bool all : {true, false}) {
@@ -1301,10 +1306,10 @@ int dark_paged_attention(const dark_paged_attention_args* p, void* stream) {
     DARK_JOIN(float, HDv);                                                              \
   } while (0)
   const int HD = p->kv.head_dim;
-  // NT: keys that, with four layers of them, cannot stay in the 256 MB behind the L2s until they are read again go past the caches (64 x 1 over up
-  // to 16384, 2.5 GB: 399 us, 435 without; head_dim 64: 207 and 234; 113 MB among other layers': 29.3 and 32.2, again and
-  // again: 27.0 and 26.0; 64 x 8 over 2000, one tile of rows: 88.5 us, 98.5 without) -- if their rows are whole 128-byte lines: a line that two rows share is then read twice (head_dim 96:
-  // 365 and 331)
+  // NT: keys that, with four layers of them, cannot stay in the 256 MB behind the L2s until they are read again go past the
+  // caches (64 x 1 over up to 16384, 2.5 GB: 403 us, 439 without; 12 heads of 64: 289 and 326; 64 x 1 over 900, 118 MB, among other
+  // layers': 42.6 and 47.7, again and again 42.0 and 40.1; 64 x 8 over 2000, one tile of rows: 88 us, 99 without) -- if their rows
+  // are whole 128-byte lines (head_dim 96: 604 past them, 543 through them)
   const bool past = HD % 64 == 0 && (int64_t)p->n_seqs * a.cap * p->kv.n_kv_heads * HD * es * 2 > (int64_t)64 << 20;
   // rows of one tile see different keys only where a token's own place bounds them and a tile holds several tokens
   if (p->causal && p->max_q > 1) {

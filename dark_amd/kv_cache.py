@@ -95,7 +95,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``block_table[b]`` (int32, an entry outside the cache leaves its keys out).  Left out are keys whose ``key_mask[b, j]``
     (uint8 or bool) is 0 and, with ``causal``, keys behind the token's own place ``q_index[t]`` (int32; default: the
     sequence's last places).  A token with no key left gets zeros (lse -inf).  ``max_q`` / ``max_kv``: the most new tokens /
-    keys of a sequence.  Tokens that belong to no sequence are not written; ``out`` must not overlap ``q``.  ``scale`` defaults to
+    keys of a sequence.  Tokens that belong to no sequence are not written; ``out`` must not overlap ``q``.  Scores and sums are
+    fp32; in bf16 the softmax weights are rounded to bf16 for the product with the values.  ``scale`` defaults to
     ``head_dim ** -0.5``.  Returns ``out``, or ``(out, lse [T, n_heads] fp32)``."""
     return (_bind or _ops()).paged_attention(_stream(q), q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_kv, q_index,
                                             key_mask, causal, scale, out, return_lse)
@@ -169,7 +170,8 @@ def forward_cached(model, cache: PagedKVCache, input_ids: torch.Tensor, seq: tor
     """The body of a ``DreamModel_length`` for new tokens (``input_ids [T]`` int64, token ``t`` = place ``index[t]`` of sequence
     ``seq[t]``, the tokens of a sequence together as ``cu_q`` says) against ``cache``: their keys and values are written to
     their slots, every new token attends over all ``kv_len`` keys of its sequence (``causal``: up to its own place).
-    ``position_ids [T]`` default to ``index``.  Returns the residual stream ``[T, hidden_size]`` (``out`` if given) for the LM
+    ``position_ids [T]`` default to ``index``.  Rows of tokens that no sequence holds (padding behind ``cu_q[-1]``, ``seq`` -1) are
+    undefined and reach no other row.  Returns the residual stream ``[T, hidden_size]`` (``out`` if given) for the LM
     head."""
     pk = model.packed()
     dev = pk.device

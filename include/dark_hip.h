@@ -426,12 +426,14 @@ int dark_kv_append(const dark_kv_append_args* a, void* stream);
  *   table and (causal) its own index leave; a token for which none is left gets zeros and lse = -inf.
  * Tokens cu_q[b] .. cu_q[b+1]-1 belong to sequence b (cu_q non-decreasing; tokens before cu_q[0] and behind
  * cu_q[n_seqs] are left as they were).  Whatever lies in slots that no key of a token uses -- NaN, infinities -- does not
- * reach its output; scores, softmax statistics and sums are fp32.
+ * reach its output; scores, softmax statistics and sums are fp32; in bf16 a softmax weight is rounded to bf16 before it
+ * multiplies its value (as in the plain forward), and the output once.
  *   q, out [n_tokens, n_heads, head_dim]: strides and alignment as above; out must not overlap q
  *   block_table [n_seqs, table_width] int32, row stride table_stride; an entry outside [0, n_pages) leaves its keys out
  *   kv_len [n_seqs] int32: keys of the sequence, the chunk's own included; clamped to [0, min(max_kv, table_width *
  *     page_size)]
- *   q_index [n_tokens] int32 or NULL = the last tokens of the sequence: kv_len - (new tokens) + i (read if causal only)
+ *   q_index [n_tokens] int32 or NULL = the last tokens of the sequence: kv_len (clamped) - (new tokens) + i (read if
+ *     causal only)
  *   key_mask [n_seqs, >= max_kv] uint8 (0 = left out), row stride mask_stride, or NULL
  *   max_q, max_kv: no sequence has more new tokens / more keys (tokens of a sequence beyond max_q may be left as they
  *     were, keys beyond max_kv are left out)
@@ -460,7 +462,8 @@ int dark_paged_attention(const dark_paged_attention_args* a, void* stream);
  * with some of them, what follows from the others' cached keys and values.
  *   kv: layer 0's cache; layer l's k and v lie layer_stride elements further each.  n_kv_heads must be n_heads.
  *   ids, pos, slots, q_index, hidden: one entry (row) a new token; pos, slots as in dark_kv_append, the rest as in
- *   dark_paged_attention (q, out, lse, workspace and their strides are not read)
+ *   dark_paged_attention (q, out, lse, workspace and their strides are not read).  Rows of tokens of no sequence (before
+ *   cu_q[0], behind cu_q[n_seqs]) are undefined and reach no other row.
  *   hidden [n_tokens, d] m->resid_dtype OUT: the residual stream after the last layer (pre final norm), for
  *   dark_lm_head_rows.  Workspace: dark_forward_cached_workspace_bytes(...) bytes, 256-byte aligned. */
 typedef struct dark_cached_tokens {

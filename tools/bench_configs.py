@@ -4,6 +4,8 @@
   3h DBpedia50 vocabulary (V=25427), B=1024 abd, 32 steps, bf16       (one GPU's share; head NOT vocab-sharded)
   4  N=128 (64 masks/row), 12 layers, 12 heads (hd=64), B=1024/GPU, 32 steps, bf16
   5  RL rollout: T=0.5, top_p=0.9, 32 steps, 4 trajectories per query, B=2048/GPU, bf16 (custom_grpo2.py:605-634)
+  kv the headline's windows with a key / value cache: 512 abduction / deduction windows, 32 steps, bf16, no cache and a whole
+     forward every 1, 2, 4, 8
   wn WN18RR vocabulary (V=41066: the sampler's rows live in the registered workspace), B=1024 abd, 32 steps, bf16
 One JSON line per config: sequences/s and the per-kernel split from HIP events is left to rocprofv3."""
 import argparse
@@ -51,7 +53,7 @@ def main():
         assert out.shape == (ids.shape[0], max_length)
         print(json.dumps({"config": name, "sequences_per_s": round(ids.shape[0] / dt, 1),
                           "ms_per_call": round(dt * 1e3, 1), "batch": ids.shape[0], **{k: v for k, v in kw.items()
-                                                                                       if k in ("steps", "temperature")}}),
+                                                                                       if k in ("steps", "temperature", "cache_interval")}}),
               flush=True)
 
     want = a.configs.split(",")
@@ -70,6 +72,13 @@ def main():
         m = model_for(torch.bfloat16, vocab_size=synth.vocab_size(**synth.WN18RR))
         ids = synth.make_inputs(1024, "abd", seed=1, **synth.WN18RR).to(dev)
         run("WN18RR V=41066 abd B=1024 32 steps bf16 (row-workspace sampler)", m, ids, 46, steps=32, temperature=0.1)
+        del m
+    if "kv" in want:
+        m = model_for(torch.bfloat16, vocab_size=synth.vocab_size(**synth.FB15K237))
+        for mode in ("abd", "ded"):
+            ids = synth.make_inputs(512, mode, seed=1).to(dev)
+            for interval in (0, 1, 2, 4, 8):
+                run(f"kv: FB15k-237 {mode} B=512 32 steps bf16", m, ids, 46, steps=32, temperature=0.1, cache_interval=interval)
         del m
     if "4" in want:
         m = model_for(torch.bfloat16, vocab_size=synth.vocab_size(**synth.FB15K237), num_hidden_layers=12,
